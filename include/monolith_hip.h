@@ -455,6 +455,83 @@ int mono_embedding_to_layout_grad(const mono_layout_slice* h_slices, int n_slice
                                   const float* const* h_out_grads, const int64_t* h_out_floats,
                                   int n_outs, int mean_divides, void* stream);
 
+/* ---- sequence attention and softmax loss over embedding rows ----
+ * No counterpart in the reference's op set. Row types: MONO_ROW_FP32, MONO_ROW_BF16; every sum,
+ * softmax statistic and partial result is fp32. Nothing here allocates or synchronises (safe under
+ * HIP graph capture): scratch is the caller's, sized by the *_workspace function for the same
+ * arguments, and belongs to one call at a time. Ragged rows are given by splits int64[batch + 1],
+ * non-decreasing, inside [0, rows]; rows in front of the first split and behind the last belong to
+ * no sequence (their outputs and gradients are zero). Splits that break this give wrong values, but
+ * no access outside the arrays. Rows are [rows, heads, dim] with the last dimension contiguous. */
+enum { MONO_ROW_FP32 = 0, MONO_ROW_BF16 = 1 };
+typedef struct {
+  const void* ptr;
+  int64_t row_stride, head_stride; /* elements */
+} mono_rows;
+typedef struct {
+  int32_t dtype;                 /* MONO_ROW_* of every rows array */
+  int32_t heads, kv_heads, dim;  /* heads is a multiple of kv_heads; 1 <= dim <= 128 */
+  int32_t causal;                /* a sequence's last query stands at its last key */
+  int32_t kv_shared;             /* backward: value is key, grad_key takes both gradients */
+  int64_t batch, n_query, n_key;
+  mono_rows query, key, value;
+  const int64_t* query_splits;   /* NULL: one query per sequence (n_query == batch) */
+  const int64_t* key_splits;
+  const uint8_t* key_mask;       /* [n_key], 0 = no query sees this key; may be NULL */
+  float scale;                   /* of the products, before the softmax */
+  /* shared prefix (mono_shared_prefix_attention only) */
+  int64_t n_prefix;
+  mono_rows prefix_key, prefix_value;
+  const uint8_t* prefix_mask;
+  /* contiguous [n_query, heads, dim]; lse float[n_query, heads] in units of log 2, written by the
+   * forward (may be NULL there) and read by the backward */
+  void* out;
+  float* lse;
+  /* backward: grad_out like query, the gradients contiguous and shaped like their inputs */
+  mono_rows grad_out;
+  void *grad_query, *grad_key, *grad_value; /* grad_key NULL: the keys' gradients are not wanted */
+  void* workspace;
+  int64_t workspace_bytes;
+} mono_attention_args;
+
+/* out = softmax(scale q k^T) v over every sequence's allowed keys; a query without any gets zeros. */
+int64_t mono_ragged_attention_workspace(const mono_attention_args* args);
+int mono_ragged_attention(const mono_attention_args* args, void* stream);
+/* its gradient: reads out and lse of the forward, recomputes the probabilities */
+int64_t mono_ragged_attention_gradient_workspace(const mono_attention_args* args);
+int mono_ragged_attention_gradient(const mono_attention_args* args, void* stream);
+/* Every query sees the n_prefix prefix rows, which lie in memory once for the whole batch, and the
+ * keys of its own sequence (key_splits NULL: none). */
+int64_t mono_shared_prefix_attention_workspace(const mono_attention_args* args);
+int mono_shared_prefix_attention(const mono_attention_args* args, void* stream);
+
+/* loss[i] = log sum_v exp(l[i, v]) - l[i, label_i], l = scale query rows^T + bias. A label of -1
+ * marks a row without one (loss 0, no gradient), any other label outside [0, vocab) gives a loss of
+ * NaN and no gradient. A bias of -inf takes a candidate out, whatever its row holds; a row whose own
+ * label is taken out has a loss of +inf and no gradient. */
+typedef struct {
+  int32_t dtype, dim;            /* 1 <= dim <= 256 */
+  int64_t n, vocab;
+  const void* query;             /* [n, dim], rows query_stride elements apart */
+  int64_t query_stride;
+  const void* rows;              /* [vocab, dim] */
+  int64_t rows_stride;
+  const int64_t* labels;         /* [n] */
+  const float* bias;             /* [vocab], may be NULL */
+  float scale;
+  float* loss;                   /* [n] */
+  float* lse;                    /* [n], in units of log 2; +inf: the row has no gradient */
+  const float* grad_loss;        /* backward: [n] */
+  void *grad_query, *grad_rows;  /* contiguous, may each be NULL */
+  float* grad_bias;              /* [vocab], may be NULL */
+  void* workspace;
+  int64_t workspace_bytes;
+} mono_softmax_ce_args;
+int64_t mono_softmax_cross_entropy_workspace(const mono_softmax_ce_args* args);
+int mono_softmax_cross_entropy(const mono_softmax_ce_args* args, void* stream);
+int64_t mono_softmax_cross_entropy_gradient_workspace(const mono_softmax_ce_args* args);
+int mono_softmax_cross_entropy_gradient(const mono_softmax_ce_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -36,6 +36,31 @@ class TableCfg(C.Structure):  # mono_table_cfg
               ("feature_evict_every_n_hours", C.c_int32)]
 
 
+class Rows(C.Structure):  # mono_rows
+  _fields_ = [("ptr", C.c_void_p), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class AttentionArgs(C.Structure):  # mono_attention_args
+  _fields_ = [("dtype", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+              ("dim", C.c_int32), ("causal", C.c_int32), ("kv_shared", C.c_int32),
+              ("batch", C.c_int64), ("n_query", C.c_int64), ("n_key", C.c_int64),
+              ("query", Rows), ("key", Rows), ("value", Rows), ("query_splits", C.c_void_p),
+              ("key_splits", C.c_void_p), ("key_mask", C.c_void_p), ("scale", C.c_float),
+              ("n_prefix", C.c_int64), ("prefix_key", Rows), ("prefix_value", Rows),
+              ("prefix_mask", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+              ("grad_out", Rows), ("grad_query", C.c_void_p), ("grad_key", C.c_void_p),
+              ("grad_value", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
+class SoftmaxCeArgs(C.Structure):  # mono_softmax_ce_args
+  _fields_ = [("dtype", C.c_int32), ("dim", C.c_int32), ("n", C.c_int64), ("vocab", C.c_int64),
+              ("query", C.c_void_p), ("query_stride", C.c_int64), ("rows", C.c_void_p),
+              ("rows_stride", C.c_int64), ("labels", C.c_void_p), ("bias", C.c_void_p),
+              ("scale", C.c_float), ("loss", C.c_void_p), ("lse", C.c_void_p),
+              ("grad_loss", C.c_void_p), ("grad_query", C.c_void_p), ("grad_rows", C.c_void_p),
+              ("grad_bias", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
 def _load():
   if not os.path.exists(LIB_PATH):
     raise ImportError(
@@ -44,6 +69,10 @@ def _load():
   lib = C.CDLL(LIB_PATH)
   lib.mono_last_error.restype = C.c_char_p
   lib.mono_fused_reorder_last_plan.restype = C.c_int64
+  for name in ("mono_ragged_attention", "mono_ragged_attention_gradient",
+               "mono_shared_prefix_attention", "mono_softmax_cross_entropy",
+               "mono_softmax_cross_entropy_gradient"):
+    getattr(lib, name + "_workspace").restype = C.c_int64
   return lib
 
 

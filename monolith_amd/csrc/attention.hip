@@ -1,0 +1,789 @@
+// attention.hip — attention over ragged embedding rows: forward, backward, and the form whose
+// batch shares a prefix. The tile scheme is described in seq_dev.h.
+//
+// The query heads of one key head lie side by side as columns of a tile ("virtual rows" token * G +
+// head), so a group's keys are read once for all of its heads and a single token still fills part of
+// a tile. Which sequence a workgroup's tile belongs to is found from the splits on the device, by
+// the rule that sequence b's tiles start at floor(start_b / BM) + b: that leaves every sequence room
+// for ceil(length / BM) tiles, needs no pass over the splits and no copy of them to the host.
+#include <algorithm>
+
+#include "mono_common.h"
+#include "seq_dev.h"
+
+namespace mono {
+namespace {
+using namespace seq;
+
+enum Mode { kSplits = 0, kOnePerSeq = 1, kWhole = 2 };
+
+struct Args {
+  const void *q, *k, *v, *go, *o;
+  int64_t qs, qh, ks, kh, vs, vh, gs, gh;
+  void *out, *dq, *dk, *dv;
+  float *lse, *delta;
+  float *part, *part2, *part_lse;  // split partials
+  const int64_t *qsp, *ksp;
+  const uint8_t* mask;
+  int B, nq, nk, H, Hkv, G, D, qmode, kmode, causal, shared;
+  int nsplit, slot0;
+  float scale, scale2;
+  int vec_q, vec_k, vec_v, vec_g, vec_o;
+};
+
+struct Seg {
+  int lo, n, b;  // first row, rows, sequence (-1: rows of no sequence)
+};
+
+__device__ inline int split_at(const int64_t* sp, int i, int n) {
+  const int64_t s = sp[i];
+  return s < 0 ? 0 : s > n ? n : (int)s;
+}
+
+__device__ inline Seg segment(const int64_t* sp, int mode, int b, int n) {
+  if (mode == kWhole) return {0, n, b};
+  if (mode == kOnePerSeq) return {b, 1, b};
+  const int lo = split_at(sp, b, n), hi = split_at(sp, b + 1, n);
+  return {lo, hi > lo ? hi - lo : 0, b};
+}
+
+// The sequence of tile `tile` (BM virtual rows each, G to a row) and the tile's place in it. Rows in
+// front of the first split and behind the last count as two more sequences.
+__device__ inline Seg find_tile(const int64_t* sp, int mode, int B, int n, int G, int BM, int tile,
+                                int* local) {
+  if (mode == kWhole) {
+    *local = tile;
+    return {0, n, 0};
+  }
+  if (mode == kOnePerSeq) {
+    const int per = (G + BM - 1) / BM;
+    *local = tile % per;
+    return {tile / per, 1, tile / per};
+  }
+  int lo = 0, hi = B + 1;  // segments 0 .. B + 1; segment i starts at start(i)
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    const int64_t start = split_at(sp, mid - 1, n);
+    if ((start * G) / BM + mid <= tile) lo = mid;
+    else hi = mid - 1;
+  }
+  const int start = lo == 0 ? 0 : split_at(sp, lo - 1, n);
+  const int end = lo == B + 1 ? n : split_at(sp, lo, n);
+  *local = tile - (int)(((int64_t)start * G) / BM) - lo;
+  return {start, end > start ? end - start : 0, lo == 0 || lo == B + 1 ? -1 : lo - 1};
+}
+int64_t tiles_for(int mode, int64_t B, int64_t n, int64_t G, int BM) {
+  if (mode == kWhole) return (n * G + BM - 1) / BM;
+  if (mode == kOnePerSeq) return B * ((G + BM - 1) / BM);
+  return n * G / BM + B + 2;
+}
+
+// rows of a streamed tile: one wave alone holds half of what four hold on their way to LDS
+template <typename T, int NW>
+struct Tile {
+  static constexpr int BN = (sizeof(T) == 2 ? 64 : 32) / (NW == 1 ? 2 : 1), NR = BN / 16;
+};
+
+// ---- forward -------------------------------------------------------------------------------
+template <typename T, int DP, int NC, int NW>
+__global__ __launch_bounds__(NW * 64) void k_attn_fwd(Args a) {
+  typedef Mma<T, DP> M;
+  constexpr int BM = NC * NW * 16, BN = Tile<T, NW>::BN, NR = Tile<T, NW>::NR, NT = NW * 64;
+  typedef Stage<T, DP, BN, NT> St;
+  __shared__ __align__(16) T lk[BN * St::LDW];
+  __shared__ __align__(16) T lv[BN * St::LDW];
+  __shared__ __align__(16) uint8_t lm[BN];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int kvh = blockIdx.x % a.Hkv, split = blockIdx.y;
+  int local;
+  const Seg sq = find_tile(a.qsp, a.qmode, a.B, a.nq, a.G, BM, blockIdx.x / a.Hkv, &local);
+  const int64_t nrow = (int64_t)sq.n * a.G;
+  const int64_t r0 = (int64_t)local * BM;
+  if (r0 >= nrow) return;
+  Seg sk = {0, 0, -1};
+  if (sq.b >= 0) sk = segment(a.ksp, a.kmode, sq.b, a.nk);
+  // every column's row, and the keys it sees: [0, klim) of its sequence
+  int tok[NC], head[NC], klim[NC];
+  bool ok[NC];
+  typename M::Frag qf[NC][M::KF];
+  int kmin = sk.n;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int64_t r = r0 + (wave * NC + c) * 16 + (lane & 15);
+    ok[c] = r < nrow;
+    tok[c] = ok[c] ? (int)(r / a.G) : 0;
+    head[c] = kvh * a.G + (ok[c] ? (int)(r % a.G) : 0);
+    int lim = sk.n;
+    if (a.causal) lim = min(lim, max(0, tok[c] + 1 + sk.n - sq.n));
+    klim[c] = ok[c] ? lim : 0;
+    if (ok[c]) kmin = min(kmin, lim);
+    M::load_cols(qf[c], (const T*)a.q + (int64_t)(sq.lo + tok[c]) * a.qs + (int64_t)head[c] * a.qh, ok[c],
+                 a.D, a.vec_q, lane);
+  }
+#pragma unroll
+  for (int x = 8; x; x >>= 1) kmin = min(kmin, __shfl_xor(kmin, x));
+  int kend = sk.n;
+  if (a.causal) {
+    const int last = (int)((min(r0 + BM, nrow) - 1) / a.G);
+    kend = min(kend, max(0, last + 1 + sk.n - sq.n));
+  }
+  int kbeg = 0;
+  if (a.nsplit > 1) {
+    const int chunk = ((kend + a.nsplit - 1) / a.nsplit + BN - 1) / BN * BN;
+    kbeg = min(kend, split * chunk);
+    kend = min(kend, kbeg + chunk);
+  }
+  const T* kb = (const T*)a.k + (int64_t)sk.lo * a.ks + (int64_t)kvh * a.kh;
+  const T* vb = (const T*)a.v + (int64_t)sk.lo * a.vs + (int64_t)kvh * a.vh;
+  const uint8_t* mb = a.mask ? a.mask + sk.lo : nullptr;
+
+  f4 acc[M::NDT][NC];
+  float m[NC], l[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    m[c] = neg_inf();
+    l[c] = 0.f;
+#pragma unroll
+    for (int d = 0; d < M::NDT; ++d) acc[d][c] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  St stk, stv;
+  uint8_t mk = 0;
+  auto fetch = [&](int y0) {
+    const auto alive = [&](int row) { return !mb || mb[row]; };
+    stk.load(kb, a.ks, y0, kend, a.D, a.vec_k, tid, alive);
+    stv.load(vb, a.vs, y0, kend, a.D, a.vec_v, tid, alive);
+    if (mb && tid < BN) mk = y0 + tid < kend ? mb[y0 + tid] : 0;
+  };
+  if (kbeg < kend) fetch(kbeg);
+  for (int y0 = kbeg; y0 < kend; y0 += BN) {
+    __syncthreads();
+    stk.store(lk, tid);
+    stv.store(lv, tid);
+    if (mb && tid < BN) lm[tid] = mk;
+    __syncthreads();
+    if (y0 + BN < kend) fetch(y0 + BN);
+    f4 s[NR][NC];
+#pragma unroll
+    for (int rt = 0; rt < NR; ++rt) M::template scores<NC>(lk, rt, qf, s[rt], lane);
+    const bool need = mb || y0 + BN > min(kmin, kend);
+    if (need) {
+#pragma unroll
+      for (int rt = 0; rt < NR; ++rt) {
+        const int y = 16 * rt + 4 * (lane >> 4);
+        const uint32_t bytes = mb ? *(const uint32_t*)(lm + y) : 0x01010101u;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+            s[rt][c][r] = (y0 + y + r < min(klim[c], kend) && ((bytes >> (8 * r)) & 0xff))
+                              ? s[rt][c][r] * a.scale2 : neg_inf();
+      }
+    } else {
+#pragma unroll
+      for (int rt = 0; rt < NR; ++rt)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) s[rt][c] *= a.scale2;
+    }
+    float alpha[NC];
+    bool moved = false;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      float mx = neg_inf();
+#pragma unroll
+      for (int rt = 0; rt < NR; ++rt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[rt][c][r]);
+      mx = fmaxf(m[c], col_max(mx));
+      const float base = mx == neg_inf() ? 0.f : mx;
+      alpha[c] = exp2_hw(m[c] - base);
+      moved |= mx != m[c];
+      m[c] = mx;
+      float sum = 0.f;
+#pragma unroll
+      for (int rt = 0; rt < NR; ++rt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float p = exp2_hw(s[rt][c][r] - base);
+          s[rt][c][r] = p;
+          sum += p;
+        }
+      l[c] = fmaf(l[c], alpha[c], sum);
+    }
+    if (__any(moved)) {
+#pragma unroll
+      for (int d = 0; d < M::NDT; ++d)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) acc[d][c] *= alpha[c];
+    }
+    M::template accumulate<NC, NR>(lv, s, acc, lane);
+  }
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const float lt = col_sum(l[c]);
+    const float inv = lt == 0.f ? 0.f : 1.f / lt;
+    const float lse = lt == 0.f ? neg_inf() : m[c] + __log2f(lt);
+    if (!ok[c]) continue;
+    const int64_t row = (int64_t)(sq.lo + tok[c]) * a.H + head[c];
+    if (a.part) {
+      const int64_t at = (int64_t)(a.slot0 + split) * a.nq * a.H + row;
+      if (lane < 16) a.part_lse[at] = lse;
+#pragma unroll
+      for (int d = 0; d < M::NDT; ++d)
+        store4(a.part + at * a.D, 16 * d + 4 * (lane >> 4), a.D, acc[d][c] * inv, a.vec_o);
+    } else {
+      if (a.lse && lane < 16) a.lse[row] = lse;
+#pragma unroll
+      for (int d = 0; d < M::NDT; ++d)
+        store4((T*)a.out + row * a.D, 16 * d + 4 * (lane >> 4), a.D, acc[d][c] * inv, a.vec_o);
+    }
+  }
+}
+
+// out = sum of the splits' results, each weighted by its share of the softmax's sum
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_join(const float* part, const float* part_lse, int n_part,
+                                                   int64_t rows, int D, T* out, float* lse) {
+  const int64_t total = rows * D;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / D;
+    float m = neg_inf();
+    for (int s = 0; s < n_part; ++s) m = fmaxf(m, part_lse[(int64_t)s * rows + row]);
+    float z = 0.f, t = 0.f;
+    for (int s = 0; s < n_part; ++s) {
+      const float e = part_lse[(int64_t)s * rows + row];
+      if (e == neg_inf()) continue;  // a split without a key: nothing was summed
+      const float w = exp2_hw(e - m);
+      z += w;
+      t = fmaf(w, part[(int64_t)s * total + i], t);
+    }
+    out[i] = (T)(z == 0.f ? 0.f : t / z);
+    if (lse && i % D == 0) lse[row] = z == 0.f ? neg_inf() : m + __log2f(z);
+  }
+}
+
+// ---- backward ------------------------------------------------------------------------------
+// dQ: the forward's tiles again. With p = exp2(s - lse) from the forward's statistics and
+// delta = g.o, ds = p (g.v - delta), dq = scale sum ds k. Also writes delta for the pass over keys.
+template <typename T, int DP, int NC, int NW>
+__global__ __launch_bounds__(NW * 64) void k_attn_dq(Args a) {
+  typedef Mma<T, DP> M;
+  constexpr int BM = NC * NW * 16, BN = Tile<T, NW>::BN, NR = Tile<T, NW>::NR, NT = NW * 64;
+  typedef Stage<T, DP, BN, NT> St;
+  __shared__ __align__(16) T lk[BN * St::LDW];
+  __shared__ __align__(16) T lv[BN * St::LDW];
+  __shared__ __align__(16) uint8_t lm[BN];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int kvh = blockIdx.x % a.Hkv, split = blockIdx.y;
+  int local;
+  const Seg sq = find_tile(a.qsp, a.qmode, a.B, a.nq, a.G, BM, blockIdx.x / a.Hkv, &local);
+  const int64_t nrow = (int64_t)sq.n * a.G;
+  const int64_t r0 = (int64_t)local * BM;
+  if (r0 >= nrow) return;
+  Seg sk = {0, 0, -1};
+  if (sq.b >= 0) sk = segment(a.ksp, a.kmode, sq.b, a.nk);
+  int tok[NC], head[NC], klim[NC];
+  bool ok[NC];
+  float lse[NC], delta[NC];
+  typename M::Frag qf[NC][M::KF], gf[NC][M::KF];
+  int kmin = sk.n;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int64_t r = r0 + (wave * NC + c) * 16 + (lane & 15);
+    ok[c] = r < nrow;
+    tok[c] = ok[c] ? (int)(r / a.G) : 0;
+    head[c] = kvh * a.G + (ok[c] ? (int)(r % a.G) : 0);
+    int lim = sk.n;
+    if (a.causal) lim = min(lim, max(0, tok[c] + 1 + sk.n - sq.n));
+    klim[c] = ok[c] ? lim : 0;
+    if (ok[c]) kmin = min(kmin, lim);
+    const int64_t t = sq.lo + tok[c], row = t * a.H + head[c];
+    M::load_cols(qf[c], (const T*)a.q + t * a.qs + (int64_t)head[c] * a.qh, ok[c], a.D, a.vec_q, lane);
+    M::load_cols(gf[c], (const T*)a.go + t * a.gs + (int64_t)head[c] * a.gh, ok[c], a.D, a.vec_g, lane);
+    typename M::Frag of[M::KF];
+    M::load_cols(of, (const T*)a.o + row * a.D, ok[c], a.D, a.vec_o, lane);
+    delta[c] = col_sum(M::dot(gf[c], of));
+    const float e = ok[c] ? a.lse[row] : neg_inf();
+    lse[c] = e == neg_inf() ? __builtin_inff() : e;  // a row without keys: every weight is 0
+    if (ok[c] && lane < 16 && split == 0) a.delta[row] = delta[c];
+  }
+#pragma unroll
+  for (int x = 8; x; x >>= 1) kmin = min(kmin, __shfl_xor(kmin, x));
+  int kend = sk.n;
+  if (a.causal) {
+    const int last = (int)((min(r0 + BM, nrow) - 1) / a.G);
+    kend = min(kend, max(0, last + 1 + sk.n - sq.n));
+  }
+  int kbeg = 0;
+  if (a.nsplit > 1) {
+    const int chunk = ((kend + a.nsplit - 1) / a.nsplit + BN - 1) / BN * BN;
+    kbeg = min(kend, split * chunk);
+    kend = min(kend, kbeg + chunk);
+  }
+  const T* kb = (const T*)a.k + (int64_t)sk.lo * a.ks + (int64_t)kvh * a.kh;
+  const T* vb = (const T*)a.v + (int64_t)sk.lo * a.vs + (int64_t)kvh * a.vh;
+  const uint8_t* mb = a.mask ? a.mask + sk.lo : nullptr;
+  f4 acc[M::NDT][NC];
+#pragma unroll
+  for (int d = 0; d < M::NDT; ++d)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc[d][c] = f4{0.f, 0.f, 0.f, 0.f};
+  St stk, stv;
+  uint8_t mk = 0;
+  auto fetch = [&](int y0) {
+    const auto alive = [&](int row) { return !mb || mb[row]; };
+    stk.load(kb, a.ks, y0, kend, a.D, a.vec_k, tid, alive);
+    stv.load(vb, a.vs, y0, kend, a.D, a.vec_v, tid, alive);
+    if (mb && tid < BN) mk = y0 + tid < kend ? mb[y0 + tid] : 0;
+  };
+  if (kbeg < kend) fetch(kbeg);
+  for (int y0 = kbeg; y0 < kend; y0 += BN) {
+    __syncthreads();
+    stk.store(lk, tid);
+    stv.store(lv, tid);
+    if (mb && tid < BN) lm[tid] = mk;
+    __syncthreads();
+    if (y0 + BN < kend) fetch(y0 + BN);
+    f4 s[NR][NC];
+    const bool need = mb || y0 + BN > min(kmin, kend);
+#pragma unroll
+    for (int rt = 0; rt < NR; ++rt) {
+      f4 dp[NC];
+      M::template scores<NC>(lk, rt, qf, s[rt], lane);
+      M::template scores<NC>(lv, rt, gf, dp, lane);
+      const int y = 16 * rt + 4 * (lane >> 4);
+      const uint32_t bytes = mb ? *(const uint32_t*)(lm + y) : 0x01010101u;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float p = exp2_hw(fmaf(s[rt][c][r], a.scale2, -lse[c]));
+          if (need && !(y0 + y + r < min(klim[c], kend) && ((bytes >> (8 * r)) & 0xff))) p = 0.f;
+          s[rt][c][r] = p * (dp[c][r] - delta[c]);
+        }
+    }
+    M::template accumulate<NC, NR>(lk, s, acc, lane);
+  }
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    if (!ok[c]) continue;
+    const int64_t row = (int64_t)(sq.lo + tok[c]) * a.H + head[c];
+    if (a.part) {
+      const int64_t at = (int64_t)split * a.nq * a.H + row;
+#pragma unroll
+      for (int d = 0; d < M::NDT; ++d)
+        store4(a.part + at * a.D, 16 * d + 4 * (lane >> 4), a.D, acc[d][c] * a.scale, a.vec_o);
+    } else {
+#pragma unroll
+      for (int d = 0; d < M::NDT; ++d)
+        store4((T*)a.dq + row * a.D, 16 * d + 4 * (lane >> 4), a.D, acc[d][c] * a.scale, a.vec_o);
+    }
+  }
+}
+
+// dK, dV: a tile of keys keeps its sums while the queries of its sequence stream by, the heads of
+// the group one after the other, so a shared key head's gradient is one sum in one order.
+template <typename T, int DP, int NC, int NW>
+__global__ __launch_bounds__(NW * 64) void k_attn_dkv(Args a) {
+  typedef Mma<T, DP> M;
+  constexpr int BM = NC * NW * 16, BN = Tile<T, NW>::BN, NR = Tile<T, NW>::NR, NT = NW * 64;
+  typedef Stage<T, DP, BN, NT> St;
+  __shared__ __align__(16) T lq[BN * St::LDW];
+  __shared__ __align__(16) T lg[BN * St::LDW];
+  __shared__ __align__(16) float ll[BN], ld[BN];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int kvh = blockIdx.x % a.Hkv, split = blockIdx.y;
+  int local;
+  const Seg sk = find_tile(a.ksp, a.kmode, a.B, a.nk, 1, BM, blockIdx.x / a.Hkv, &local);
+  const int j0 = local * BM;
+  if (j0 >= sk.n) return;
+  Seg sq = {0, 0, -1};
+  if (sk.b >= 0) sq = segment(a.qsp, a.qmode, sk.b, a.nq);
+  // every column's key, and the queries that see it: [qlim, n) of its sequence
+  int qlim[NC], key[NC];
+  bool ok[NC];
+  typename M::Frag kf[NC][M::KF], vf[NC][M::KF];
+  int qmax = 0;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int j = j0 + (wave * NC + c) * 16 + (lane & 15);
+    ok[c] = j < sk.n;
+    key[c] = sk.lo + (ok[c] ? j : 0);
+    const bool seen = ok[c] && (!a.mask || a.mask[key[c]]);
+    qlim[c] = seen ? (a.causal ? max(0, j - (sk.n - sq.n)) : 0) : 0x7fffffff;
+    if (ok[c]) qmax = max(qmax, qlim[c]);
+    M::load_cols(kf[c], (const T*)a.k + (int64_t)key[c] * a.ks + (int64_t)kvh * a.kh, seen, a.D, a.vec_k, lane);
+    M::load_cols(vf[c], (const T*)a.v + (int64_t)key[c] * a.vs + (int64_t)kvh * a.vh, seen, a.D, a.vec_v, lane);
+  }
+#pragma unroll
+  for (int x = 8; x; x >>= 1) qmax = max(qmax, __shfl_xor(qmax, x));
+  f4 ak[M::NDT][NC], av[M::NDT][NC];
+#pragma unroll
+  for (int d = 0; d < M::NDT; ++d)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) ak[d][c] = av[d][c] = f4{0.f, 0.f, 0.f, 0.f};
+  // tiles of queries, head after head
+  const int tfirst = a.causal ? max(0, j0 - (sk.n - sq.n)) / BN : 0;
+  const int nt = max(0, (sq.n + BN - 1) / BN - tfirst);
+  int64_t ibeg = 0, iend = (int64_t)nt * a.G;
+  if (a.nsplit > 1) {
+    const int64_t chunk = (iend + a.nsplit - 1) / a.nsplit;
+    ibeg = min(iend, split * chunk);
+    iend = min(iend, ibeg + chunk);
+  }
+  St stq, stg;
+  float el = 0.f, ed = 0.f;
+  auto fetch = [&](int64_t it) {
+    const auto all = [](int) { return true; };
+    const int head = kvh * a.G + (int)(it / nt), y0 = (int)(tfirst + it % nt) * BN;
+    stq.load((const T*)a.q + (int64_t)sq.lo * a.qs + (int64_t)head * a.qh, a.qs, y0, sq.n, a.D, a.vec_q,
+             tid, all);
+    stg.load((const T*)a.go + (int64_t)sq.lo * a.gs + (int64_t)head * a.gh, a.gs, y0, sq.n, a.D, a.vec_g,
+             tid, all);
+    if (tid < BN) {
+      el = __builtin_inff();
+      ed = 0.f;
+      if (y0 + tid < sq.n) {
+        const int64_t row = (int64_t)(sq.lo + y0 + tid) * a.H + head;
+        const float e = a.lse[row];
+        if (e != neg_inf()) {
+          el = e;
+          ed = a.delta[row];
+        }
+      }
+    }
+  };
+  if (ibeg < iend) fetch(ibeg);
+  for (int64_t it = ibeg; it < iend; ++it) {
+    __syncthreads();
+    stq.store(lq, tid);
+    stg.store(lg, tid);
+    if (tid < BN) {
+      ll[tid] = el;
+      ld[tid] = ed;
+    }
+    __syncthreads();
+    const int y0 = (int)(tfirst + it % nt) * BN;
+    if (it + 1 < iend) fetch(it + 1);
+    f4 p[NR][NC], ds[NR][NC];
+    const bool need = y0 < qmax;
+#pragma unroll
+    for (int rt = 0; rt < NR; ++rt) {
+      M::template scores<NC>(lq, rt, kf, p[rt], lane);
+      M::template scores<NC>(lg, rt, vf, ds[rt], lane);
+      const int y = 16 * rt + 4 * (lane >> 4);
+      const f4 e = *(const f4*)(ll + y), dl = *(const f4*)(ld + y);
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float w = exp2_hw(fmaf(p[rt][c][r], a.scale2, -e[r]));
+          if (need && y0 + y + r < qlim[c]) w = 0.f;
+          p[rt][c][r] = w;
+          ds[rt][c][r] = w * (ds[rt][c][r] - dl[r]);
+        }
+    }
+    M::template accumulate<NC, NR>(lg, p, av, lane);
+    M::template accumulate<NC, NR>(lq, ds, ak, lane);
+  }
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    if (!ok[c]) continue;
+    const int64_t row = (int64_t)key[c] * a.Hkv + kvh;
+#pragma unroll
+    for (int d = 0; d < M::NDT; ++d) {
+      const int d0 = 16 * d + 4 * (lane >> 4);
+      f4 dk = ak[d][c] * a.scale;
+      if (a.shared) dk += av[d][c];
+      if (a.part) {
+        const int64_t at = ((int64_t)split * a.nk * a.Hkv + row) * a.D;
+        store4(a.part + at, d0, a.D, dk, a.vec_o);
+        if (!a.shared) store4(a.part2 + at, d0, a.D, av[d][c], a.vec_o);
+      } else {
+        store4((T*)a.dk + row * a.D, d0, a.D, dk, a.vec_o);
+        if (!a.shared) store4((T*)a.dv + row * a.D, d0, a.D, av[d][c], a.vec_o);
+      }
+    }
+  }
+}
+
+// out = the splits' partial sums, first to last
+template <typename T>
+__global__ __launch_bounds__(256) void k_sum_parts(const float* part, int n_part, int64_t total, T* out) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    float t = 0.f;
+    for (int s = 0; s < n_part; ++s) t += part[(int64_t)s * total + i];
+    out[i] = (T)t;
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------
+struct Shape {
+  int nc, nw, bm;
+};
+// Short sequences (32 rows of a key head or fewer on average) leave most of a 64- or 128-row tile
+// empty: one wave with 16 columns per workgroup then.
+Shape shape_for(int dtype, double rows_per_seq) {
+  if (rows_per_seq <= 32) return {1, 1, 16};
+  const int nc = dtype == MONO_ROW_BF16 ? 2 : 1;
+  return {nc, 4, nc * 64};
+}
+// Workgroups that fill the card some times over: few tiles are split along the streamed axis, down
+// to pieces of `least` rows.
+int splits_for(int64_t tiles, int nw, double stream_rows, int least) {
+  const int64_t want = nw == 1 ? 256 * 12 : 256 * 3;
+  if (tiles <= 0 || tiles >= want) return 1;
+  const int64_t by_len = (int64_t)(stream_rows / least);
+  int64_t n = std::min((want + tiles - 1) / tiles, by_len);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(n, 256));
+}
+
+bool aligned_rows(const mono_rows& r, int dtype, int D) {
+  const int e = dtype == MONO_ROW_BF16 ? 8 : 4;
+  return D % e == 0 && r.row_stride % e == 0 && r.head_stride % e == 0 && ((uintptr_t)r.ptr & 15) == 0;
+}
+
+int check(const mono_attention_args* p, const char* who) {
+  MONO_REQUIRE(p != nullptr, "%s: args is NULL", who);
+  MONO_REQUIRE(p->dtype == MONO_ROW_FP32 || p->dtype == MONO_ROW_BF16, "%s: unknown row type %d", who, p->dtype);
+  MONO_REQUIRE(p->dim >= 1 && p->dim <= 128, "%s: dim must be in [1, 128], got %d", who, p->dim);
+  MONO_REQUIRE(p->heads >= 1 && p->kv_heads >= 1 && p->heads % p->kv_heads == 0,
+               "%s: heads (%d) must be a positive multiple of kv_heads (%d)", who, p->heads, p->kv_heads);
+  MONO_REQUIRE(p->batch >= 0 && p->n_query >= 0 && p->n_key >= 0 && p->n_prefix >= 0, "%s: negative size", who);
+  MONO_REQUIRE(p->n_query * p->heads < (1LL << 31) && p->n_key * p->kv_heads < (1LL << 31) &&
+                   p->n_prefix * p->kv_heads < (1LL << 31) && p->batch * p->kv_heads < (1LL << 31),
+               "%s: more than 2^31 rows", who);
+  MONO_REQUIRE(p->query_splits || p->n_query == p->batch,
+               "%s: without query_splits there is one query per sequence (n_query %lld, batch %lld)", who,
+               (long long)p->n_query, (long long)p->batch);
+  return 0;
+}
+
+Args base_args(const mono_attention_args* p) {
+  Args a{};
+  a.q = p->query.ptr, a.qs = p->query.row_stride, a.qh = p->query.head_stride;
+  a.k = p->key.ptr, a.ks = p->key.row_stride, a.kh = p->key.head_stride;
+  a.v = p->value.ptr, a.vs = p->value.row_stride, a.vh = p->value.head_stride;
+  a.go = p->grad_out.ptr, a.gs = p->grad_out.row_stride, a.gh = p->grad_out.head_stride;
+  a.o = p->out, a.out = p->out, a.lse = p->lse;
+  a.dq = p->grad_query, a.dk = p->grad_key, a.dv = p->grad_value;
+  a.qsp = p->query_splits, a.ksp = p->key_splits, a.mask = p->key_mask;
+  a.B = (int)p->batch, a.nq = (int)p->n_query, a.nk = (int)p->n_key;
+  a.H = p->heads, a.Hkv = p->kv_heads, a.G = p->heads / p->kv_heads, a.D = p->dim;
+  a.qmode = p->query_splits ? kSplits : kOnePerSeq;
+  a.kmode = kSplits;
+  a.causal = p->causal, a.shared = p->kv_shared;
+  a.nsplit = 1;
+  a.scale = p->scale, a.scale2 = p->scale * kLog2e;
+  a.vec_q = aligned_rows(p->query, p->dtype, p->dim);
+  a.vec_k = aligned_rows(p->key, p->dtype, p->dim);
+  a.vec_v = aligned_rows(p->value, p->dtype, p->dim);
+  a.vec_g = aligned_rows(p->grad_out, p->dtype, p->dim);
+  a.vec_o = p->dim % (p->dtype == MONO_ROW_BF16 ? 8 : 4) == 0 && (((uintptr_t)p->out | (uintptr_t)p->grad_query |
+             (uintptr_t)p->grad_key | (uintptr_t)p->grad_value) & 15) == 0;
+  return a;
+}
+
+// how one kernel's work is cut
+struct Plan {
+  Shape sh;
+  int64_t tiles;
+  int nsplit;
+};
+Plan plan_tiles(int dtype, int mode, int64_t B, int64_t n, int64_t G, int64_t heads, double stream_rows) {
+  Plan pl;
+  const double per = mode == kWhole ? (double)n * G : (double)n * G / std::max<int64_t>(1, B);
+  pl.sh = shape_for(dtype, per);
+  pl.tiles = tiles_for(mode, B, n, G, pl.sh.bm);
+  pl.nsplit = splits_for(pl.tiles * heads, pl.sh.nw, stream_rows, 256);
+  return pl;
+}
+double average(int64_t n, int64_t B) { return (double)n / std::max<int64_t>(1, B); }
+
+Plan plan_fwd(const mono_attention_args* p) {
+  return plan_tiles(p->dtype, p->query_splits ? kSplits : kOnePerSeq, p->batch, p->n_query,
+                    p->heads / p->kv_heads, p->kv_heads, average(p->n_key, p->batch));
+}
+Plan plan_dkv(const mono_attention_args* p) {
+  return plan_tiles(p->dtype, kSplits, p->batch, p->n_key, 1, p->kv_heads,
+                    average(p->n_query, p->batch) * (p->heads / p->kv_heads));
+}
+
+enum Which { kFwd, kDq, kDkv };
+template <int W, typename T, int DP, int NC, int NW>
+int launch1(const Args& a, const Plan& pl, hipStream_t st) {
+  const dim3 grid((unsigned)(pl.tiles * a.Hkv), (unsigned)a.nsplit);
+  if (W == kFwd) k_attn_fwd<T, DP, NC, NW><<<grid, NW * 64, 0, st>>>(a);
+  else if (W == kDq) k_attn_dq<T, DP, NC, NW><<<grid, NW * 64, 0, st>>>(a);
+  else k_attn_dkv<T, DP, NC, NW><<<grid, NW * 64, 0, st>>>(a);
+  MONO_HIP(hipGetLastError());
+  return 0;
+}
+template <int W, typename T, int DP>
+int launch2(const Args& a, const Plan& pl, hipStream_t st) {
+  if (pl.tiles * a.Hkv == 0) return 0;
+  MONO_REQUIRE(pl.tiles * a.Hkv < (1LL << 31), "attention: too many tiles");
+  if (pl.sh.nw == 1) return launch1<W, T, DP, 1, 1>(a, pl, st);
+  return launch1<W, T, DP, sizeof(T) == 2 ? 2 : 1, 4>(a, pl, st);
+}
+template <int W>
+int launch(int dtype, const Args& a, const Plan& pl, hipStream_t st) {
+  if (dtype == MONO_ROW_BF16) {
+    if (a.D <= 32) return launch2<W, bf16, 32>(a, pl, st);
+    if (a.D <= 64) return launch2<W, bf16, 64>(a, pl, st);
+    return launch2<W, bf16, 128>(a, pl, st);
+  }
+  if (a.D <= 16) return launch2<W, float, 16>(a, pl, st);
+  if (a.D <= 32) return launch2<W, float, 32>(a, pl, st);
+  if (a.D <= 64) return launch2<W, float, 64>(a, pl, st);
+  return launch2<W, float, 128>(a, pl, st);
+}
+
+int64_t round16(int64_t b) { return (b + 15) & ~(int64_t)15; }
+int64_t parts_bytes(int64_t n_part, int64_t rows, int64_t D) {
+  return n_part <= 1 ? 0 : round16(n_part * rows * D * 4) + round16(n_part * rows * 4);
+}
+
+int join(const mono_attention_args* p, const float* part, const float* part_lse, int n_part, hipStream_t st) {
+  const int64_t rows = p->n_query * p->heads;
+  if (rows == 0) return 0;
+  const int grid = grid_for(rows * p->dim, 256);
+  if (p->dtype == MONO_ROW_BF16)
+    k_attn_join<bf16><<<grid, 256, 0, st>>>(part, part_lse, n_part, rows, p->dim, (bf16*)p->out, p->lse);
+  else
+    k_attn_join<float><<<grid, 256, 0, st>>>(part, part_lse, n_part, rows, p->dim, (float*)p->out, p->lse);
+  MONO_HIP(hipGetLastError());
+  return 0;
+}
+int sum_parts(int dtype, const float* part, int n_part, int64_t total, void* out, hipStream_t st) {
+  if (total == 0) return 0;
+  const int grid = grid_for(total, 256);
+  if (dtype == MONO_ROW_BF16) k_sum_parts<bf16><<<grid, 256, 0, st>>>(part, n_part, total, (bf16*)out);
+  else k_sum_parts<float><<<grid, 256, 0, st>>>(part, n_part, total, (float*)out);
+  MONO_HIP(hipGetLastError());
+  return 0;
+}
+
+// the two launches of the shared prefix: over the prefix, where the whole batch is one sequence, and
+// over every sequence's own keys
+struct PrefixPlan {
+  Plan pre, own;
+  int slots;
+};
+PrefixPlan plan_prefix(const mono_attention_args* p) {
+  PrefixPlan r;
+  const int64_t G = p->heads / p->kv_heads;
+  r.pre = plan_tiles(p->dtype, kWhole, 1, p->n_query, G, p->kv_heads, (double)p->n_prefix);
+  r.slots = r.pre.nsplit;
+  if (p->key_splits) {
+    r.own = plan_fwd(p);
+    r.slots += r.own.nsplit;
+  }
+  return r;
+}
+}  // namespace
+}  // namespace mono
+
+extern "C" {
+using namespace mono;
+
+int64_t mono_ragged_attention_workspace(const mono_attention_args* p) {
+  if (check(p, "mono_ragged_attention_workspace")) return -1;
+  return parts_bytes(plan_fwd(p).nsplit, p->n_query * p->heads, p->dim);
+}
+
+int mono_ragged_attention(const mono_attention_args* p, void* stream) {
+  MONO_TRY(check(p, "mono_ragged_attention"));
+  MONO_REQUIRE(p->key_splits, "mono_ragged_attention: key_splits is NULL");
+  if (p->n_query == 0) return 0;
+  const Plan pl = plan_fwd(p);
+  const int64_t rows = p->n_query * p->heads;
+  MONO_REQUIRE(p->workspace_bytes >= parts_bytes(pl.nsplit, rows, p->dim),
+               "mono_ragged_attention: workspace of %lld bytes is too small", (long long)p->workspace_bytes);
+  Args a = base_args(p);
+  a.nsplit = pl.nsplit;
+  if (pl.nsplit > 1) {
+    a.part = (float*)p->workspace;
+    a.part_lse = (float*)((char*)p->workspace + round16(pl.nsplit * rows * p->dim * 4));
+  }
+  MONO_TRY(launch<kFwd>(p->dtype, a, pl, (hipStream_t)stream));
+  return pl.nsplit > 1 ? join(p, a.part, a.part_lse, pl.nsplit, (hipStream_t)stream) : 0;
+}
+
+int64_t mono_ragged_attention_gradient_workspace(const mono_attention_args* p) {
+  if (check(p, "mono_ragged_attention_gradient_workspace")) return -1;
+  const Plan q = plan_fwd(p), k = plan_dkv(p);
+  const int64_t nk = p->n_key * p->kv_heads;
+  return round16(p->n_query * p->heads * 4) +
+         std::max(parts_bytes(q.nsplit, p->n_query * p->heads, p->dim),
+                  k.nsplit <= 1 ? 0 : 2 * round16(k.nsplit * nk * p->dim * 4));
+}
+
+int mono_ragged_attention_gradient(const mono_attention_args* p, void* stream) {
+  MONO_TRY(check(p, "mono_ragged_attention_gradient"));
+  MONO_REQUIRE(p->key_splits, "mono_ragged_attention_gradient: key_splits is NULL");
+  MONO_REQUIRE(!p->grad_key || p->kv_shared || p->grad_value,
+               "mono_ragged_attention_gradient: grad_value is NULL");
+  MONO_REQUIRE(p->workspace_bytes >= mono_ragged_attention_gradient_workspace(p),
+               "mono_ragged_attention_gradient: workspace of %lld bytes is too small",
+               (long long)p->workspace_bytes);
+  hipStream_t st = (hipStream_t)stream;
+  const Plan plq = plan_fwd(p), plk = plan_dkv(p);
+  const int64_t rows = p->n_query * p->heads, krows = p->n_key * p->kv_heads;
+  float* scratch = (float*)((char*)p->workspace + round16(rows * 4));
+  Args a = base_args(p);
+  a.delta = (float*)p->workspace;
+  a.nsplit = plq.nsplit;
+  a.part = plq.nsplit > 1 ? scratch : nullptr;
+  MONO_TRY(launch<kDq>(p->dtype, a, plq, st));
+  if (a.part) MONO_TRY(sum_parts(p->dtype, a.part, plq.nsplit, rows * p->dim, p->grad_query, st));
+  if (!p->grad_key) return 0;
+  a.nsplit = plk.nsplit;
+  a.part = plk.nsplit > 1 ? scratch : nullptr;
+  a.part2 = a.part ? (float*)((char*)scratch + round16(plk.nsplit * krows * p->dim * 4)) : nullptr;
+  MONO_TRY(launch<kDkv>(p->dtype, a, plk, st));
+  if (a.part) {
+    MONO_TRY(sum_parts(p->dtype, a.part, plk.nsplit, krows * p->dim, p->grad_key, st));
+    if (!p->kv_shared) MONO_TRY(sum_parts(p->dtype, a.part2, plk.nsplit, krows * p->dim, p->grad_value, st));
+  }
+  return 0;
+}
+
+int64_t mono_shared_prefix_attention_workspace(const mono_attention_args* p) {
+  if (check(p, "mono_shared_prefix_attention_workspace")) return -1;
+  return parts_bytes(plan_prefix(p).slots, p->n_query * p->heads, p->dim);
+}
+
+int mono_shared_prefix_attention(const mono_attention_args* p, void* stream) {
+  MONO_TRY(check(p, "mono_shared_prefix_attention"));
+  if (p->n_query == 0) return 0;
+  const PrefixPlan pl = plan_prefix(p);
+  const int64_t rows = p->n_query * p->heads;
+  MONO_REQUIRE(p->workspace_bytes >= parts_bytes(pl.slots, rows, p->dim),
+               "mono_shared_prefix_attention: workspace of %lld bytes is too small",
+               (long long)p->workspace_bytes);
+  hipStream_t st = (hipStream_t)stream;
+  Args a = base_args(p);
+  if (pl.slots > 1) {
+    a.part = (float*)p->workspace;
+    a.part_lse = (float*)((char*)p->workspace + round16(pl.slots * rows * p->dim * 4));
+  }
+  if (p->key_splits) {
+    a.nsplit = pl.own.nsplit;
+    a.slot0 = pl.pre.nsplit;
+    MONO_TRY(launch<kFwd>(p->dtype, a, pl.own, st));
+  }
+  a.k = p->prefix_key.ptr, a.ks = p->prefix_key.row_stride, a.kh = p->prefix_key.head_stride;
+  a.v = p->prefix_value.ptr, a.vs = p->prefix_value.row_stride, a.vh = p->prefix_value.head_stride;
+  a.vec_k = aligned_rows(p->prefix_key, p->dtype, p->dim);
+  a.vec_v = aligned_rows(p->prefix_value, p->dtype, p->dim);
+  a.mask = p->prefix_mask;
+  a.nk = (int)p->n_prefix;
+  a.qmode = a.kmode = kWhole;
+  a.B = 1;
+  a.causal = 0;
+  a.nsplit = pl.pre.nsplit;
+  a.slot0 = 0;
+  MONO_TRY(launch<kFwd>(p->dtype, a, pl.pre, st));
+  return pl.slots > 1 ? join(p, a.part, a.part_lse, pl.slots, st) : 0;
+}
+}

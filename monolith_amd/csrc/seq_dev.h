@@ -1,0 +1,247 @@
+// Device parts that the attention kernels (attention.hip) and the softmax cross entropy
+// (softmax_ce.hip) share (gfx950 only).
+//
+// All of them are one scheme. A workgroup keeps a tile of rows X ("columns" of the products) in
+// registers as B operands and streams rows Y through LDS. A 16x16 matrix instruction gives
+// S[y][x] = Y X^T with x = lane & 15 and y = 4 * (lane >> 4) + r in accumulator r, so whatever
+// belongs to a column (softmax maximum and sum, label, limit) is one register of a lane, and the
+// weights P = f(S) lie in the lanes exactly as the B operand of the second product
+// Z^T P = sum over y of Z[y][d] P[y][x] wants them, up to an order of the summation index y that
+// the A operand Z^T follows: P never goes through LDS. Z^T comes out of the row-major LDS tile by
+// the transposing LDS read (bf16) or by 4-byte reads (fp32).
+#ifndef MONO_SEQ_DEV_H_
+#define MONO_SEQ_DEV_H_
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace mono {
+namespace seq {
+
+typedef __bf16 bf16;
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf4 __attribute__((ext_vector_type(4)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ inline float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ inline float neg_inf() { return -__builtin_inff(); }
+
+// reductions over the four lanes that hold one column
+__device__ inline float col_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ inline float col_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+// Where a row of D elements starts, and how it may be read: `vec` rows start on 16 bytes and hold
+// whole 16-byte chunks.
+template <typename T>
+__device__ inline u4 load_chunk(const T* row, int e0, int D, bool vec) {
+  constexpr int E = 16 / sizeof(T);
+  u4 out = {0u, 0u, 0u, 0u};
+  if (e0 >= D) return out;
+  if (vec) return *(const u4*)(row + e0);
+  T tmp[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) tmp[i] = e0 + i < D ? row[e0 + i] : (T)0.0f;
+  __builtin_memcpy(&out, tmp, 16);
+  return out;
+}
+
+// A tile of BN rows on its way from global memory to LDS: load() takes the thread's chunks into
+// registers (rows outside [0, n) or not alive become zeros, so that nothing that lies in such a row
+// reaches a product), store() writes them.
+template <typename T, int DP, int BN, int NT>
+struct Stage {
+  static constexpr int E = 16 / sizeof(T);   // elements of a chunk
+  static constexpr int CH = DP / E;          // chunks of a row
+  static constexpr int PER = (BN * CH + NT - 1) / NT;
+  static constexpr int LDW = DP + E;         // LDS row: 16 bytes of padding against bank conflicts
+  u4 r[PER];
+
+  template <typename Alive>
+  __device__ inline void load(const T* base, int64_t stride, int row0, int n, int D, bool vec, int tid,
+                              Alive alive) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = tid + i * NT, row = row0 + c / CH, e0 = (c % CH) * E;
+      r[i] = u4{0u, 0u, 0u, 0u};
+      if (c < BN * CH && row < n && alive(row))
+        r[i] = load_chunk(base + (int64_t)row * stride, e0, D, vec);
+    }
+  }
+  __device__ inline void store(T* lds, int tid) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = tid + i * NT;
+      if (c < BN * CH) *(u4*)(lds + (c / CH) * LDW + (c % CH) * E) = r[i];
+    }
+  }
+};
+
+template <typename T, int DP>
+struct Mma;
+
+// bf16: 16x16x32, the operands' 8 elements of a lane are k = 8 * (lane >> 4) + j.
+template <int DP>
+struct Mma<bf16, DP> {
+  static constexpr int KF = DP / 32, NDT = DP / 16, LDW = DP + 8;
+  typedef bf8 Frag;
+  template <int NC>
+  static __device__ inline void scores(const bf16* lds, int rt, const Frag (&x)[NC][KF], f4 (&s)[NC],
+                                       int lane) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) s[c] = f4{0.f, 0.f, 0.f, 0.f};
+    const bf16* p = lds + (rt * 16 + (lane & 15)) * LDW + 8 * (lane >> 4);
+#pragma unroll
+    for (int k = 0; k < KF; ++k) {
+      const bf8 a = *(const bf8*)(p + 32 * k);
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        s[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, x[c][k], s[c], 0, 0, 0);
+    }
+  }
+  static __device__ inline void load_cols(Frag (&f)[KF], const bf16* row, bool ok, int D, bool vec,
+                                          int lane) {
+#pragma unroll
+    for (int k = 0; k < KF; ++k) {
+      u4 c = {0u, 0u, 0u, 0u};
+      if (ok) c = load_chunk(row, 32 * k + 8 * (lane >> 4), D, vec);
+      f[k] = __builtin_bit_cast(bf8, c);
+    }
+  }
+  static __device__ inline float dot(const Frag (&a)[KF], const Frag (&b)[KF]) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < KF; ++k)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) t = fmaf((float)a[k][j], (float)b[k][j], t);
+    return t;
+  }
+  // Four rows y..y+3 of columns d0..d0+15 of a row-major tile, transposed: in every group of 16
+  // lanes, lane i addresses 8 bytes (row i / 4, columns 4 * (i % 4)..) and receives column i.
+  static __device__ inline s4 read_tr(const bf16* lds, int y, int d0, int lane) {
+    const bf16* p = lds + (y + ((lane & 15) >> 2)) * LDW + d0 + 4 * (lane & 3);
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p);
+  }
+  // acc[dt][c] += sum over the tile's rows of Z[y][16 dt + ..] P[y][x]. P is rounded to bf16 here:
+  // half a step of 2^-8 of every weight, independent from weight to weight, beside the one rounding
+  // of the result to the same type.
+  template <int NC, int NR>
+  static __device__ inline void accumulate(const bf16* lds, const f4 (&p)[NR][NC], f4 (&acc)[NDT][NC],
+                                           int lane) {
+#pragma unroll
+    for (int t = 0; t < NR / 2; ++t) {
+      bf8 b[NC];
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          b[c][j] = (bf16)p[2 * t][c][j];
+          b[c][4 + j] = (bf16)p[2 * t + 1][c][j];
+        }
+      const int y = 32 * t + 4 * (lane >> 4);
+#pragma unroll
+      for (int d = 0; d < NDT; ++d) {
+        const s4 lo = read_tr(lds, y, 16 * d, lane), hi = read_tr(lds, y + 16, 16 * d, lane);
+        const bf4 l = __builtin_bit_cast(bf4, lo), h = __builtin_bit_cast(bf4, hi);
+        const bf8 a = {l[0], l[1], l[2], l[3], h[0], h[1], h[2], h[3]};
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          acc[d][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[c], acc[d][c], 0, 0, 0);
+      }
+    }
+  }
+};
+
+// fp32: 16x16x4, one element of a lane, k = lane >> 4. A lane's 16-byte chunk serves four
+// instructions: which k slot stands for which element is free as long as both operands agree.
+template <int DP>
+struct Mma<float, DP> {
+  static constexpr int KF = DP / 16, NDT = DP / 16, LDW = DP + 4;
+  typedef f4 Frag;
+  template <int NC>
+  static __device__ inline void scores(const float* lds, int rt, const Frag (&x)[NC][KF], f4 (&s)[NC],
+                                       int lane) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) s[c] = f4{0.f, 0.f, 0.f, 0.f};
+    const float* p = lds + (rt * 16 + (lane & 15)) * LDW + 4 * (lane >> 4);
+#pragma unroll
+    for (int k = 0; k < KF; ++k) {
+      const f4 a = *(const f4*)(p + 16 * k);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          s[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], x[c][k][j], s[c], 0, 0, 0);
+    }
+  }
+  static __device__ inline void load_cols(Frag (&f)[KF], const float* row, bool ok, int D, bool vec,
+                                          int lane) {
+#pragma unroll
+    for (int k = 0; k < KF; ++k) {
+      u4 c = {0u, 0u, 0u, 0u};
+      if (ok) c = load_chunk(row, 16 * k + 4 * (lane >> 4), D, vec);
+      f[k] = __builtin_bit_cast(f4, c);
+    }
+  }
+  static __device__ inline float dot(const Frag (&a)[KF], const Frag (&b)[KF]) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < KF; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t = fmaf(a[k][j], b[k][j], t);
+    return t;
+  }
+  template <int NC, int NR>
+  static __device__ inline void accumulate(const float* lds, const f4 (&p)[NR][NC], f4 (&acc)[NDT][NC],
+                                           int lane) {
+#pragma unroll
+    for (int t = 0; t < NR; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float* z = lds + (16 * t + 4 * (lane >> 4) + r) * LDW + (lane & 15);
+#pragma unroll
+        for (int d = 0; d < NDT; ++d) {
+          const float a = z[16 * d];
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+            acc[d][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, p[t][c][r], acc[d][c], 0, 0, 0);
+        }
+      }
+  }
+};
+
+// four consecutive elements of a row of D
+template <typename T>
+__device__ inline void store4(T* row, int d0, int D, f4 v, bool vec) {
+  if (vec && d0 + 4 <= D) {
+    T t[4] = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    if (sizeof(T) == 4) {
+      u4 w;
+      __builtin_memcpy(&w, t, 16);
+      *(u4*)(row + d0) = w;
+    } else {
+      uint64_t w;
+      __builtin_memcpy(&w, t, 8);
+      *(uint64_t*)(row + d0) = w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (d0 + i < D) row[d0 + i] = (T)v[i];
+  }
+}
+
+}  // namespace seq
+}  // namespace mono
+
+#endif  // MONO_SEQ_DEV_H_

@@ -1,0 +1,495 @@
+// softmax_ce.hip — softmax cross entropy of queries against embedding rows, and its gradient. The
+// logits are made tile by tile in registers (seq_dev.h) and never stored: the forward keeps one
+// running maximum and sum per query, the backward makes the logits again from the same tiles.
+#include <algorithm>
+
+#include "mono_common.h"
+#include "seq_dev.h"
+
+namespace mono {
+namespace {
+using namespace seq;
+
+struct Args {
+  const void *q, *w;
+  int64_t qs, ws;
+  const int64_t* labels;
+  const float *bias, *grad;
+  float *lse, *loss;
+  void *dq, *dw;
+  float* db;
+  float *part, *part2;  // forward: maximum and sum of every split; backward: partial gradients
+  int n, v, D, nsplit;
+  float scale, scale2;
+  int vec_q, vec_w, vec_o;
+};
+
+template <typename T>
+struct Tile {
+  static constexpr int BN = sizeof(T) == 2 ? 64 : 32, NR = BN / 16;
+};
+
+__device__ inline float bias2(const float* bias, int v) { return bias ? bias[v] * kLog2e : 0.f; }
+__device__ inline void range_of(int n, int nsplit, int split, int BN, int* beg, int* end) {
+  const int chunk = ((n + nsplit - 1) / nsplit + BN - 1) / BN * BN;
+  *beg = (int)min((int64_t)n, (int64_t)split * chunk);
+  *end = (int)min((int64_t)n, (int64_t)*beg + chunk);
+}
+
+// ---- forward: running maximum and sum of a tile of queries over one piece of the vocabulary ----
+template <typename T, int DP, int NC>
+__global__ __launch_bounds__(256) void k_ce_fwd(Args a) {
+  typedef Mma<T, DP> M;
+  constexpr int BM = NC * 64, BN = Tile<T>::BN, NR = Tile<T>::NR;
+  typedef Stage<T, DP, BN, 256> St;
+  __shared__ __align__(16) T lw[BN * St::LDW];
+  __shared__ __align__(16) float lb[BN];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int col[NC];
+  typename M::Frag qf[NC][M::KF];
+  float m[NC], l[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    col[c] = blockIdx.x * BM + (wave * NC + c) * 16 + (lane & 15);
+    const bool ok = col[c] < a.n;
+    M::load_cols(qf[c], (const T*)a.q + (int64_t)(ok ? col[c] : 0) * a.qs, ok, a.D, a.vec_q, lane);
+    m[c] = neg_inf();
+    l[c] = 0.f;
+  }
+  int vbeg, vend;
+  range_of(a.v, a.nsplit, blockIdx.y, BN, &vbeg, &vend);
+  St st;
+  float eb = 0.f;
+  auto fetch = [&](int y0) {
+    st.load((const T*)a.w, a.ws, y0, vend, a.D, a.vec_w, tid,
+            [&](int row) { return !a.bias || a.bias[row] != neg_inf(); });
+    if (tid < BN) eb = y0 + tid < vend ? bias2(a.bias, y0 + tid) : neg_inf();
+  };
+  if (vbeg < vend) fetch(vbeg);
+  for (int y0 = vbeg; y0 < vend; y0 += BN) {
+    __syncthreads();
+    st.store(lw, tid);
+    if (tid < BN) lb[tid] = eb;
+    __syncthreads();
+    if (y0 + BN < vend) fetch(y0 + BN);
+    f4 s[NR][NC];
+#pragma unroll
+    for (int rt = 0; rt < NR; ++rt) {
+      M::template scores<NC>(lw, rt, qf, s[rt], lane);
+      const f4 b = *(const f4*)(lb + 16 * rt + 4 * (lane >> 4));
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[rt][c][r] = fmaf(s[rt][c][r], a.scale2, b[r]);
+    }
+    // every lane keeps the maximum and sum of the candidates that it holds itself; the four lanes
+    // of a query are joined once, behind the loop
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      float mx = m[c];
+#pragma unroll
+      for (int rt = 0; rt < NR; ++rt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[rt][c][r]);
+      const float base = mx == neg_inf() ? 0.f : mx;
+      float sum = 0.f;
+#pragma unroll
+      for (int rt = 0; rt < NR; ++rt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum += exp2_hw(s[rt][c][r] - base);
+      l[c] = fmaf(l[c], exp2_hw(m[c] - base), sum);
+      m[c] = mx;
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const float mx = col_max(m[c]), base = mx == neg_inf() ? 0.f : mx;
+    const float sum = col_sum(l[c] * exp2_hw(m[c] - base));
+    if (lane < 16 && col[c] < a.n) {
+      a.part[(int64_t)blockIdx.y * a.n + col[c]] = mx;
+      a.part2[(int64_t)blockIdx.y * a.n + col[c]] = sum;
+    }
+  }
+}
+
+// One wave per query: joins the pieces of the vocabulary and takes the label's own logit off.
+template <typename T>
+__global__ __launch_bounds__(256) void k_ce_loss(Args a) {
+  const int lane = threadIdx.x & 63;
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= a.n) return;
+  float m = neg_inf();
+  for (int s = lane; s < a.nsplit; s += 64) m = fmaxf(m, a.part[(int64_t)s * a.n + i]);
+#pragma unroll
+  for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+  const float base = m == neg_inf() ? 0.f : m;
+  float z = 0.f;
+  for (int s = lane; s < a.nsplit; s += 64)
+    z += a.part2[(int64_t)s * a.n + i] * exp2_hw(a.part[(int64_t)s * a.n + i] - base);
+  const int64_t label = a.labels[i];
+  const bool known = label >= 0 && label < a.v;
+  float hit = 0.f;
+  if (known)
+    for (int d = lane; d < a.D; d += 64)
+      hit = fmaf((float)((const T*)a.q)[(int64_t)i * a.qs + d], (float)((const T*)a.w)[label * a.ws + d], hit);
+#pragma unroll
+  for (int x = 32; x; x >>= 1) {
+    z += __shfl_xor(z, x);
+    hit += __shfl_xor(hit, x);
+  }
+  if (lane) return;
+  const float b = known && a.bias ? a.bias[label] : 0.f;
+  const bool out = b == neg_inf();
+  const float lse = m + __log2f(z);
+  float loss = fmaf(lse, kLn2, -fmaf(hit, a.scale, b));
+  if (out) loss = __builtin_inff();
+  if (!known) loss = label == -1 ? 0.f : __builtin_nanf("");
+  a.loss[i] = loss;
+  a.lse[i] = known && !out ? lse : __builtin_inff();
+}
+
+// ---- backward ------------------------------------------------------------------------------
+// dquery_i = scale g_i (sum_v p_iv w_v - w_label): g and the label's row are taken in behind the
+// loop, in 32 bits, so that the products see nothing but the probabilities.
+template <typename T>
+__device__ inline f4 minus_label(const Args& a, int i, int d0, f4 t) {
+  const float lse = a.lse[i];
+  if (lse == __builtin_inff()) return f4{0.f, 0.f, 0.f, 0.f};
+  const float g = a.grad[i] * a.scale;
+  const T* w = (const T*)a.w + a.labels[i] * a.ws;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) t[r] = d0 + r < a.D ? g * (t[r] - (float)w[d0 + r]) : 0.f;
+  return t;
+}
+
+template <typename T, int DP, int NC>
+__global__ __launch_bounds__(256) void k_ce_dq(Args a) {
+  typedef Mma<T, DP> M;
+  constexpr int BM = NC * 64, BN = Tile<T>::BN, NR = Tile<T>::NR;
+  typedef Stage<T, DP, BN, 256> St;
+  __shared__ __align__(16) T lw[BN * St::LDW];
+  __shared__ __align__(16) float lb[BN];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int col[NC];
+  typename M::Frag qf[NC][M::KF];
+  float lse[NC];
+  f4 acc[M::NDT][NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    col[c] = blockIdx.x * BM + (wave * NC + c) * 16 + (lane & 15);
+    const bool ok = col[c] < a.n;
+    M::load_cols(qf[c], (const T*)a.q + (int64_t)(ok ? col[c] : 0) * a.qs, ok, a.D, a.vec_q, lane);
+    lse[c] = ok ? a.lse[col[c]] : __builtin_inff();
+#pragma unroll
+    for (int d = 0; d < M::NDT; ++d) acc[d][c] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  int vbeg, vend;
+  range_of(a.v, a.nsplit, blockIdx.y, BN, &vbeg, &vend);
+  St st;
+  float eb = 0.f;
+  auto fetch = [&](int y0) {
+    st.load((const T*)a.w, a.ws, y0, vend, a.D, a.vec_w, tid,
+            [&](int row) { return !a.bias || a.bias[row] != neg_inf(); });
+    if (tid < BN) eb = y0 + tid < vend ? bias2(a.bias, y0 + tid) : neg_inf();
+  };
+  if (vbeg < vend) fetch(vbeg);
+  for (int y0 = vbeg; y0 < vend; y0 += BN) {
+    __syncthreads();
+    st.store(lw, tid);
+    if (tid < BN) lb[tid] = eb;
+    __syncthreads();
+    if (y0 + BN < vend) fetch(y0 + BN);
+    f4 s[NR][NC];
+#pragma unroll
+    for (int rt = 0; rt < NR; ++rt) {
+      M::template scores<NC>(lw, rt, qf, s[rt], lane);
+      const f4 b = *(const f4*)(lb + 16 * rt + 4 * (lane >> 4));
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[rt][c][r] = exp2_hw(fmaf(s[rt][c][r], a.scale2, b[r] - lse[c]));
+    }
+    M::template accumulate<NC, NR>(lw, s, acc, lane);
+  }
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    if (col[c] >= a.n) continue;
+#pragma unroll
+    for (int d = 0; d < M::NDT; ++d) {
+      const int d0 = 16 * d + 4 * (lane >> 4);
+      if (a.part) {
+        store4(a.part + ((int64_t)blockIdx.y * a.n + col[c]) * a.D, d0, a.D, acc[d][c], a.vec_o);
+      } else if (d0 < a.D) {
+        store4((T*)a.dq + (int64_t)col[c] * a.D, d0, a.D, minus_label<T>(a, col[c], d0, acc[d][c]), a.vec_o);
+      }
+    }
+  }
+}
+
+// dquery from the splits' partial sums, four elements of a row per thread
+template <typename T>
+__global__ __launch_bounds__(256) void k_ce_dq_join(Args a) {
+  const int per = (a.D + 3) / 4;
+  const int64_t total = (int64_t)a.n * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int row = (int)(i / per), d0 = (int)(i % per) * 4;
+    f4 t = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.nsplit; ++s) {
+      const float* p = a.part + ((int64_t)s * a.n + row) * a.D;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (d0 + r < a.D) t[r] += p[d0 + r];
+    }
+    store4((T*)a.dq + (int64_t)row * a.D, d0, a.D, minus_label<T>(a, row, d0, t), a.vec_o);
+  }
+}
+
+// drows_v = scale sum_i g_i (p_iv - [v = label_i]) query_i, dbias_v the same without scale and query:
+// a tile of candidates keeps its sums while all queries stream by. The label's share is rare: one
+// ballot per tile of queries says whether any label falls into the candidates of the workgroup.
+template <typename T, int DP, int NC>
+__global__ __launch_bounds__(256) void k_ce_dw(Args a) {
+  typedef Mma<T, DP> M;
+  constexpr int BM = NC * 64, BN = Tile<T>::BN, NR = Tile<T>::NR;
+  typedef Stage<T, DP, BN, 256> St;
+  __shared__ __align__(16) T lq[BN * St::LDW];
+  __shared__ __align__(16) float ll[BN], lg[BN];
+  __shared__ __align__(16) int lab[BN];
+  typedef int i4 __attribute__((ext_vector_type(4)));
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int v0 = blockIdx.x * BM;
+  int col[NC];
+  typename M::Frag wf[NC][M::KF];
+  float b2[NC], sb[NC];
+  f4 acc[M::NDT][NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    col[c] = v0 + (wave * NC + c) * 16 + (lane & 15);
+    const bool ok = col[c] < a.v;
+    b2[c] = ok ? bias2(a.bias, col[c]) : neg_inf();
+    M::load_cols(wf[c], (const T*)a.w + (int64_t)(ok ? col[c] : 0) * a.ws, b2[c] != neg_inf(), a.D, a.vec_w, lane);
+    sb[c] = 0.f;
+#pragma unroll
+    for (int d = 0; d < M::NDT; ++d) acc[d][c] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  int nbeg, nend;
+  range_of(a.n, a.nsplit, blockIdx.y, BN, &nbeg, &nend);
+  St st;
+  float el = 0.f, eg = 0.f;
+  int lb = -1;
+  auto fetch = [&](int y0) {
+    st.load((const T*)a.q, a.qs, y0, nend, a.D, a.vec_q, tid,
+            [&](int row) { return a.lse[row] != __builtin_inff(); });
+    if (tid < BN) {
+      el = __builtin_inff();
+      eg = 0.f;
+      lb = -1;
+      if (y0 + tid < nend) {
+        el = a.lse[y0 + tid];
+        if (el != __builtin_inff()) {
+          eg = a.grad[y0 + tid];
+          lb = (int)a.labels[y0 + tid];
+        }
+      }
+    }
+  };
+  if (nbeg < nend) fetch(nbeg);
+  for (int y0 = nbeg; y0 < nend; y0 += BN) {
+    __syncthreads();
+    st.store(lq, tid);
+    if (tid < BN) {
+      ll[tid] = el;
+      lg[tid] = eg;
+      lab[tid] = lb;
+    }
+    __syncthreads();
+    if (y0 + BN < nend) fetch(y0 + BN);
+    const int mine = lab[lane & (BN - 1)];
+    const bool hits = __any(mine >= v0 && mine < v0 + BM);
+    f4 s[NR][NC];
+#pragma unroll
+    for (int rt = 0; rt < NR; ++rt) {
+      M::template scores<NC>(lq, rt, wf, s[rt], lane);
+      const int y = 16 * rt + 4 * (lane >> 4);
+      const f4 e = *(const f4*)(ll + y), g = *(const f4*)(lg + y);
+      const i4 lbl = *(const i4*)(lab + y);
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float p = exp2_hw(fmaf(s[rt][c][r], a.scale2, b2[c] - e[r]));
+          if (hits && lbl[r] == col[c]) p -= 1.f;
+          s[rt][c][r] = p * g[r];
+        }
+    }
+    if (a.db) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int rt = 0; rt < NR; ++rt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sb[c] += s[rt][c][r];
+    }
+    M::template accumulate<NC, NR>(lq, s, acc, lane);
+  }
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const float b = col_sum(sb[c]);
+    if (col[c] >= a.v) continue;
+    const int64_t row = (a.nsplit > 1 ? (int64_t)blockIdx.y * a.v : 0) + col[c];
+    if (a.db && lane < 16) (a.nsplit > 1 ? a.part2 : a.db)[row] = b;
+    if (!a.dw) continue;
+#pragma unroll
+    for (int d = 0; d < M::NDT; ++d) {
+      const int d0 = 16 * d + 4 * (lane >> 4);
+      if (a.nsplit > 1) store4(a.part + row * a.D, d0, a.D, acc[d][c] * a.scale, a.vec_o);
+      else store4((T*)a.dw + row * a.D, d0, a.D, acc[d][c] * a.scale, a.vec_o);
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_ce_sum(const float* part, int n_part, int64_t total, T* out) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    float t = 0.f;
+    for (int s = 0; s < n_part; ++s) t += part[(int64_t)s * total + i];
+    out[i] = (T)t;
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------
+int cols_of(const mono_softmax_ce_args* p) { return p->dtype == MONO_ROW_BF16 && p->dim <= 128 ? 2 : 1; }
+// tiles of `kept` rows, and pieces of the streamed rows that fill the card when there are few tiles
+int64_t tiles_of(const mono_softmax_ce_args* p, int64_t kept) {
+  const int bm = 64 * cols_of(p);
+  return (kept + bm - 1) / bm;
+}
+int pieces_of(const mono_softmax_ce_args* p, int64_t kept, int64_t streamed) {
+  const int64_t tiles = tiles_of(p, kept), want = 256 * 4;
+  if (tiles >= want) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>((want + tiles - 1) / std::max<int64_t>(1, tiles), streamed / 256));
+}
+
+int check(const mono_softmax_ce_args* p, const char* who) {
+  MONO_REQUIRE(p != nullptr, "%s: args is NULL", who);
+  MONO_REQUIRE(p->dtype == MONO_ROW_FP32 || p->dtype == MONO_ROW_BF16, "%s: unknown row type %d", who, p->dtype);
+  MONO_REQUIRE(p->dim >= 1 && p->dim <= 256, "%s: dim must be in [1, 256], got %d", who, p->dim);
+  MONO_REQUIRE(p->n >= 0 && p->vocab >= 1 && p->n < (1LL << 31) - 65536 && p->vocab < (1LL << 31) - 65536,
+               "%s: %lld queries and %lld rows are out of range", who, (long long)p->n, (long long)p->vocab);
+  return 0;
+}
+Args base_args(const mono_softmax_ce_args* p) {
+  Args a{};
+  const int e = p->dtype == MONO_ROW_BF16 ? 8 : 4;
+  a.q = p->query, a.qs = p->query_stride, a.w = p->rows, a.ws = p->rows_stride;
+  a.labels = p->labels, a.bias = p->bias, a.grad = p->grad_loss, a.lse = p->lse, a.loss = p->loss;
+  a.dq = p->grad_query, a.dw = p->grad_rows, a.db = p->grad_bias;
+  a.n = (int)p->n, a.v = (int)p->vocab, a.D = p->dim, a.nsplit = 1;
+  a.scale = p->scale, a.scale2 = p->scale * kLog2e;
+  a.vec_q = p->dim % e == 0 && p->query_stride % e == 0 && ((uintptr_t)p->query & 15) == 0;
+  a.vec_w = p->dim % e == 0 && p->rows_stride % e == 0 && ((uintptr_t)p->rows & 15) == 0;
+  a.vec_o = p->dim % e == 0 && (((uintptr_t)p->grad_query | (uintptr_t)p->grad_rows) & 15) == 0;
+  return a;
+}
+
+enum Which { kFwd, kDq, kDw };
+template <int W, typename T, int DP, int NC>
+int launch1(const Args& a, int64_t tiles, hipStream_t st) {
+  const dim3 grid((unsigned)tiles, (unsigned)a.nsplit);
+  if (W == kFwd) k_ce_fwd<T, DP, NC><<<grid, 256, 0, st>>>(a);
+  else if (W == kDq) k_ce_dq<T, DP, NC><<<grid, 256, 0, st>>>(a);
+  else k_ce_dw<T, DP, NC><<<grid, 256, 0, st>>>(a);
+  MONO_HIP(hipGetLastError());
+  return 0;
+}
+template <int W>
+int launch(int dtype, const Args& a, int64_t tiles, hipStream_t st) {
+  if (dtype == MONO_ROW_BF16) {
+    if (a.D <= 32) return launch1<W, bf16, 32, 2>(a, tiles, st);
+    if (a.D <= 64) return launch1<W, bf16, 64, 2>(a, tiles, st);
+    if (a.D <= 128) return launch1<W, bf16, 128, 2>(a, tiles, st);
+    return launch1<W, bf16, 256, 1>(a, tiles, st);
+  }
+  if (a.D <= 16) return launch1<W, float, 16, 1>(a, tiles, st);
+  if (a.D <= 32) return launch1<W, float, 32, 1>(a, tiles, st);
+  if (a.D <= 64) return launch1<W, float, 64, 1>(a, tiles, st);
+  if (a.D <= 128) return launch1<W, float, 128, 1>(a, tiles, st);
+  return launch1<W, float, 256, 1>(a, tiles, st);
+}
+int64_t round16(int64_t b) { return (b + 15) & ~(int64_t)15; }
+template <typename T>
+int sum_parts(const float* part, int n_part, int64_t total, T* out, hipStream_t st) {
+  k_ce_sum<T><<<grid_for(total, 256), 256, 0, st>>>(part, n_part, total, out);
+  MONO_HIP(hipGetLastError());
+  return 0;
+}
+}  // namespace
+}  // namespace mono
+
+extern "C" {
+using namespace mono;
+
+int64_t mono_softmax_cross_entropy_workspace(const mono_softmax_ce_args* p) {
+  if (check(p, "mono_softmax_cross_entropy_workspace")) return -1;
+  return 2 * round16((int64_t)pieces_of(p, p->n, p->vocab) * p->n * 4);
+}
+
+int mono_softmax_cross_entropy(const mono_softmax_ce_args* p, void* stream) {
+  MONO_TRY(check(p, "mono_softmax_cross_entropy"));
+  if (p->n == 0) return 0;
+  MONO_REQUIRE(p->workspace_bytes >= mono_softmax_cross_entropy_workspace(p),
+               "mono_softmax_cross_entropy: workspace of %lld bytes is too small", (long long)p->workspace_bytes);
+  hipStream_t st = (hipStream_t)stream;
+  Args a = base_args(p);
+  a.nsplit = pieces_of(p, p->n, p->vocab);
+  a.part = (float*)p->workspace;
+  a.part2 = (float*)((char*)p->workspace + round16((int64_t)a.nsplit * p->n * 4));
+  MONO_TRY(launch<kFwd>(p->dtype, a, tiles_of(p, p->n), st));
+  const unsigned grid = (unsigned)((p->n + 3) / 4);
+  if (p->dtype == MONO_ROW_BF16) k_ce_loss<bf16><<<grid, 256, 0, st>>>(a);
+  else k_ce_loss<float><<<grid, 256, 0, st>>>(a);
+  MONO_HIP(hipGetLastError());
+  return 0;
+}
+
+int64_t mono_softmax_cross_entropy_gradient_workspace(const mono_softmax_ce_args* p) {
+  if (check(p, "mono_softmax_cross_entropy_gradient_workspace")) return -1;
+  const int64_t sq = pieces_of(p, p->n, p->vocab), sw = pieces_of(p, p->vocab, p->n);
+  return std::max(sq <= 1 ? 0 : round16(sq * p->n * p->dim * 4),
+                  sw <= 1 ? 0 : round16(sw * p->vocab * p->dim * 4) + round16(sw * p->vocab * 4));
+}
+
+int mono_softmax_cross_entropy_gradient(const mono_softmax_ce_args* p, void* stream) {
+  MONO_TRY(check(p, "mono_softmax_cross_entropy_gradient"));
+  MONO_REQUIRE(p->workspace_bytes >= mono_softmax_cross_entropy_gradient_workspace(p),
+               "mono_softmax_cross_entropy_gradient: workspace of %lld bytes is too small",
+               (long long)p->workspace_bytes);
+  hipStream_t st = (hipStream_t)stream;
+  const bool half = p->dtype == MONO_ROW_BF16;
+  Args a = base_args(p);
+  if (p->grad_query && p->n) {
+    a.nsplit = pieces_of(p, p->n, p->vocab);
+    a.part = a.nsplit > 1 ? (float*)p->workspace : nullptr;
+    MONO_TRY(launch<kDq>(p->dtype, a, tiles_of(p, p->n), st));
+    if (a.part) {
+      const int grid = grid_for(p->n * ((p->dim + 3) / 4), 256);
+      if (half) k_ce_dq_join<bf16><<<grid, 256, 0, st>>>(a);
+      else k_ce_dq_join<float><<<grid, 256, 0, st>>>(a);
+      MONO_HIP(hipGetLastError());
+    }
+  }
+  if (p->grad_rows || p->grad_bias) {
+    a.nsplit = pieces_of(p, p->vocab, p->n);
+    const int64_t total = p->vocab * p->dim;
+    a.part = (float*)p->workspace;
+    a.part2 = (float*)((char*)p->workspace + round16((int64_t)a.nsplit * total * 4));
+    MONO_TRY(launch<kDw>(p->dtype, a, tiles_of(p, p->vocab), st));
+    if (a.nsplit > 1) {
+      if (p->grad_rows && half) MONO_TRY(sum_parts(a.part, a.nsplit, total, (bf16*)p->grad_rows, st));
+      if (p->grad_rows && !half) MONO_TRY(sum_parts(a.part, a.nsplit, total, (float*)p->grad_rows, st));
+      if (p->grad_bias) MONO_TRY(sum_parts(a.part2, a.nsplit, p->vocab, p->grad_bias, st));
+    }
+  }
+  return 0;
+}
+}

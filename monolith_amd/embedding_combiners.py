@@ -4,11 +4,11 @@ A ragged key batch (tf.RaggedTensor in the reference) is carried as `Ragged(valu
 `values` int64[n] FIDs, `row_splits` int64[batch + 1] on the same device."""
 import abc
 import ctypes as C
-from typing import NamedTuple
+from typing import NamedTuple, Optional
 
 import torch
 
-from monolith_amd import _lib, distribution_ops
+from monolith_amd import _lib, attention_ops, distribution_ops
 from monolith_amd._lib import vp
 
 
@@ -109,3 +109,32 @@ class FirstN(Combiner):  # embedding_combiners.py:71-100
     """out[batch, seq_length, dim]: the first seq_length embeddings of every row, zero padded."""
     return _FirstN.apply(key.value_rowids().contiguous(), embedding, key.nrows(),
                          self.max_seq_length)
+
+
+class Attention(Combiner):
+  """Pools every row's embeddings by their softmax weights under a query of the row (a candidate's
+  embedding against its user's behaviours). No counterpart in the reference's combiners; the op is
+  attention_ops.ragged_attention with one query per row and the embeddings as keys and values."""
+
+  def __init__(self, query: torch.Tensor, num_heads: int = 1,
+               key_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None):
+    """query [batch, dim], float32 or bfloat16 like the embeddings; dim is cut into num_heads heads
+    that weigh the row each for itself. key_mask: bool [n], False = the value does not take part (an
+    id the table does not hold). scale: of the products, 1 / sqrt(dim / num_heads) by default."""
+    super().__init__(0)
+    if query.dim() != 2 or num_heads < 1 or query.shape[1] % num_heads:
+      raise ValueError("Attention: query must be [batch, dim] with dim a multiple of num_heads")
+    self._query, self._heads, self._mask, self._scale = query, num_heads, key_mask, scale
+
+  def combine(self, key: Ragged, embedding: torch.Tensor, name: str = None):
+    """out[batch, dim]; a row without values gets zeros."""
+    q = self._query
+    if q.shape[0] != key.nrows() or embedding.dim() != 2 or embedding.shape[1] != q.shape[1] or \
+        embedding.shape[0] != key.values.numel():
+      raise ValueError("Attention: query %s, embedding %s and a key of %d rows and %d values do not "
+                       "belong together" % (tuple(q.shape), tuple(embedding.shape), key.nrows(),
+                                            key.values.numel()))
+    split = (self._heads, q.shape[1] // self._heads)
+    out = attention_ops.ragged_attention(q.unflatten(1, split), embedding.unflatten(1, split), None,
+                                         key.row_splits, key_mask=self._mask, scale=self._scale)
+    return out.flatten(1)

@@ -1,0 +1,119 @@
+"""GPU: the sequence operators together with the table, as a sequential recommender uses them: behaviours
+are looked up, encoded by self attention, pooled by the candidate, scored against candidate rows, and
+the gradients go back into the table; then the trained rows answer a ranking request."""
+import numpy as np
+import pytest
+import torch
+
+from tests import seq_ref
+from tests.test_attention_gpu import dev, on, splits
+
+pytestmark = [pytest.mark.gpu, pytest.mark.timeout(300)]
+DIM, HEADS = 16, 2
+
+
+def _table(name):
+  from monolith_amd import entry, hash_table_ops
+  tc = entry.EmbeddingHashTableConfig(segments=[
+      entry.CombineAsSegment(DIM, entry.RandomUniformInitializer(-0.5, 0.5), entry.SgdOptimizer(),
+                             entry.Fp32Compressor())])
+  return hash_table_ops.hash_table_from_config(entry.HashTableConfigInstance(tc, [0.1]), name_suffix=name)
+
+
+def test_attention_combiner():
+  from monolith_amd import embedding_combiners as ec
+  rng = np.random.default_rng(0)
+  lens = [3, 0, 1, 40, 7]
+  s = splits(lens)
+  n = int(s[-1])
+  e64, q64 = rng.standard_normal((n, DIM)).astype(np.float32), rng.standard_normal((5, DIM)).astype(np.float32)
+  g64 = rng.standard_normal((5, DIM)).astype(np.float32)
+  mask = rng.random(n) > 0.2
+  e, q = on(e64).requires_grad_(), on(q64).requires_grad_()
+  key = ec.Ragged(torch.arange(n, device=dev()), on(s))
+  out = ec.Attention(q, HEADS, on(mask)).combine(key, e)
+  cut = lambda x: x.astype(np.float64).reshape(len(x), HEADS, -1)
+  segs = seq_ref.segments(None, s)
+  want = seq_ref.attention(cut(q64), cut(e64), cut(e64), segs, seq_ref.keep_rule(segs, mask, False),
+                           (DIM // HEADS) ** -0.5, "fp32", cut(g64))
+  flat = lambda x: tuple(y.reshape(len(y), -1) for y in x)
+  seq_ref.check(out, flat(want["out"]), "out")
+  out.backward(on(g64))
+  seq_ref.check(q.grad, flat(want["dq"]), "dq")
+  seq_ref.check(e.grad, flat(want["dkv"]), "dk")
+  with pytest.raises(ValueError):
+    ec.Attention(q[:4], HEADS).combine(key, e)
+  with pytest.raises(ValueError):
+    ec.Attention(q, 3)
+  with pytest.raises(ValueError):
+    ec.Attention(q, 1).combine(key, e[:-1])
+
+
+def test_training_step_and_ranking_request():
+  """Two steps against the same model in 64 bits: the table's rows after SGD. A step moves a row by
+  lr * gradient; the gradient's relative error is that of a few hundred 32-bit roundings (2^-24 * 500 =
+  3e-5 of the sum of magnitudes, here below 8)."""
+  from monolith_amd import attention_ops, embedding_combiners as ec, loss_ops
+  rng = np.random.default_rng(1)
+  table = _table("seq_together")
+  ids = rng.permutation(300).astype(np.int64)
+  table = table.assign(ids, rng.uniform(-1, 1, (300, DIM)).astype(np.float32))
+  lens = [5, 0, 33, 70, 1, 20]
+  s = on(splits(lens))
+  cand = on(np.arange(200, 300, dtype=np.int64))
+  bias = torch.rand(100, device=dev())
+  for step in range(2):
+    beh = on(rng.integers(0, 320, sum(lens)).astype(np.int64))  # some the table does not hold
+    target = on(rng.integers(200, 300, len(lens)).astype(np.int64))
+    labels = target - 200
+    labels[1] = -1
+    known = table.contains(beh)
+    before = [table.lookup(x).double().cpu() for x in (beh, target, cand)]
+    x, t, w = (table.lookup(i).requires_grad_() for i in (beh, target, cand))
+    h = x.view(-1, HEADS, DIM // HEADS)
+    seq = attention_ops.ragged_attention(h, h, h, s, s, known, causal=True).flatten(1) + x
+    user = ec.Attention(t, key_mask=known).combine(ec.Ragged(beh, s), seq)
+    loss = loss_ops.softmax_cross_entropy(user, w, labels, bias)
+    loss.sum().backward()
+    # the same in 64 bits by torch's own operations
+    x6, t6, w6 = (b.clone().requires_grad_() for b in before)
+    total, at = 0.0, 0
+    ok = known.cpu()
+    for b, n in enumerate(lens):
+      rows, m = x6[at:at + n], ok[at:at + n]
+      hh = rows.view(n, HEADS, -1).transpose(0, 1)
+      sc = (hh @ hh.transpose(1, 2)) / (DIM // HEADS) ** 0.5
+      keep = torch.tril(torch.ones(n, n, dtype=torch.bool)) & m[None, :]
+      p = torch.softmax(sc.masked_fill(~keep, -1e300), -1) * keep.any(-1)[:, None]
+      sq = (p @ hh).transpose(0, 1).reshape(n, DIM) + rows
+      pw = torch.softmax((sq @ t6[b] / DIM ** 0.5).masked_fill(~m, -1e300), 0) * m.any()
+      u = (pw[:, None] * sq).sum(0) if n else torch.zeros(DIM, dtype=torch.float64)
+      lg = w6 @ u + bias.double().cpu()
+      if labels[b] >= 0:
+        total = total + torch.logsumexp(lg, 0) - lg[labels[b].item()]
+      at += n
+    assert abs(total.item() - loss.double().sum().item()) < 1e-5
+    total.backward()
+    for got, want in ((x.grad, x6.grad), (t.grad, t6.grad), (w.grad, w6.grad)):
+      assert (got.double().cpu() - want).abs().max() <= 2.5e-4
+    grads = {}
+    for i, g in ((beh, x6.grad), (target, t6.grad), (cand, w6.grad)):
+      for k, r in zip(i.tolist(), g):
+        grads[k] = grads.get(k, 0) + r
+    held = torch.cat([beh, target, cand])
+    g = torch.cat([x.grad, t.grad, w.grad])
+    keep = torch.cat([known, torch.ones(len(target) + len(cand), dtype=torch.bool, device=dev())])
+    was = {k: r for k, r in zip(held.tolist(), torch.cat(before))}
+    table = table.apply_gradients(held[keep], g[keep], step, enable_dedup=True)
+    for k, r in zip(held[keep].tolist(), table.lookup(held[keep]).double().cpu()):
+      assert (r - (was[k] - 0.1 * grads[k])).abs().max() <= 1e-4, k
+  # serving: the candidates behind one user's history
+  hist = table.lookup(on(ids[:250].copy())).view(250, HEADS, -1)
+  c = table.lookup(cand).view(100, HEADS, -1)
+  got = attention_ops.shared_prefix_attention(c, hist, None, c, None, on(splits([1] * 100)))
+  h6, c6 = hist.double().cpu().numpy(), c.double().cpu().numpy()
+  segs = [(np.array([i]), np.append(np.arange(250), 250 + i)) for i in range(100)]
+  every = np.concatenate([h6, c6])
+  want = seq_ref.attention(c6, every, every, segs, lambda i, n, m: np.ones((n, m), bool),
+                           (DIM // HEADS) ** -0.5, "fp32")["out"]
+  seq_ref.check(got, (want[0], want[1] + 64 * seq_ref.U32 * np.abs(want[0])), "ranking")
