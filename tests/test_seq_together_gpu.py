@@ -81,7 +81,7 @@ def test_training_step_and_ranking_request():
     ok = known.cpu()
     for b, n in enumerate(lens):
       rows, m = x6[at:at + n], ok[at:at + n]
-      hh = rows.view(n, HEADS, -1).transpose(0, 1)
+      hh = rows.view(n, HEADS, DIM // HEADS).transpose(0, 1)
       sc = (hh @ hh.transpose(1, 2)) / (DIM // HEADS) ** 0.5
       keep = torch.tril(torch.ones(n, n, dtype=torch.bool)) & m[None, :]
       p = torch.softmax(sc.masked_fill(~keep, -1e300), -1) * keep.any(-1)[:, None]
