@@ -78,17 +78,17 @@ int64_t tiles_for(int mode, int64_t B, int64_t n, int64_t G, int BM) {
   return n * G / BM + B + 2;
 }
 
-// rows of a streamed tile: one wave alone holds half of what four hold on their way to LDS
-template <typename T, int NW>
+// rows of a streamed tile: fewer where the registers that hold it on its way to LDS are few
+template <typename T, int DP, int NW>
 struct Tile {
-  static constexpr int BN = (sizeof(T) == 2 ? 64 : 32) / (NW == 1 ? 2 : 1), NR = BN / 16;
+  static constexpr int BN = sizeof(T) == 2 && NW > 1 && DP <= 64 ? 64 : 32, NR = BN / 16;
 };
 
 // ---- forward -------------------------------------------------------------------------------
 template <typename T, int DP, int NC, int NW>
-__global__ __launch_bounds__(NW * 64) void k_attn_fwd(Args a) {
+__global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(Args a) {
   typedef Mma<T, DP> M;
-  constexpr int BM = NC * NW * 16, BN = Tile<T, NW>::BN, NR = Tile<T, NW>::NR, NT = NW * 64;
+  constexpr int BM = NC * NW * 16, BN = Tile<T, DP, NW>::BN, NR = Tile<T, DP, NW>::NR, NT = NW * 64;
   typedef Stage<T, DP, BN, NT> St;
   __shared__ __align__(16) T lk[BN * St::LDW];
   __shared__ __align__(16) T lv[BN * St::LDW];
@@ -98,8 +98,9 @@ __global__ __launch_bounds__(NW * 64) void k_attn_fwd(Args a) {
   int local;
   const Seg sq = find_tile(a.qsp, a.qmode, a.B, a.nq, a.G, BM, blockIdx.x / a.Hkv, &local);
   const int64_t nrow = (int64_t)sq.n * a.G;
-  const int64_t r0 = (int64_t)local * BM;
+  int64_t r0 = (int64_t)local * BM;
   if (r0 >= nrow) return;
+  if (a.causal) r0 = (nrow - 1) / BM * BM - r0;  // a sequence's last rows see the most keys: first
   Seg sk = {0, 0, -1};
   if (sq.b >= 0) sk = segment(a.ksp, a.kmode, sq.b, a.nk);
   // every column's row, and the keys it sees: [0, klim) of its sequence
@@ -133,8 +134,8 @@ __global__ __launch_bounds__(NW * 64) void k_attn_fwd(Args a) {
     kbeg = min(kend, split * chunk);
     kend = min(kend, kbeg + chunk);
   }
-  const T* kb = (const T*)a.k + (int64_t)sk.lo * a.ks + (int64_t)kvh * a.kh;
-  const T* vb = (const T*)a.v + (int64_t)sk.lo * a.vs + (int64_t)kvh * a.vh;
+  const Rows<T> kr = {(const T*)a.k + (int64_t)sk.lo * a.ks + (int64_t)kvh * a.kh, a.ks, a.D, a.vec_k != 0};
+  const Rows<T> vr = {(const T*)a.v + (int64_t)sk.lo * a.vs + (int64_t)kvh * a.vh, a.vs, a.D, a.vec_v != 0};
   const uint8_t* mb = a.mask ? a.mask + sk.lo : nullptr;
 
   f4 acc[M::NDT][NC];
@@ -149,53 +150,50 @@ __global__ __launch_bounds__(NW * 64) void k_attn_fwd(Args a) {
   St stk, stv;
   uint8_t mk = 0;
   auto fetch = [&](int y0) {
-    const auto alive = [&](int row) { return !mb || mb[row]; };
-    stk.load(kb, a.ks, y0, kend, a.D, a.vec_k, tid, alive);
-    stv.load(vb, a.vs, y0, kend, a.D, a.vec_v, tid, alive);
+    const auto alive = [&](int row) { return mb[row] != 0; };
+    stk.load(kr, y0, kend, tid, mb, alive);
+    stv.load(vr, y0, kend, tid, mb, alive);
     if (mb && tid < BN) mk = y0 + tid < kend ? mb[y0 + tid] : 0;
   };
   if (kbeg < kend) fetch(kbeg);
   for (int y0 = kbeg; y0 < kend; y0 += BN) {
     __syncthreads();
-    stk.store(lk, tid);
-    stv.store(lv, tid);
+    stk.store(lk, tid, mb);
+    stv.store(lv, tid, mb);
     if (mb && tid < BN) lm[tid] = mk;
     __syncthreads();
     if (y0 + BN < kend) fetch(y0 + BN);
     f4 s[NR][NC];
 #pragma unroll
-    for (int rt = 0; rt < NR; ++rt) M::template scores<NC>(lk, rt, qf, s[rt], lane);
-    const bool need = mb || y0 + BN > min(kmin, kend);
-    if (need) {
+    for (int rt = 0; rt < NR; ++rt)
+      M::template scores<NC>(lk, rt, qf, s[rt], f4{0.f, 0.f, 0.f, 0.f}, lane);
+    if (mb || y0 + BN > min(kmin, kend)) {
 #pragma unroll
       for (int rt = 0; rt < NR; ++rt) {
         const int y = 16 * rt + 4 * (lane >> 4);
         const uint32_t bytes = mb ? *(const uint32_t*)(lm + y) : 0x01010101u;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+        for (int c = 0; c < NC; ++c) {
+          const int lim = min(klim[c], kend) - y0 - y;
 #pragma unroll
-          for (int c = 0; c < NC; ++c)
-            s[rt][c][r] = (y0 + y + r < min(klim[c], kend) && ((bytes >> (8 * r)) & 0xff))
-                              ? s[rt][c][r] * a.scale2 : neg_inf();
+          for (int r = 0; r < 4; ++r)
+            if (r >= lim || !(bytes & (0xffu << (8 * r)))) s[rt][c][r] = neg_inf();
+        }
       }
-    } else {
-#pragma unroll
-      for (int rt = 0; rt < NR; ++rt)
-#pragma unroll
-        for (int c = 0; c < NC; ++c) s[rt][c] *= a.scale2;
     }
+    // m is the running maximum of the products themselves: scale > 0, so the softmax's base is m * scale
     float alpha[NC];
     bool moved = false;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      float mx = neg_inf();
+      float mx = m[c];
 #pragma unroll
       for (int rt = 0; rt < NR; ++rt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[rt][c][r]);
-      mx = fmaxf(m[c], col_max(mx));
-      const float base = mx == neg_inf() ? 0.f : mx;
-      alpha[c] = exp2_hw(m[c] - base);
+        for (int r = 0; r < 4; r += 2) mx = fmaxf(fmaxf(mx, s[rt][c][r]), s[rt][c][r + 1]);
+      mx = col_max(mx);
+      const float base = mx == neg_inf() ? 0.f : mx * a.scale2;
+      alpha[c] = exp2_hw(fmaf(m[c], a.scale2, -base));
       moved |= mx != m[c];
       m[c] = mx;
       float sum = 0.f;
@@ -203,7 +201,7 @@ __global__ __launch_bounds__(NW * 64) void k_attn_fwd(Args a) {
       for (int rt = 0; rt < NR; ++rt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float p = exp2_hw(s[rt][c][r] - base);
+          const float p = exp2_hw(fmaf(s[rt][c][r], a.scale2, -base));
           s[rt][c][r] = p;
           sum += p;
         }
@@ -215,13 +213,19 @@ __global__ __launch_bounds__(NW * 64) void k_attn_fwd(Args a) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) acc[d][c] *= alpha[c];
     }
-    M::template accumulate<NC, NR>(lv, s, acc, lane);
+#pragma unroll
+    for (int rt = 0; rt < NR; rt += 2) {
+      f4 p[2][NC];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) p[0][c] = s[rt][c], p[1][c] = s[rt + 1][c];
+      M::template accumulate<NC>(lv, rt, p, acc, lane);
+    }
   }
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const float lt = col_sum(l[c]);
     const float inv = lt == 0.f ? 0.f : 1.f / lt;
-    const float lse = lt == 0.f ? neg_inf() : m[c] + __log2f(lt);
+    const float lse = lt == 0.f ? neg_inf() : fmaf(m[c], a.scale2, __log2f(lt));
     if (!ok[c]) continue;
     const int64_t row = (int64_t)(sq.lo + tok[c]) * a.H + head[c];
     if (a.part) {
@@ -265,9 +269,9 @@ __global__ __launch_bounds__(256) void k_attn_join(const float* part, const floa
 // dQ: the forward's tiles again. With p = exp2(s - lse) from the forward's statistics and
 // delta = g.o, ds = p (g.v - delta), dq = scale sum ds k. Also writes delta for the pass over keys.
 template <typename T, int DP, int NC, int NW>
-__global__ __launch_bounds__(NW * 64) void k_attn_dq(Args a) {
+__global__ __launch_bounds__(NW * 64, 2) void k_attn_dq(Args a) {
   typedef Mma<T, DP> M;
-  constexpr int BM = NC * NW * 16, BN = Tile<T, NW>::BN, NR = Tile<T, NW>::NR, NT = NW * 64;
+  constexpr int BM = NC * NW * 16, BN = Tile<T, DP, NW>::BN, NR = Tile<T, DP, NW>::NR, NT = NW * 64;
   typedef Stage<T, DP, BN, NT> St;
   __shared__ __align__(16) T lk[BN * St::LDW];
   __shared__ __align__(16) T lv[BN * St::LDW];
@@ -277,8 +281,9 @@ __global__ __launch_bounds__(NW * 64) void k_attn_dq(Args a) {
   int local;
   const Seg sq = find_tile(a.qsp, a.qmode, a.B, a.nq, a.G, BM, blockIdx.x / a.Hkv, &local);
   const int64_t nrow = (int64_t)sq.n * a.G;
-  const int64_t r0 = (int64_t)local * BM;
+  int64_t r0 = (int64_t)local * BM;
   if (r0 >= nrow) return;
+  if (a.causal) r0 = (nrow - 1) / BM * BM - r0;  // a sequence's last rows see the most keys: first
   Seg sk = {0, 0, -1};
   if (sq.b >= 0) sk = segment(a.ksp, a.kmode, sq.b, a.nk);
   int tok[NC], head[NC], klim[NC];
@@ -319,8 +324,8 @@ __global__ __launch_bounds__(NW * 64) void k_attn_dq(Args a) {
     kbeg = min(kend, split * chunk);
     kend = min(kend, kbeg + chunk);
   }
-  const T* kb = (const T*)a.k + (int64_t)sk.lo * a.ks + (int64_t)kvh * a.kh;
-  const T* vb = (const T*)a.v + (int64_t)sk.lo * a.vs + (int64_t)kvh * a.vh;
+  const Rows<T> kr = {(const T*)a.k + (int64_t)sk.lo * a.ks + (int64_t)kvh * a.kh, a.ks, a.D, a.vec_k != 0};
+  const Rows<T> vr = {(const T*)a.v + (int64_t)sk.lo * a.vs + (int64_t)kvh * a.vh, a.vs, a.D, a.vec_v != 0};
   const uint8_t* mb = a.mask ? a.mask + sk.lo : nullptr;
   f4 acc[M::NDT][NC];
 #pragma unroll
@@ -330,38 +335,47 @@ __global__ __launch_bounds__(NW * 64) void k_attn_dq(Args a) {
   St stk, stv;
   uint8_t mk = 0;
   auto fetch = [&](int y0) {
-    const auto alive = [&](int row) { return !mb || mb[row]; };
-    stk.load(kb, a.ks, y0, kend, a.D, a.vec_k, tid, alive);
-    stv.load(vb, a.vs, y0, kend, a.D, a.vec_v, tid, alive);
+    const auto alive = [&](int row) { return mb[row] != 0; };
+    stk.load(kr, y0, kend, tid, mb, alive);
+    stv.load(vr, y0, kend, tid, mb, alive);
     if (mb && tid < BN) mk = y0 + tid < kend ? mb[y0 + tid] : 0;
   };
   if (kbeg < kend) fetch(kbeg);
   for (int y0 = kbeg; y0 < kend; y0 += BN) {
     __syncthreads();
-    stk.store(lk, tid);
-    stv.store(lv, tid);
+    stk.store(lk, tid, mb);
+    stv.store(lv, tid, mb);
     if (mb && tid < BN) lm[tid] = mk;
     __syncthreads();
     if (y0 + BN < kend) fetch(y0 + BN);
-    f4 s[NR][NC];
     const bool need = mb || y0 + BN > min(kmin, kend);
 #pragma unroll
-    for (int rt = 0; rt < NR; ++rt) {
-      f4 dp[NC];
-      M::template scores<NC>(lk, rt, qf, s[rt], lane);
-      M::template scores<NC>(lv, rt, gf, dp, lane);
-      const int y = 16 * rt + 4 * (lane >> 4);
-      const uint32_t bytes = mb ? *(const uint32_t*)(lm + y) : 0x01010101u;
+    for (int rt = 0; rt < NR; rt += 2) {
+      f4 s[2][NC];
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
+      for (int t = 0; t < 2; ++t) {
+        f4 dp[NC];
+        M::template scores<NC>(lk, rt + t, qf, s[t], f4{0.f, 0.f, 0.f, 0.f}, lane);
+        M::template scores<NC>(lv, rt + t, gf, dp, f4{0.f, 0.f, 0.f, 0.f}, lane);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float p = exp2_hw(fmaf(s[rt][c][r], a.scale2, -lse[c]));
-          if (need && !(y0 + y + r < min(klim[c], kend) && ((bytes >> (8 * r)) & 0xff))) p = 0.f;
-          s[rt][c][r] = p * (dp[c][r] - delta[c]);
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            s[t][c][r] = exp2_hw(fmaf(s[t][c][r], a.scale2, -lse[c])) * (dp[c][r] - delta[c]);
+        if (need) {
+          const int y = 16 * (rt + t) + 4 * (lane >> 4);
+          const uint32_t bytes = mb ? *(const uint32_t*)(lm + y) : 0x01010101u;
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            const int lim = min(klim[c], kend) - y0 - y;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (r >= lim || !(bytes & (0xffu << (8 * r)))) s[t][c][r] = 0.f;
+          }
         }
+      }
+      M::template accumulate<NC>(lk, rt, s, acc, lane);
     }
-    M::template accumulate<NC, NR>(lk, s, acc, lane);
   }
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
@@ -383,9 +397,9 @@ __global__ __launch_bounds__(NW * 64) void k_attn_dq(Args a) {
 // dK, dV: a tile of keys keeps its sums while the queries of its sequence stream by, the heads of
 // the group one after the other, so a shared key head's gradient is one sum in one order.
 template <typename T, int DP, int NC, int NW>
-__global__ __launch_bounds__(NW * 64) void k_attn_dkv(Args a) {
+__global__ __launch_bounds__(NW * 64, 2) void k_attn_dkv(Args a) {
   typedef Mma<T, DP> M;
-  constexpr int BM = NC * NW * 16, BN = Tile<T, NW>::BN, NR = Tile<T, NW>::NR, NT = NW * 64;
+  constexpr int BM = NC * NW * 16, BN = Tile<T, DP, NW>::BN, NR = Tile<T, DP, NW>::NR, NT = NW * 64;
   typedef Stage<T, DP, BN, NT> St;
   __shared__ __align__(16) T lq[BN * St::LDW];
   __shared__ __align__(16) T lg[BN * St::LDW];
@@ -432,13 +446,14 @@ __global__ __launch_bounds__(NW * 64) void k_attn_dkv(Args a) {
   }
   St stq, stg;
   float el = 0.f, ed = 0.f;
+  const float inv_scale2 = 1.f / a.scale2;
   auto fetch = [&](int64_t it) {
     const auto all = [](int) { return true; };
     const int head = kvh * a.G + (int)(it / nt), y0 = (int)(tfirst + it % nt) * BN;
-    stq.load((const T*)a.q + (int64_t)sq.lo * a.qs + (int64_t)head * a.qh, a.qs, y0, sq.n, a.D, a.vec_q,
-             tid, all);
-    stg.load((const T*)a.go + (int64_t)sq.lo * a.gs + (int64_t)head * a.gh, a.gs, y0, sq.n, a.D, a.vec_g,
-             tid, all);
+    const Rows<T> qr = {(const T*)a.q + (int64_t)sq.lo * a.qs + (int64_t)head * a.qh, a.qs, a.D, a.vec_q != 0};
+    const Rows<T> gr = {(const T*)a.go + (int64_t)sq.lo * a.gs + (int64_t)head * a.gh, a.gs, a.D, a.vec_g != 0};
+    stq.load(qr, y0, sq.n, tid, false, all);
+    stg.load(gr, y0, sq.n, tid, false, all);
     if (tid < BN) {
       el = __builtin_inff();
       ed = 0.f;
@@ -455,35 +470,44 @@ __global__ __launch_bounds__(NW * 64) void k_attn_dkv(Args a) {
   if (ibeg < iend) fetch(ibeg);
   for (int64_t it = ibeg; it < iend; ++it) {
     __syncthreads();
-    stq.store(lq, tid);
-    stg.store(lg, tid);
+    stq.store(lq, tid, false);
+    stg.store(lg, tid, false);
     if (tid < BN) {
-      ll[tid] = el;
-      ld[tid] = ed;
+      ll[tid] = -el * inv_scale2;
+      ld[tid] = -ed;
     }
     __syncthreads();
     const int y0 = (int)(tfirst + it % nt) * BN;
     if (it + 1 < iend) fetch(it + 1);
-    f4 p[NR][NC], ds[NR][NC];
     const bool need = y0 < qmax;
 #pragma unroll
-    for (int rt = 0; rt < NR; ++rt) {
-      M::template scores<NC>(lq, rt, kf, p[rt], lane);
-      M::template scores<NC>(lg, rt, vf, ds[rt], lane);
-      const int y = 16 * rt + 4 * (lane >> 4);
-      const f4 e = *(const f4*)(ll + y), dl = *(const f4*)(ld + y);
+    for (int rt = 0; rt < NR; rt += 2) {
+      f4 p[2][NC], ds[2][NC];
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
+      for (int t = 0; t < 2; ++t) {
+        // the rows' statistics are where the products start from: s - lse / scale and dp - delta
+        const int y = 16 * (rt + t) + 4 * (lane >> 4);
+        M::template scores<NC>(lq, rt + t, kf, p[t], *(const f4*)(ll + y), lane);
+        M::template scores<NC>(lg, rt + t, vf, ds[t], *(const f4*)(ld + y), lane);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float w = exp2_hw(fmaf(p[rt][c][r], a.scale2, -e[r]));
-          if (need && y0 + y + r < qlim[c]) w = 0.f;
-          p[rt][c][r] = w;
-          ds[rt][c][r] = w * (ds[rt][c][r] - dl[r]);
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) p[t][c][r] = exp2_hw(p[t][c][r] * a.scale2);
+        if (need) {
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            const int lim = qlim[c] - y0 - y;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (r < lim) p[t][c][r] = 0.f;
+          }
         }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) ds[t][c] *= p[t][c];
+      }
+      M::template accumulate<NC>(lg, rt, p, av, lane);
+      M::template accumulate<NC>(lq, rt, ds, ak, lane);
     }
-    M::template accumulate<NC, NR>(lg, p, av, lane);
-    M::template accumulate<NC, NR>(lq, ds, ak, lane);
   }
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
@@ -522,9 +546,13 @@ struct Shape {
 };
 // Short sequences (32 rows of a key head or fewer on average) leave most of a 64- or 128-row tile
 // empty: one wave with 16 columns per workgroup then.
-Shape shape_for(int dtype, double rows_per_seq) {
-  if (rows_per_seq <= 32) return {1, 1, 16};
-  const int nc = dtype == MONO_ROW_BF16 ? 2 : 1;
+// (fp32 rows of more than 64 elements: a tile's way to LDS alone would take a wave's registers.)
+// Two columns of 16 per wave where the registers of two waves per SIMD hold them: not in fp32, and
+// not in the pass over keys, which keeps two sums, with more than 64 elements.
+Shape shape_for(int dtype, int D, bool two_sums, double rows_per_seq) {
+  const bool half = dtype == MONO_ROW_BF16;
+  if (rows_per_seq <= 32 && (half || D <= 64)) return {1, 1, 16};
+  const int nc = half && !(two_sums && D > 64) ? 2 : 1;
   return {nc, 4, nc * 64};
 }
 // Workgroups that fill the card some times over: few tiles are split along the streamed axis, down
@@ -548,6 +576,7 @@ int check(const mono_attention_args* p, const char* who) {
   MONO_REQUIRE(p->dim >= 1 && p->dim <= 128, "%s: dim must be in [1, 128], got %d", who, p->dim);
   MONO_REQUIRE(p->heads >= 1 && p->kv_heads >= 1 && p->heads % p->kv_heads == 0,
                "%s: heads (%d) must be a positive multiple of kv_heads (%d)", who, p->heads, p->kv_heads);
+  MONO_REQUIRE(p->scale > 0.f && p->scale < __builtin_inff(), "%s: scale must be positive and finite", who);
   MONO_REQUIRE(p->batch >= 0 && p->n_query >= 0 && p->n_key >= 0 && p->n_prefix >= 0, "%s: negative size", who);
   MONO_REQUIRE(p->n_query * p->heads < (1LL << 31) && p->n_key * p->kv_heads < (1LL << 31) &&
                    p->n_prefix * p->kv_heads < (1LL << 31) && p->batch * p->kv_heads < (1LL << 31),
@@ -589,10 +618,11 @@ struct Plan {
   int64_t tiles;
   int nsplit;
 };
-Plan plan_tiles(int dtype, int mode, int64_t B, int64_t n, int64_t G, int64_t heads, double stream_rows) {
+Plan plan_tiles(int dtype, int D, bool two_sums, int mode, int64_t B, int64_t n, int64_t G, int64_t heads,
+                double stream_rows) {
   Plan pl;
   const double per = mode == kWhole ? (double)n * G : (double)n * G / std::max<int64_t>(1, B);
-  pl.sh = shape_for(dtype, per);
+  pl.sh = shape_for(dtype, D, two_sums, per);
   pl.tiles = tiles_for(mode, B, n, G, pl.sh.bm);
   pl.nsplit = splits_for(pl.tiles * heads, pl.sh.nw, stream_rows, 256);
   return pl;
@@ -600,11 +630,11 @@ Plan plan_tiles(int dtype, int mode, int64_t B, int64_t n, int64_t G, int64_t he
 double average(int64_t n, int64_t B) { return (double)n / std::max<int64_t>(1, B); }
 
 Plan plan_fwd(const mono_attention_args* p) {
-  return plan_tiles(p->dtype, p->query_splits ? kSplits : kOnePerSeq, p->batch, p->n_query,
+  return plan_tiles(p->dtype, p->dim, false, p->query_splits ? kSplits : kOnePerSeq, p->batch, p->n_query,
                     p->heads / p->kv_heads, p->kv_heads, average(p->n_key, p->batch));
 }
 Plan plan_dkv(const mono_attention_args* p) {
-  return plan_tiles(p->dtype, kSplits, p->batch, p->n_key, 1, p->kv_heads,
+  return plan_tiles(p->dtype, p->dim, true, kSplits, p->batch, p->n_key, 1, p->kv_heads,
                     average(p->n_query, p->batch) * (p->heads / p->kv_heads));
 }
 
@@ -622,8 +652,10 @@ template <int W, typename T, int DP>
 int launch2(const Args& a, const Plan& pl, hipStream_t st) {
   if (pl.tiles * a.Hkv == 0) return 0;
   MONO_REQUIRE(pl.tiles * a.Hkv < (1LL << 31), "attention: too many tiles");
-  if (pl.sh.nw == 1) return launch1<W, T, DP, 1, 1>(a, pl, st);
-  return launch1<W, T, DP, sizeof(T) == 2 ? 2 : 1, 4>(a, pl, st);
+  constexpr bool half = sizeof(T) == 2;
+  if constexpr (half || DP <= 64)
+    if (pl.sh.nw == 1) return launch1<W, T, DP, 1, 1>(a, pl, st);
+  return launch1<W, T, DP, half && !(W == kDkv && DP > 64) ? 2 : 1, 4>(a, pl, st);
 }
 template <int W>
 int launch(int dtype, const Args& a, const Plan& pl, hipStream_t st) {
@@ -672,7 +704,7 @@ struct PrefixPlan {
 PrefixPlan plan_prefix(const mono_attention_args* p) {
   PrefixPlan r;
   const int64_t G = p->heads / p->kv_heads;
-  r.pre = plan_tiles(p->dtype, kWhole, 1, p->n_query, G, p->kv_heads, (double)p->n_prefix);
+  r.pre = plan_tiles(p->dtype, p->dim, false, kWhole, 1, p->n_query, G, p->kv_heads, (double)p->n_prefix);
   r.slots = r.pre.nsplit;
   if (p->key_splits) {
     r.own = plan_fwd(p);

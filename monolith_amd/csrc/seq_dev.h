@@ -56,33 +56,64 @@ __device__ inline u4 load_chunk(const T* row, int e0, int D, bool vec) {
   return out;
 }
 
+// A rows array as the tile loads see it.
+template <typename T>
+struct Rows {
+  const T* base;    // first row
+  int64_t stride;   // elements from row to row
+  int D;
+  bool vec;         // rows start on 16 bytes and are whole 16-byte chunks
+};
+
 // A tile of BN rows on its way from global memory to LDS: load() takes the thread's chunks into
-// registers (rows outside [0, n) or not alive become zeros, so that nothing that lies in such a row
-// reaches a product), store() writes them.
+// registers, store() writes them. Rows outside [0, n) and rows that are not alive(row) become zeros,
+// so that nothing that lies in such a row reaches a product; what alive() reads is read beside the
+// row and needed only by store().
 template <typename T, int DP, int BN, int NT>
 struct Stage {
   static constexpr int E = 16 / sizeof(T);   // elements of a chunk
   static constexpr int CH = DP / E;          // chunks of a row
   static constexpr int PER = (BN * CH + NT - 1) / NT;
+  static constexpr int STEP = NT / CH;       // rows between a thread's chunks
   static constexpr int LDW = DP + E;         // LDS row: 16 bytes of padding against bank conflicts
+  static_assert(NT % CH == 0 && (PER == 1 || BN * CH % NT == 0), "every thread holds one column of chunks");
   u4 r[PER];
+  bool live[PER];
 
   template <typename Alive>
-  __device__ inline void load(const T* base, int64_t stride, int row0, int n, int D, bool vec, int tid,
-                              Alive alive) {
+  __device__ inline void load(const Rows<T>& x, int row0, int n, int tid, bool filter, Alive alive) {
+    const int row = row0 + tid / CH, e0 = tid % CH * E;
+    const bool mine = (PER > 1 || tid < BN * CH) && e0 < x.D;
+    const T* p = x.base + (int64_t)row * x.stride + e0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int c = tid + i * NT, row = row0 + c / CH, e0 = (c % CH) * E;
       r[i] = u4{0u, 0u, 0u, 0u};
-      if (c < BN * CH && row < n && alive(row))
-        r[i] = load_chunk(base + (int64_t)row * stride, e0, D, vec);
+      live[i] = true;
     }
-  }
-  __device__ inline void store(T* lds, int tid) const {
+    if (x.vec && row0 + BN <= n) {
+      if (mine)
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int c = tid + i * NT;
-      if (c < BN * CH) *(u4*)(lds + (c / CH) * LDW + (c % CH) * E) = r[i];
+        for (int i = 0; i < PER; ++i) r[i] = *(const u4*)(p + i * (STEP * x.stride));
+    } else if (x.vec) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (mine && row + i * STEP < n) r[i] = *(const u4*)(p + i * (STEP * x.stride));
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (mine && row + i * STEP < n) r[i] = load_chunk(p + i * (STEP * x.stride) - e0, e0, x.D, false);
+    }
+    if (filter)
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (mine && row + i * STEP < n) live[i] = alive(row + i * STEP);
+  }
+  __device__ inline void store(T* lds, int tid, bool filter) const {
+    if (PER > 1 || tid < BN * CH) {
+      T* p = lds + tid / CH * LDW + tid % CH * E;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        *(u4*)(p + i * STEP * LDW) = !filter || live[i] ? r[i] : u4{0u, 0u, 0u, 0u};
     }
   }
 };
@@ -97,9 +128,9 @@ struct Mma<bf16, DP> {
   typedef bf8 Frag;
   template <int NC>
   static __device__ inline void scores(const bf16* lds, int rt, const Frag (&x)[NC][KF], f4 (&s)[NC],
-                                       int lane) {
+                                       f4 from, int lane) {
 #pragma unroll
-    for (int c = 0; c < NC; ++c) s[c] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < NC; ++c) s[c] = from;
     const bf16* p = lds + (rt * 16 + (lane & 15)) * LDW + 8 * (lane >> 4);
 #pragma unroll
     for (int k = 0; k < KF; ++k) {
@@ -132,32 +163,29 @@ struct Mma<bf16, DP> {
     const bf16* p = lds + (y + ((lane & 15) >> 2)) * LDW + d0 + 4 * (lane & 3);
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p);
   }
-  // acc[dt][c] += sum over the tile's rows of Z[y][16 dt + ..] P[y][x]. P is rounded to bf16 here:
+  // acc[dt][c] += sum over the 32 rows from 16 rt on of Z[y][16 dt + ..] P[y][x]. P is rounded to bf16 here:
   // half a step of 2^-8 of every weight, independent from weight to weight, beside the one rounding
   // of the result to the same type.
-  template <int NC, int NR>
-  static __device__ inline void accumulate(const bf16* lds, const f4 (&p)[NR][NC], f4 (&acc)[NDT][NC],
+  template <int NC>
+  static __device__ inline void accumulate(const bf16* lds, int rt, const f4 (&p)[2][NC], f4 (&acc)[NDT][NC],
                                            int lane) {
+    bf8 b[NC];
 #pragma unroll
-    for (int t = 0; t < NR / 2; ++t) {
-      bf8 b[NC];
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        b[c][j] = (bf16)p[0][c][j];
+        b[c][4 + j] = (bf16)p[1][c][j];
+      }
+    const int y = 16 * rt + 4 * (lane >> 4);
+#pragma unroll
+    for (int d = 0; d < NDT; ++d) {
+      const s4 lo = read_tr(lds, y, 16 * d, lane), hi = read_tr(lds, y + 16, 16 * d, lane);
+      const bf4 l = __builtin_bit_cast(bf4, lo), h = __builtin_bit_cast(bf4, hi);
+      const bf8 a = {l[0], l[1], l[2], l[3], h[0], h[1], h[2], h[3]};
 #pragma unroll
       for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          b[c][j] = (bf16)p[2 * t][c][j];
-          b[c][4 + j] = (bf16)p[2 * t + 1][c][j];
-        }
-      const int y = 32 * t + 4 * (lane >> 4);
-#pragma unroll
-      for (int d = 0; d < NDT; ++d) {
-        const s4 lo = read_tr(lds, y, 16 * d, lane), hi = read_tr(lds, y + 16, 16 * d, lane);
-        const bf4 l = __builtin_bit_cast(bf4, lo), h = __builtin_bit_cast(bf4, hi);
-        const bf8 a = {l[0], l[1], l[2], l[3], h[0], h[1], h[2], h[3]};
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-          acc[d][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[c], acc[d][c], 0, 0, 0);
-      }
+        acc[d][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[c], acc[d][c], 0, 0, 0);
     }
   }
 };
@@ -170,9 +198,9 @@ struct Mma<float, DP> {
   typedef f4 Frag;
   template <int NC>
   static __device__ inline void scores(const float* lds, int rt, const Frag (&x)[NC][KF], f4 (&s)[NC],
-                                       int lane) {
+                                       f4 from, int lane) {
 #pragma unroll
-    for (int c = 0; c < NC; ++c) s[c] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < NC; ++c) s[c] = from;
     const float* p = lds + (rt * 16 + (lane & 15)) * LDW + 4 * (lane >> 4);
 #pragma unroll
     for (int k = 0; k < KF; ++k) {
@@ -201,14 +229,14 @@ struct Mma<float, DP> {
       for (int j = 0; j < 4; ++j) t = fmaf(a[k][j], b[k][j], t);
     return t;
   }
-  template <int NC, int NR>
-  static __device__ inline void accumulate(const float* lds, const f4 (&p)[NR][NC], f4 (&acc)[NDT][NC],
+  template <int NC>
+  static __device__ inline void accumulate(const float* lds, int rt, const f4 (&p)[2][NC], f4 (&acc)[NDT][NC],
                                            int lane) {
 #pragma unroll
-    for (int t = 0; t < NR; ++t)
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float* z = lds + (16 * t + 4 * (lane >> 4) + r) * LDW + (lane & 15);
+        const float* z = lds + (16 * (rt + t) + 4 * (lane >> 4) + r) * LDW + (lane & 15);
 #pragma unroll
         for (int d = 0; d < NDT; ++d) {
           const float a = z[16 * d];

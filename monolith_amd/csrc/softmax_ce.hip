@@ -29,7 +29,10 @@ struct Tile {
   static constexpr int BN = sizeof(T) == 2 ? 64 : 32, NR = BN / 16;
 };
 
-__device__ inline float bias2(const float* bias, int v) { return bias ? bias[v] * kLog2e : 0.f; }
+// what the products of a candidate start from: its bias in units of scale
+__device__ inline float start_of(const float* bias, int v, float inv_scale) {
+  return bias ? bias[v] * inv_scale : 0.f;
+}
 __device__ inline void range_of(int n, int nsplit, int split, int BN, int* beg, int* end) {
   const int chunk = ((n + nsplit - 1) / nsplit + BN - 1) / BN * BN;
   *beg = (int)min((int64_t)n, (int64_t)split * chunk);
@@ -38,7 +41,7 @@ __device__ inline void range_of(int n, int nsplit, int split, int BN, int* beg, 
 
 // ---- forward: running maximum and sum of a tile of queries over one piece of the vocabulary ----
 template <typename T, int DP, int NC>
-__global__ __launch_bounds__(256) void k_ce_fwd(Args a) {
+__global__ __launch_bounds__(256, 2) void k_ce_fwd(Args a) {
   typedef Mma<T, DP> M;
   constexpr int BM = NC * 64, BN = Tile<T>::BN, NR = Tile<T>::NR;
   typedef Stage<T, DP, BN, 256> St;
@@ -60,51 +63,46 @@ __global__ __launch_bounds__(256) void k_ce_fwd(Args a) {
   range_of(a.v, a.nsplit, blockIdx.y, BN, &vbeg, &vend);
   St st;
   float eb = 0.f;
+  const float inv_scale = 1.f / a.scale;
+  const Rows<T> wr = {(const T*)a.w, a.ws, a.D, a.vec_w != 0};
   auto fetch = [&](int y0) {
-    st.load((const T*)a.w, a.ws, y0, vend, a.D, a.vec_w, tid,
-            [&](int row) { return !a.bias || a.bias[row] != neg_inf(); });
-    if (tid < BN) eb = y0 + tid < vend ? bias2(a.bias, y0 + tid) : neg_inf();
+    st.load(wr, y0, vend, tid, a.bias, [&](int row) { return a.bias[row] != neg_inf(); });
+    if (tid < BN) eb = y0 + tid < vend ? start_of(a.bias, y0 + tid, inv_scale) : neg_inf();
   };
   if (vbeg < vend) fetch(vbeg);
   for (int y0 = vbeg; y0 < vend; y0 += BN) {
     __syncthreads();
-    st.store(lw, tid);
+    st.store(lw, tid, a.bias);
     if (tid < BN) lb[tid] = eb;
     __syncthreads();
     if (y0 + BN < vend) fetch(y0 + BN);
     f4 s[NR][NC];
 #pragma unroll
-    for (int rt = 0; rt < NR; ++rt) {
-      M::template scores<NC>(lw, rt, qf, s[rt], lane);
-      const f4 b = *(const f4*)(lb + 16 * rt + 4 * (lane >> 4));
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[rt][c][r] = fmaf(s[rt][c][r], a.scale2, b[r]);
-    }
+    for (int rt = 0; rt < NR; ++rt)
+      M::template scores<NC>(lw, rt, qf, s[rt], *(const f4*)(lb + 16 * rt + 4 * (lane >> 4)), lane);
     // every lane keeps the maximum and sum of the candidates that it holds itself; the four lanes
-    // of a query are joined once, behind the loop
+    // of a query are joined once, behind the loop. m is in units of scale (scale > 0).
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       float mx = m[c];
 #pragma unroll
       for (int rt = 0; rt < NR; ++rt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[rt][c][r]);
-      const float base = mx == neg_inf() ? 0.f : mx;
+        for (int r = 0; r < 4; r += 2) mx = fmaxf(fmaxf(mx, s[rt][c][r]), s[rt][c][r + 1]);
+      const float base = mx == neg_inf() ? 0.f : mx * a.scale2;
       float sum = 0.f;
 #pragma unroll
       for (int rt = 0; rt < NR; ++rt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sum += exp2_hw(s[rt][c][r] - base);
-      l[c] = fmaf(l[c], exp2_hw(m[c] - base), sum);
+        for (int r = 0; r < 4; ++r) sum += exp2_hw(fmaf(s[rt][c][r], a.scale2, -base));
+      l[c] = fmaf(l[c], exp2_hw(fmaf(m[c], a.scale2, -base)), sum);
       m[c] = mx;
     }
   }
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    const float mx = col_max(m[c]), base = mx == neg_inf() ? 0.f : mx;
-    const float sum = col_sum(l[c] * exp2_hw(m[c] - base));
+    const float mx = col_max(m[c]) * a.scale2, base = mx == neg_inf() ? 0.f : mx;
+    const float sum = col_sum(l[c] * exp2_hw(fmaf(m[c], a.scale2, -base)));
     if (lane < 16 && col[c] < a.n) {
       a.part[(int64_t)blockIdx.y * a.n + col[c]] = mx;
       a.part2[(int64_t)blockIdx.y * a.n + col[c]] = sum;
@@ -163,7 +161,7 @@ __device__ inline f4 minus_label(const Args& a, int i, int d0, f4 t) {
 }
 
 template <typename T, int DP, int NC>
-__global__ __launch_bounds__(256) void k_ce_dq(Args a) {
+__global__ __launch_bounds__(256, 2) void k_ce_dq(Args a) {
   typedef Mma<T, DP> M;
   constexpr int BM = NC * 64, BN = Tile<T>::BN, NR = Tile<T>::NR;
   typedef Stage<T, DP, BN, 256> St;
@@ -187,29 +185,32 @@ __global__ __launch_bounds__(256) void k_ce_dq(Args a) {
   range_of(a.v, a.nsplit, blockIdx.y, BN, &vbeg, &vend);
   St st;
   float eb = 0.f;
+  const float inv_scale = 1.f / a.scale;
+  const Rows<T> wr = {(const T*)a.w, a.ws, a.D, a.vec_w != 0};
   auto fetch = [&](int y0) {
-    st.load((const T*)a.w, a.ws, y0, vend, a.D, a.vec_w, tid,
-            [&](int row) { return !a.bias || a.bias[row] != neg_inf(); });
-    if (tid < BN) eb = y0 + tid < vend ? bias2(a.bias, y0 + tid) : neg_inf();
+    st.load(wr, y0, vend, tid, a.bias, [&](int row) { return a.bias[row] != neg_inf(); });
+    if (tid < BN) eb = y0 + tid < vend ? start_of(a.bias, y0 + tid, inv_scale) : neg_inf();
   };
   if (vbeg < vend) fetch(vbeg);
   for (int y0 = vbeg; y0 < vend; y0 += BN) {
     __syncthreads();
-    st.store(lw, tid);
+    st.store(lw, tid, a.bias);
     if (tid < BN) lb[tid] = eb;
     __syncthreads();
     if (y0 + BN < vend) fetch(y0 + BN);
-    f4 s[NR][NC];
 #pragma unroll
-    for (int rt = 0; rt < NR; ++rt) {
-      M::template scores<NC>(lw, rt, qf, s[rt], lane);
-      const f4 b = *(const f4*)(lb + 16 * rt + 4 * (lane >> 4));
+    for (int rt = 0; rt < NR; rt += 2) {
+      f4 s[2][NC];
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
+      for (int t = 0; t < 2; ++t) {
+        M::template scores<NC>(lw, rt + t, qf, s[t], *(const f4*)(lb + 16 * (rt + t) + 4 * (lane >> 4)), lane);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[rt][c][r] = exp2_hw(fmaf(s[rt][c][r], a.scale2, b[r] - lse[c]));
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[t][c][r] = exp2_hw(fmaf(s[t][c][r], a.scale2, -lse[c]));
+      }
+      M::template accumulate<NC>(lw, rt, s, acc, lane);
     }
-    M::template accumulate<NC, NR>(lw, s, acc, lane);
   }
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
@@ -248,7 +249,7 @@ __global__ __launch_bounds__(256) void k_ce_dq_join(Args a) {
 // a tile of candidates keeps its sums while all queries stream by. The label's share is rare: one
 // ballot per tile of queries says whether any label falls into the candidates of the workgroup.
 template <typename T, int DP, int NC>
-__global__ __launch_bounds__(256) void k_ce_dw(Args a) {
+__global__ __launch_bounds__(256, 2) void k_ce_dw(Args a) {
   typedef Mma<T, DP> M;
   constexpr int BM = NC * 64, BN = Tile<T>::BN, NR = Tile<T>::NR;
   typedef Stage<T, DP, BN, 256> St;
@@ -266,7 +267,7 @@ __global__ __launch_bounds__(256) void k_ce_dw(Args a) {
   for (int c = 0; c < NC; ++c) {
     col[c] = v0 + (wave * NC + c) * 16 + (lane & 15);
     const bool ok = col[c] < a.v;
-    b2[c] = ok ? bias2(a.bias, col[c]) : neg_inf();
+    b2[c] = !ok ? neg_inf() : a.bias ? a.bias[col[c]] * kLog2e : 0.f;
     M::load_cols(wf[c], (const T*)a.w + (int64_t)(ok ? col[c] : 0) * a.ws, b2[c] != neg_inf(), a.D, a.vec_w, lane);
     sb[c] = 0.f;
 #pragma unroll
@@ -275,11 +276,12 @@ __global__ __launch_bounds__(256) void k_ce_dw(Args a) {
   int nbeg, nend;
   range_of(a.n, a.nsplit, blockIdx.y, BN, &nbeg, &nend);
   St st;
+  const Rows<T> qr = {(const T*)a.q, a.qs, a.D, a.vec_q != 0};
+  const float inv_scale2 = 1.f / a.scale2;
   float el = 0.f, eg = 0.f;
   int lb = -1;
   auto fetch = [&](int y0) {
-    st.load((const T*)a.q, a.qs, y0, nend, a.D, a.vec_q, tid,
-            [&](int row) { return a.lse[row] != __builtin_inff(); });
+    st.load(qr, y0, nend, tid, true, [&](int row) { return a.lse[row] != __builtin_inff(); });
     if (tid < BN) {
       el = __builtin_inff();
       eg = 0.f;
@@ -296,9 +298,9 @@ __global__ __launch_bounds__(256) void k_ce_dw(Args a) {
   if (nbeg < nend) fetch(nbeg);
   for (int y0 = nbeg; y0 < nend; y0 += BN) {
     __syncthreads();
-    st.store(lq, tid);
+    st.store(lq, tid, true);
     if (tid < BN) {
-      ll[tid] = el;
+      ll[tid] = -el * inv_scale2;
       lg[tid] = eg;
       lab[tid] = lb;
     }
@@ -306,31 +308,35 @@ __global__ __launch_bounds__(256) void k_ce_dw(Args a) {
     if (y0 + BN < nend) fetch(y0 + BN);
     const int mine = lab[lane & (BN - 1)];
     const bool hits = __any(mine >= v0 && mine < v0 + BM);
-    f4 s[NR][NC];
 #pragma unroll
-    for (int rt = 0; rt < NR; ++rt) {
-      M::template scores<NC>(lq, rt, wf, s[rt], lane);
-      const int y = 16 * rt + 4 * (lane >> 4);
-      const f4 e = *(const f4*)(ll + y), g = *(const f4*)(lg + y);
-      const i4 lbl = *(const i4*)(lab + y);
+    for (int rt = 0; rt < NR; rt += 2) {
+      f4 s[2][NC];
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
+      for (int t = 0; t < 2; ++t) {
+        const int y = 16 * (rt + t) + 4 * (lane >> 4);
+        M::template scores<NC>(lq, rt + t, wf, s[t], *(const f4*)(ll + y), lane);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float p = exp2_hw(fmaf(s[rt][c][r], a.scale2, b2[c] - e[r]));
-          if (hits && lbl[r] == col[c]) p -= 1.f;
-          s[rt][c][r] = p * g[r];
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[t][c][r] = exp2_hw(fmaf(s[t][c][r], a.scale2, b2[c]));
+        if (hits) {
+          const i4 lbl = *(const i4*)(lab + y);
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (lbl[r] == col[c]) s[t][c][r] -= 1.f;
         }
+        const f4 g = *(const f4*)(lg + y);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) s[t][c] *= g;
+        if (a.db) {
+#pragma unroll
+          for (int c = 0; c < NC; ++c) sb[c] += (s[t][c][0] + s[t][c][1]) + (s[t][c][2] + s[t][c][3]);
+        }
+      }
+      M::template accumulate<NC>(lq, rt, s, acc, lane);
     }
-    if (a.db) {
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int rt = 0; rt < NR; ++rt)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) sb[c] += s[rt][c][r];
-    }
-    M::template accumulate<NC, NR>(lq, s, acc, lane);
   }
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
@@ -374,6 +380,7 @@ int check(const mono_softmax_ce_args* p, const char* who) {
   MONO_REQUIRE(p != nullptr, "%s: args is NULL", who);
   MONO_REQUIRE(p->dtype == MONO_ROW_FP32 || p->dtype == MONO_ROW_BF16, "%s: unknown row type %d", who, p->dtype);
   MONO_REQUIRE(p->dim >= 1 && p->dim <= 256, "%s: dim must be in [1, 256], got %d", who, p->dim);
+  MONO_REQUIRE(p->scale > 0.f && p->scale < __builtin_inff(), "%s: scale must be positive and finite", who);
   MONO_REQUIRE(p->n >= 0 && p->vocab >= 1 && p->n < (1LL << 31) - 65536 && p->vocab < (1LL << 31) - 65536,
                "%s: %lld queries and %lld rows are out of range", who, (long long)p->n, (long long)p->vocab);
   return 0;
