@@ -60,13 +60,20 @@ __device__ inline Seg find_tile(const int64_t* sp, int mode, int B, int n, int G
     *local = tile % per;
     return {tile / per, 1, tile / per};
   }
-  int lo = 0, hi = B + 1;  // segments 0 .. B + 1; segment i starts at start(i)
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    const int64_t start = split_at(sp, mid - 1, n);
-    if ((start * G) / BM + mid <= tile) lo = mid;
-    else hi = mid - 1;
+  // the last of segments 0 .. B + 1 (segment i starts at start(i)) whose tiles start at or before this
+  // one, 64 candidates at a time: every step is one load's latency at the head of each workgroup
+  int lo = 0, len = B + 2;
+  const int lane = threadIdx.x & 63;
+  while (len > 1) {
+    const int step = (len + 63) / 64, i = lo + lane * step;
+    bool at = false;
+    if (i < lo + len) at = i == 0 || ((int64_t)split_at(sp, i - 1, n) * G) / BM + i <= tile;
+    const uint64_t found = __ballot(at);
+    const int last = found ? 63 - __builtin_clzll(found) : 0;
+    len = min(step, len - last * step);
+    lo += last * step;
   }
+  lo = __builtin_amdgcn_readfirstlane(lo);
   const int start = lo == 0 ? 0 : split_at(sp, lo - 1, n);
   const int end = lo == B + 1 ? n : split_at(sp, lo, n);
   *local = tile - (int)(((int64_t)start * G) / BM) - lo;
@@ -81,14 +88,26 @@ int64_t tiles_for(int mode, int64_t B, int64_t n, int64_t G, int BM) {
 // rows of a streamed tile: fewer where the registers that hold it on its way to LDS are few
 template <typename T, int DP, int NW>
 struct Tile {
-  static constexpr int BN = sizeof(T) == 2 && NW > 1 && DP <= 64 ? 64 : 32, NR = BN / 16;
+  static constexpr int BN = sizeof(T) == 2 && NW > 1 && DP <= 64 ? 64 : 32, NR = BN / 32;
 };
+
+// v where a column's key (rows y of a tile, from its row 0 on) is not below lim or not alive
+__device__ inline void hide(f16v& s, int lim, const uint8_t* alive, float v, int lane) {
+  lim -= 4 * (lane >> 5);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint32_t bytes = alive ? *(const uint32_t*)(alive + 8 * q + 4 * (lane >> 5)) : 0x01010101u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (8 * q + i >= lim || !(bytes & (0xffu << (8 * i)))) s[4 * q + i] = v;
+  }
+}
 
 // ---- forward -------------------------------------------------------------------------------
 template <typename T, int DP, int NC, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(Args a) {
   typedef Mma<T, DP> M;
-  constexpr int BM = NC * NW * 16, BN = Tile<T, DP, NW>::BN, NR = Tile<T, DP, NW>::NR, NT = NW * 64;
+  constexpr int BM = NC * NW * 32, BN = Tile<T, DP, NW>::BN, NR = Tile<T, DP, NW>::NR, NT = NW * 64;
   typedef Stage<T, DP, BN, NT> St;
   __shared__ __align__(16) T lk[BN * St::LDW];
   __shared__ __align__(16) T lv[BN * St::LDW];
@@ -107,22 +126,25 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(Args a) {
   int tok[NC], head[NC], klim[NC];
   bool ok[NC];
   typename M::Frag qf[NC][M::KF];
-  int kmin = sk.n;
+  int kmin = sk.n, kmax = 0;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    const int64_t r = r0 + (wave * NC + c) * 16 + (lane & 15);
+    const int64_t r = r0 + (wave * NC + c) * 32 + (lane & 31);
     ok[c] = r < nrow;
     tok[c] = ok[c] ? (int)(r / a.G) : 0;
     head[c] = kvh * a.G + (ok[c] ? (int)(r % a.G) : 0);
     int lim = sk.n;
     if (a.causal) lim = min(lim, max(0, tok[c] + 1 + sk.n - sq.n));
     klim[c] = ok[c] ? lim : 0;
-    if (ok[c]) kmin = min(kmin, lim);
+    if (ok[c]) kmin = min(kmin, lim), kmax = max(kmax, lim);
     M::load_cols(qf[c], (const T*)a.q + (int64_t)(sq.lo + tok[c]) * a.qs + (int64_t)head[c] * a.qh, ok[c],
                  a.D, a.vec_q, lane);
   }
 #pragma unroll
-  for (int x = 8; x; x >>= 1) kmin = min(kmin, __shfl_xor(kmin, x));
+  for (int x = 16; x; x >>= 1) {
+    kmin = min(kmin, __shfl_xor(kmin, x));
+    kmax = max(kmax, __shfl_xor(kmax, x));
+  }
   int kend = sk.n;
   if (a.causal) {
     const int last = (int)((min(r0 + BM, nrow) - 1) / a.G);
@@ -138,14 +160,14 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(Args a) {
   const Rows<T> vr = {(const T*)a.v + (int64_t)sk.lo * a.vs + (int64_t)kvh * a.vh, a.vs, a.D, a.vec_v != 0};
   const uint8_t* mb = a.mask ? a.mask + sk.lo : nullptr;
 
-  f4 acc[M::NDT][NC];
+  f16v acc[M::NDT][NC];
   float m[NC], l[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     m[c] = neg_inf();
     l[c] = 0.f;
 #pragma unroll
-    for (int d = 0; d < M::NDT; ++d) acc[d][c] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < M::NDT; ++d) acc[d][c] = all_of(0.f);
   }
   St stk, stv;
   uint8_t mk = 0;
@@ -163,23 +185,16 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(Args a) {
     if (mb && tid < BN) lm[tid] = mk;
     __syncthreads();
     if (y0 + BN < kend) fetch(y0 + BN);
-    f4 s[NR][NC];
+    if (y0 >= kmax) continue;  // (per wave: every later tile only has keys that none of its rows sees)
+    f16v s[NR][NC];
 #pragma unroll
-    for (int rt = 0; rt < NR; ++rt)
-      M::template scores<NC>(lk, rt, qf, s[rt], f4{0.f, 0.f, 0.f, 0.f}, lane);
+    for (int rt = 0; rt < NR; ++rt) M::template scores<NC>(lk, rt, qf, s[rt], all_of(0.f), lane);
     if (mb || y0 + BN > min(kmin, kend)) {
 #pragma unroll
-      for (int rt = 0; rt < NR; ++rt) {
-        const int y = 16 * rt + 4 * (lane >> 4);
-        const uint32_t bytes = mb ? *(const uint32_t*)(lm + y) : 0x01010101u;
+      for (int rt = 0; rt < NR; ++rt)
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const int lim = min(klim[c], kend) - y0 - y;
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (r >= lim || !(bytes & (0xffu << (8 * r)))) s[rt][c][r] = neg_inf();
-        }
-      }
+        for (int c = 0; c < NC; ++c)
+          hide(s[rt][c], min(klim[c], kend) - y0 - 32 * rt, mb ? lm + 32 * rt : nullptr, neg_inf(), lane);
     }
     // m is the running maximum of the products themselves: scale > 0, so the softmax's base is m * scale
     float alpha[NC];
@@ -190,22 +205,22 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(Args a) {
 #pragma unroll
       for (int rt = 0; rt < NR; ++rt)
 #pragma unroll
-        for (int r = 0; r < 4; r += 2) mx = fmaxf(fmaxf(mx, s[rt][c][r]), s[rt][c][r + 1]);
+        for (int r = 0; r < 16; r += 2) mx = fmaxf(fmaxf(mx, s[rt][c][r]), s[rt][c][r + 1]);
       mx = col_max(mx);
       const float base = mx == neg_inf() ? 0.f : mx * a.scale2;
       alpha[c] = exp2_hw(fmaf(m[c], a.scale2, -base));
       moved |= mx != m[c];
       m[c] = mx;
-      float sum = 0.f;
+      float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int rt = 0; rt < NR; ++rt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
+        for (int r = 0; r < 16; ++r) {
           const float p = exp2_hw(fmaf(s[rt][c][r], a.scale2, -base));
           s[rt][c][r] = p;
-          sum += p;
+          sum[r & 1] += p;
         }
-      l[c] = fmaf(l[c], alpha[c], sum);
+      l[c] = fmaf(l[c], alpha[c], sum[0] + sum[1]);
     }
     if (__any(moved)) {
 #pragma unroll
@@ -214,12 +229,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(Args a) {
         for (int c = 0; c < NC; ++c) acc[d][c] *= alpha[c];
     }
 #pragma unroll
-    for (int rt = 0; rt < NR; rt += 2) {
-      f4 p[2][NC];
-#pragma unroll
-      for (int c = 0; c < NC; ++c) p[0][c] = s[rt][c], p[1][c] = s[rt + 1][c];
-      M::template accumulate<NC>(lv, rt, p, acc, lane);
-    }
+    for (int rt = 0; rt < NR; ++rt) M::template accumulate<NC>(lv, rt, s[rt], acc, lane);
   }
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
@@ -230,15 +240,11 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(Args a) {
     const int64_t row = (int64_t)(sq.lo + tok[c]) * a.H + head[c];
     if (a.part) {
       const int64_t at = (int64_t)(a.slot0 + split) * a.nq * a.H + row;
-      if (lane < 16) a.part_lse[at] = lse;
-#pragma unroll
-      for (int d = 0; d < M::NDT; ++d)
-        store4(a.part + at * a.D, 16 * d + 4 * (lane >> 4), a.D, acc[d][c] * inv, a.vec_o);
+      if (lane < 32) a.part_lse[at] = lse;
+      store_col(a.part + at * a.D, a.D, acc, c, inv, a.vec_o, lane);
     } else {
-      if (a.lse && lane < 16) a.lse[row] = lse;
-#pragma unroll
-      for (int d = 0; d < M::NDT; ++d)
-        store4((T*)a.out + row * a.D, 16 * d + 4 * (lane >> 4), a.D, acc[d][c] * inv, a.vec_o);
+      if (a.lse && lane < 32) a.lse[row] = lse;
+      store_col((T*)a.out + row * a.D, a.D, acc, c, inv, a.vec_o, lane);
     }
   }
 }
@@ -269,9 +275,9 @@ __global__ __launch_bounds__(256) void k_attn_join(const float* part, const floa
 // dQ: the forward's tiles again. With p = exp2(s - lse) from the forward's statistics and
 // delta = g.o, ds = p (g.v - delta), dq = scale sum ds k. Also writes delta for the pass over keys.
 template <typename T, int DP, int NC, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void k_attn_dq(Args a) {
+__global__ __launch_bounds__(NW * 64, DP <= 64 || (sizeof(T) == 2 && NW > 1) ? 2 : 1) void k_attn_dq(Args a) {
   typedef Mma<T, DP> M;
-  constexpr int BM = NC * NW * 16, BN = Tile<T, DP, NW>::BN, NR = Tile<T, DP, NW>::NR, NT = NW * 64;
+  constexpr int BM = NC * NW * 32, BN = Tile<T, DP, NW>::BN, NR = Tile<T, DP, NW>::NR, NT = NW * 64;
   typedef Stage<T, DP, BN, NT> St;
   __shared__ __align__(16) T lk[BN * St::LDW];
   __shared__ __align__(16) T lv[BN * St::LDW];
@@ -290,17 +296,17 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_dq(Args a) {
   bool ok[NC];
   float lse[NC], delta[NC];
   typename M::Frag qf[NC][M::KF], gf[NC][M::KF];
-  int kmin = sk.n;
+  int kmin = sk.n, kmax = 0;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    const int64_t r = r0 + (wave * NC + c) * 16 + (lane & 15);
+    const int64_t r = r0 + (wave * NC + c) * 32 + (lane & 31);
     ok[c] = r < nrow;
     tok[c] = ok[c] ? (int)(r / a.G) : 0;
     head[c] = kvh * a.G + (ok[c] ? (int)(r % a.G) : 0);
     int lim = sk.n;
     if (a.causal) lim = min(lim, max(0, tok[c] + 1 + sk.n - sq.n));
     klim[c] = ok[c] ? lim : 0;
-    if (ok[c]) kmin = min(kmin, lim);
+    if (ok[c]) kmin = min(kmin, lim), kmax = max(kmax, lim);
     const int64_t t = sq.lo + tok[c], row = t * a.H + head[c];
     M::load_cols(qf[c], (const T*)a.q + t * a.qs + (int64_t)head[c] * a.qh, ok[c], a.D, a.vec_q, lane);
     M::load_cols(gf[c], (const T*)a.go + t * a.gs + (int64_t)head[c] * a.gh, ok[c], a.D, a.vec_g, lane);
@@ -309,10 +315,13 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_dq(Args a) {
     delta[c] = col_sum(M::dot(gf[c], of));
     const float e = ok[c] ? a.lse[row] : neg_inf();
     lse[c] = e == neg_inf() ? __builtin_inff() : e;  // a row without keys: every weight is 0
-    if (ok[c] && lane < 16 && split == 0) a.delta[row] = delta[c];
+    if (ok[c] && lane < 32 && split == 0) a.delta[row] = delta[c];
   }
 #pragma unroll
-  for (int x = 8; x; x >>= 1) kmin = min(kmin, __shfl_xor(kmin, x));
+  for (int x = 16; x; x >>= 1) {
+    kmin = min(kmin, __shfl_xor(kmin, x));
+    kmax = max(kmax, __shfl_xor(kmax, x));
+  }
   int kend = sk.n;
   if (a.causal) {
     const int last = (int)((min(r0 + BM, nrow) - 1) / a.G);
@@ -327,11 +336,11 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_dq(Args a) {
   const Rows<T> kr = {(const T*)a.k + (int64_t)sk.lo * a.ks + (int64_t)kvh * a.kh, a.ks, a.D, a.vec_k != 0};
   const Rows<T> vr = {(const T*)a.v + (int64_t)sk.lo * a.vs + (int64_t)kvh * a.vh, a.vs, a.D, a.vec_v != 0};
   const uint8_t* mb = a.mask ? a.mask + sk.lo : nullptr;
-  f4 acc[M::NDT][NC];
+  f16v acc[M::NDT][NC];
 #pragma unroll
   for (int d = 0; d < M::NDT; ++d)
 #pragma unroll
-    for (int c = 0; c < NC; ++c) acc[d][c] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < NC; ++c) acc[d][c] = all_of(0.f);
   St stk, stv;
   uint8_t mk = 0;
   auto fetch = [&](int y0) {
@@ -348,31 +357,21 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_dq(Args a) {
     if (mb && tid < BN) lm[tid] = mk;
     __syncthreads();
     if (y0 + BN < kend) fetch(y0 + BN);
-    const bool need = mb || y0 + BN > min(kmin, kend);
+    if (y0 >= kmax) continue;
 #pragma unroll
-    for (int rt = 0; rt < NR; rt += 2) {
-      f4 s[2][NC];
+    for (int rt = 0; rt < NR; ++rt) {
+      f16v s[NC], dp[NC];
+      M::template scores<NC>(lk, rt, qf, s, all_of(0.f), lane);
+      M::template scores<NC>(lv, rt, gf, dp, all_of(0.f), lane);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        f4 dp[NC];
-        M::template scores<NC>(lk, rt + t, qf, s[t], f4{0.f, 0.f, 0.f, 0.f}, lane);
-        M::template scores<NC>(lv, rt + t, gf, dp, f4{0.f, 0.f, 0.f, 0.f}, lane);
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          s[c][r] = exp2_hw(fmaf(s[c][r], a.scale2, -lse[c])) * (dp[c][r] - delta[c]);
+      if (mb || y0 + BN > min(kmin, kend)) {
 #pragma unroll
         for (int c = 0; c < NC; ++c)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            s[t][c][r] = exp2_hw(fmaf(s[t][c][r], a.scale2, -lse[c])) * (dp[c][r] - delta[c]);
-        if (need) {
-          const int y = 16 * (rt + t) + 4 * (lane >> 4);
-          const uint32_t bytes = mb ? *(const uint32_t*)(lm + y) : 0x01010101u;
-#pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            const int lim = min(klim[c], kend) - y0 - y;
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (r >= lim || !(bytes & (0xffu << (8 * r)))) s[t][c][r] = 0.f;
-          }
-        }
+          hide(s[c], min(klim[c], kend) - y0 - 32 * rt, mb ? lm + 32 * rt : nullptr, 0.f, lane);
       }
       M::template accumulate<NC>(lk, rt, s, acc, lane);
     }
@@ -383,13 +382,9 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_dq(Args a) {
     const int64_t row = (int64_t)(sq.lo + tok[c]) * a.H + head[c];
     if (a.part) {
       const int64_t at = (int64_t)split * a.nq * a.H + row;
-#pragma unroll
-      for (int d = 0; d < M::NDT; ++d)
-        store4(a.part + at * a.D, 16 * d + 4 * (lane >> 4), a.D, acc[d][c] * a.scale, a.vec_o);
+      store_col(a.part + at * a.D, a.D, acc, c, a.scale, a.vec_o, lane);
     } else {
-#pragma unroll
-      for (int d = 0; d < M::NDT; ++d)
-        store4((T*)a.dq + row * a.D, 16 * d + 4 * (lane >> 4), a.D, acc[d][c] * a.scale, a.vec_o);
+      store_col((T*)a.dq + row * a.D, a.D, acc, c, a.scale, a.vec_o, lane);
     }
   }
 }
@@ -397,9 +392,9 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_dq(Args a) {
 // dK, dV: a tile of keys keeps its sums while the queries of its sequence stream by, the heads of
 // the group one after the other, so a shared key head's gradient is one sum in one order.
 template <typename T, int DP, int NC, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void k_attn_dkv(Args a) {
+__global__ __launch_bounds__(NW * 64, DP * sizeof(T) <= 128 ? 2 : 1) void k_attn_dkv(Args a) {
   typedef Mma<T, DP> M;
-  constexpr int BM = NC * NW * 16, BN = Tile<T, DP, NW>::BN, NR = Tile<T, DP, NW>::NR, NT = NW * 64;
+  constexpr int BM = NC * NW * 32, BN = Tile<T, DP, NW>::BN, NR = Tile<T, DP, NW>::NR, NT = NW * 64;
   typedef Stage<T, DP, BN, NT> St;
   __shared__ __align__(16) T lq[BN * St::LDW];
   __shared__ __align__(16) T lg[BN * St::LDW];
@@ -419,7 +414,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_dkv(Args a) {
   int qmax = 0;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    const int j = j0 + (wave * NC + c) * 16 + (lane & 15);
+    const int j = j0 + (wave * NC + c) * 32 + (lane & 31);
     ok[c] = j < sk.n;
     key[c] = sk.lo + (ok[c] ? j : 0);
     const bool seen = ok[c] && (!a.mask || a.mask[key[c]]);
@@ -429,12 +424,12 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_dkv(Args a) {
     M::load_cols(vf[c], (const T*)a.v + (int64_t)key[c] * a.vs + (int64_t)kvh * a.vh, seen, a.D, a.vec_v, lane);
   }
 #pragma unroll
-  for (int x = 8; x; x >>= 1) qmax = max(qmax, __shfl_xor(qmax, x));
-  f4 ak[M::NDT][NC], av[M::NDT][NC];
+  for (int x = 16; x; x >>= 1) qmax = max(qmax, __shfl_xor(qmax, x));
+  f16v ak[M::NDT][NC], av[M::NDT][NC];
 #pragma unroll
   for (int d = 0; d < M::NDT; ++d)
 #pragma unroll
-    for (int c = 0; c < NC; ++c) ak[d][c] = av[d][c] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < NC; ++c) ak[d][c] = av[d][c] = all_of(0.f);
   // tiles of queries, head after head
   const int tfirst = a.causal ? max(0, j0 - (sk.n - sq.n)) / BN : 0;
   const int nt = max(0, (sq.n + BN - 1) / BN - tfirst);
@@ -481,30 +476,26 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_dkv(Args a) {
     if (it + 1 < iend) fetch(it + 1);
     const bool need = y0 < qmax;
 #pragma unroll
-    for (int rt = 0; rt < NR; rt += 2) {
-      f4 p[2][NC], ds[2][NC];
+    for (int rt = 0; rt < NR; ++rt) {
+      f16v p[NC], ds[NC];
+      // the rows' statistics are where the products start from: s - lse / scale and dp - delta
+      M::template scores<NC>(lq, rt, kf, p, by_rows(ll + 32 * rt, lane), lane);
+      M::template scores<NC>(lg, rt, vf, ds, by_rows(ld + 32 * rt, lane), lane);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        // the rows' statistics are where the products start from: s - lse / scale and dp - delta
-        const int y = 16 * (rt + t) + 4 * (lane >> 4);
-        M::template scores<NC>(lq, rt + t, kf, p[t], *(const f4*)(ll + y), lane);
-        M::template scores<NC>(lg, rt + t, vf, ds[t], *(const f4*)(ld + y), lane);
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+        for (int r = 0; r < 16; ++r) p[c][r] = exp2_hw(p[c][r] * a.scale2);
+      if (need) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) p[t][c][r] = exp2_hw(p[t][c][r] * a.scale2);
-        if (need) {
+        for (int c = 0; c < NC; ++c) {
+          const int lim = qlim[c] - y0 - 32 * rt - 4 * (lane >> 5);
 #pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            const int lim = qlim[c] - y0 - y;
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (r < lim) p[t][c][r] = 0.f;
-          }
+          for (int r = 0; r < 16; ++r)
+            if (8 * (r >> 2) + (r & 3) < lim) p[c][r] = 0.f;
         }
-#pragma unroll
-        for (int c = 0; c < NC; ++c) ds[t][c] *= p[t][c];
       }
+#pragma unroll
+      for (int c = 0; c < NC; ++c) ds[c] *= p[c];
       M::template accumulate<NC>(lg, rt, p, av, lane);
       M::template accumulate<NC>(lq, rt, ds, ak, lane);
     }
@@ -513,19 +504,19 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_dkv(Args a) {
   for (int c = 0; c < NC; ++c) {
     if (!ok[c]) continue;
     const int64_t row = (int64_t)key[c] * a.Hkv + kvh;
+    if (a.shared)
 #pragma unroll
-    for (int d = 0; d < M::NDT; ++d) {
-      const int d0 = 16 * d + 4 * (lane >> 4);
-      f4 dk = ak[d][c] * a.scale;
-      if (a.shared) dk += av[d][c];
-      if (a.part) {
-        const int64_t at = ((int64_t)split * a.nk * a.Hkv + row) * a.D;
-        store4(a.part + at, d0, a.D, dk, a.vec_o);
-        if (!a.shared) store4(a.part2 + at, d0, a.D, av[d][c], a.vec_o);
-      } else {
-        store4((T*)a.dk + row * a.D, d0, a.D, dk, a.vec_o);
-        if (!a.shared) store4((T*)a.dv + row * a.D, d0, a.D, av[d][c], a.vec_o);
-      }
+      for (int d = 0; d < M::NDT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ak[d][c][r] = fmaf(ak[d][c][r], a.scale, av[d][c][r]);
+    const float f = a.shared ? 1.f : a.scale;
+    if (a.part) {
+      const int64_t at = ((int64_t)split * a.nk * a.Hkv + row) * a.D;
+      store_col(a.part + at, a.D, ak, c, f, a.vec_o, lane);
+      if (!a.shared) store_col(a.part2 + at, a.D, av, c, 1.f, a.vec_o, lane);
+    } else {
+      store_col((T*)a.dk + row * a.D, a.D, ak, c, f, a.vec_o, lane);
+      if (!a.shared) store_col((T*)a.dv + row * a.D, a.D, av, c, 1.f, a.vec_o, lane);
     }
   }
 }
@@ -544,16 +535,12 @@ __global__ __launch_bounds__(256) void k_sum_parts(const float* part, int n_part
 struct Shape {
   int nc, nw, bm;
 };
-// Short sequences (32 rows of a key head or fewer on average) leave most of a 64- or 128-row tile
-// empty: one wave with 16 columns per workgroup then.
-// (fp32 rows of more than 64 elements: a tile's way to LDS alone would take a wave's registers.)
-// Two columns of 16 per wave where the registers of two waves per SIMD hold them: not in fp32, and
-// not in the pass over keys, which keeps two sums, with more than 64 elements.
-Shape shape_for(int dtype, int D, bool two_sums, double rows_per_seq) {
-  const bool half = dtype == MONO_ROW_BF16;
-  if (rows_per_seq <= 32 && (half || D <= 64)) return {1, 1, 16};
-  const int nc = half && !(two_sums && D > 64) ? 2 : 1;
-  return {nc, 4, nc * 64};
+// Short sequences (64 rows of a key head or fewer on average) leave most of a 128-row tile empty: one
+// wave with 32 columns per workgroup then. (fp32 rows of more than 32 elements: a tile's way to LDS
+// alone would take a wave's registers.)
+Shape shape_for(int dtype, int D, double rows_per_seq) {
+  if (rows_per_seq <= 64 && (dtype == MONO_ROW_BF16 || D <= 32)) return {1, 1, 32};
+  return {1, 4, 128};
 }
 // Workgroups that fill the card some times over: few tiles are split along the streamed axis, down
 // to pieces of `least` rows.
@@ -618,11 +605,11 @@ struct Plan {
   int64_t tiles;
   int nsplit;
 };
-Plan plan_tiles(int dtype, int D, bool two_sums, int mode, int64_t B, int64_t n, int64_t G, int64_t heads,
+Plan plan_tiles(int dtype, int D, int mode, int64_t B, int64_t n, int64_t G, int64_t heads,
                 double stream_rows) {
   Plan pl;
   const double per = mode == kWhole ? (double)n * G : (double)n * G / std::max<int64_t>(1, B);
-  pl.sh = shape_for(dtype, D, two_sums, per);
+  pl.sh = shape_for(dtype, D, per);
   pl.tiles = tiles_for(mode, B, n, G, pl.sh.bm);
   pl.nsplit = splits_for(pl.tiles * heads, pl.sh.nw, stream_rows, 256);
   return pl;
@@ -630,11 +617,11 @@ Plan plan_tiles(int dtype, int D, bool two_sums, int mode, int64_t B, int64_t n,
 double average(int64_t n, int64_t B) { return (double)n / std::max<int64_t>(1, B); }
 
 Plan plan_fwd(const mono_attention_args* p) {
-  return plan_tiles(p->dtype, p->dim, false, p->query_splits ? kSplits : kOnePerSeq, p->batch, p->n_query,
+  return plan_tiles(p->dtype, p->dim, p->query_splits ? kSplits : kOnePerSeq, p->batch, p->n_query,
                     p->heads / p->kv_heads, p->kv_heads, average(p->n_key, p->batch));
 }
 Plan plan_dkv(const mono_attention_args* p) {
-  return plan_tiles(p->dtype, p->dim, true, kSplits, p->batch, p->n_key, 1, p->kv_heads,
+  return plan_tiles(p->dtype, p->dim, kSplits, p->batch, p->n_key, 1, p->kv_heads,
                     average(p->n_query, p->batch) * (p->heads / p->kv_heads));
 }
 
@@ -653,9 +640,9 @@ int launch2(const Args& a, const Plan& pl, hipStream_t st) {
   if (pl.tiles * a.Hkv == 0) return 0;
   MONO_REQUIRE(pl.tiles * a.Hkv < (1LL << 31), "attention: too many tiles");
   constexpr bool half = sizeof(T) == 2;
-  if constexpr (half || DP <= 64)
+  if constexpr (half || DP <= 32)
     if (pl.sh.nw == 1) return launch1<W, T, DP, 1, 1>(a, pl, st);
-  return launch1<W, T, DP, half && !(W == kDkv && DP > 64) ? 2 : 1, 4>(a, pl, st);
+  return launch1<W, T, DP, 1, 4>(a, pl, st);
 }
 template <int W>
 int launch(int dtype, const Args& a, const Plan& pl, hipStream_t st) {
@@ -664,7 +651,6 @@ int launch(int dtype, const Args& a, const Plan& pl, hipStream_t st) {
     if (a.D <= 64) return launch2<W, bf16, 64>(a, pl, st);
     return launch2<W, bf16, 128>(a, pl, st);
   }
-  if (a.D <= 16) return launch2<W, float, 16>(a, pl, st);
   if (a.D <= 32) return launch2<W, float, 32>(a, pl, st);
   if (a.D <= 64) return launch2<W, float, 64>(a, pl, st);
   return launch2<W, float, 128>(a, pl, st);
@@ -704,7 +690,7 @@ struct PrefixPlan {
 PrefixPlan plan_prefix(const mono_attention_args* p) {
   PrefixPlan r;
   const int64_t G = p->heads / p->kv_heads;
-  r.pre = plan_tiles(p->dtype, p->dim, false, kWhole, 1, p->n_query, G, p->kv_heads, (double)p->n_prefix);
+  r.pre = plan_tiles(p->dtype, p->dim, kWhole, 1, p->n_query, G, p->kv_heads, (double)p->n_prefix);
   r.slots = r.pre.nsplit;
   if (p->key_splits) {
     r.own = plan_fwd(p);

@@ -2,8 +2,8 @@
 // (softmax_ce.hip) share (gfx950 only).
 //
 // All of them are one scheme. A workgroup keeps a tile of rows X ("columns" of the products) in
-// registers as B operands and streams rows Y through LDS. A 16x16 matrix instruction gives
-// S[y][x] = Y X^T with x = lane & 15 and y = 4 * (lane >> 4) + r in accumulator r, so whatever
+// registers as B operands and streams rows Y through LDS. A 32x32 matrix instruction gives
+// S[y][x] = Y X^T with x = lane & 31 and y = tile_row(r, lane) in accumulator r, so whatever
 // belongs to a column (softmax maximum and sum, label, limit) is one register of a lane, and the
 // weights P = f(S) lie in the lanes exactly as the B operand of the second product
 // Z^T P = sum over y of Z[y][d] P[y][x] wants them, up to an order of the summation index y that
@@ -20,6 +20,7 @@ namespace seq {
 
 typedef __bf16 bf16;
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
 typedef bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef bf16 bf4 __attribute__((ext_vector_type(4)));
 typedef short s4 __attribute__((ext_vector_type(4)));
@@ -31,15 +32,9 @@ constexpr float kLn2 = 0.6931471805599453f;
 __device__ inline float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ inline float neg_inf() { return -__builtin_inff(); }
 
-// reductions over the four lanes that hold one column
-__device__ inline float col_max(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
-}
-__device__ inline float col_sum(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
-}
+// reductions over the two lanes that hold one column
+__device__ inline float col_max(float x) { return fmaxf(x, __shfl_xor(x, 32)); }
+__device__ inline float col_sum(float x) { return x + __shfl_xor(x, 32); }
 
 // Where a row of D elements starts, and how it may be read: `vec` rows start on 16 bytes and hold
 // whole 16-byte chunks.
@@ -118,26 +113,51 @@ struct Stage {
   }
 };
 
+// The 32x32 matrix instructions: a C tile gives lane l column l & 31 and, in register r, row
+// tile_row(r, l). They are taken in place of the 16x16 ones of the same rate because every matrix
+// instruction keeps the vector unit, which bounds these kernels, from issuing for a few cycles: on one
+// SIMD with four waves 16 exponentials and 8 16x16x32 take 203 cycles, with 4 32x32x16 171.
+__device__ inline int tile_row(int r, int lane) { return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3); }
+
+// a row statistic (one float per row of a 32-row tile, in LDS) in the place of every C register
+__device__ inline f16v by_rows(const float* x, int lane) {
+  f16v v;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const f4 t = *(const f4*)(x + 8 * q + 4 * (lane >> 5));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[4 * q + i] = t[i];
+  }
+  return v;
+}
+__device__ inline f16v all_of(float x) {
+  f16v v;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = x;
+  return v;
+}
+
 template <typename T, int DP>
 struct Mma;
 
-// bf16: 16x16x32, the operands' 8 elements of a lane are k = 8 * (lane >> 4) + j.
+// bf16: 32x32x16, the operands' 8 elements of a lane are k = 8 * (lane >> 5) + j.
 template <int DP>
 struct Mma<bf16, DP> {
-  static constexpr int KF = DP / 32, NDT = DP / 16, LDW = DP + 8;
+  static constexpr int KF = DP / 16, NDT = DP / 32, LDW = DP + 8;
   typedef bf8 Frag;
+  // s[c] = from + rows 32 rt .. of the tile times the columns' rows
   template <int NC>
-  static __device__ inline void scores(const bf16* lds, int rt, const Frag (&x)[NC][KF], f4 (&s)[NC],
-                                       f4 from, int lane) {
+  static __device__ inline void scores(const bf16* lds, int rt, const Frag (&x)[NC][KF], f16v (&s)[NC],
+                                       f16v from, int lane) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) s[c] = from;
-    const bf16* p = lds + (rt * 16 + (lane & 15)) * LDW + 8 * (lane >> 4);
+    const bf16* p = lds + (rt * 32 + (lane & 31)) * LDW + 8 * (lane >> 5);
 #pragma unroll
     for (int k = 0; k < KF; ++k) {
-      const bf8 a = *(const bf8*)(p + 32 * k);
+      const bf8 a = *(const bf8*)(p + 16 * k);
 #pragma unroll
       for (int c = 0; c < NC; ++c)
-        s[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, x[c][k], s[c], 0, 0, 0);
+        s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, x[c][k], s[c], 0, 0, 0);
     }
   }
   static __device__ inline void load_cols(Frag (&f)[KF], const bf16* row, bool ok, int D, bool vec,
@@ -145,7 +165,7 @@ struct Mma<bf16, DP> {
 #pragma unroll
     for (int k = 0; k < KF; ++k) {
       u4 c = {0u, 0u, 0u, 0u};
-      if (ok) c = load_chunk(row, 32 * k + 8 * (lane >> 4), D, vec);
+      if (ok) c = load_chunk(row, 16 * k + 8 * (lane >> 5), D, vec);
       f[k] = __builtin_bit_cast(bf8, c);
     }
   }
@@ -157,59 +177,59 @@ struct Mma<bf16, DP> {
       for (int j = 0; j < 8; ++j) t = fmaf((float)a[k][j], (float)b[k][j], t);
     return t;
   }
-  // Four rows y..y+3 of columns d0..d0+15 of a row-major tile, transposed: in every group of 16
+  // Four rows from y on of columns d0 .. d0 + 31 of a row-major tile, transposed: in every group of 16
   // lanes, lane i addresses 8 bytes (row i / 4, columns 4 * (i % 4)..) and receives column i.
   static __device__ inline s4 read_tr(const bf16* lds, int y, int d0, int lane) {
-    const bf16* p = lds + (y + ((lane & 15) >> 2)) * LDW + d0 + 4 * (lane & 3);
+    const bf16* p = lds + (y + ((lane & 15) >> 2)) * LDW + d0 + (lane & 16) + 4 * (lane & 3);
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p);
   }
-  // acc[dt][c] += sum over the 32 rows from 16 rt on of Z[y][16 dt + ..] P[y][x]. P is rounded to bf16 here:
-  // half a step of 2^-8 of every weight, independent from weight to weight, beside the one rounding
-  // of the result to the same type.
+  // acc[dt][c] += sum over the 32 rows from 32 rt on of Z[y][32 dt + ..] P[y][x]. P is rounded to bf16
+  // here: half a step of 2^-8 of every weight, independent from weight to weight, beside the one
+  // rounding of the result to the same type.
   template <int NC>
-  static __device__ inline void accumulate(const bf16* lds, int rt, const f4 (&p)[2][NC], f4 (&acc)[NDT][NC],
+  static __device__ inline void accumulate(const bf16* lds, int rt, const f16v (&p)[NC], f16v (&acc)[NDT][NC],
                                            int lane) {
-    bf8 b[NC];
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        b[c][j] = (bf16)p[0][c][j];
-        b[c][4 + j] = (bf16)p[1][c][j];
-      }
-    const int y = 16 * rt + 4 * (lane >> 4);
-#pragma unroll
-    for (int d = 0; d < NDT; ++d) {
-      const s4 lo = read_tr(lds, y, 16 * d, lane), hi = read_tr(lds, y + 16, 16 * d, lane);
-      const bf4 l = __builtin_bit_cast(bf4, lo), h = __builtin_bit_cast(bf4, hi);
-      const bf8 a = {l[0], l[1], l[2], l[3], h[0], h[1], h[2], h[3]};
+    for (int k = 0; k < 2; ++k) {
+      bf8 b[NC];
 #pragma unroll
       for (int c = 0; c < NC; ++c)
-        acc[d][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[c], acc[d][c], 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) b[c][j] = (bf16)p[c][8 * k + j];
+      const int y = 32 * rt + 16 * k + 4 * (lane >> 5);
+#pragma unroll
+      for (int d = 0; d < NDT; ++d) {
+        const bf4 l = __builtin_bit_cast(bf4, read_tr(lds, y, 32 * d, lane));
+        const bf4 h = __builtin_bit_cast(bf4, read_tr(lds, y + 8, 32 * d, lane));
+        const bf8 a = {l[0], l[1], l[2], l[3], h[0], h[1], h[2], h[3]};
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          acc[d][c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[c], acc[d][c], 0, 0, 0);
+      }
     }
   }
 };
 
-// fp32: 16x16x4, one element of a lane, k = lane >> 4. A lane's 16-byte chunk serves four
+// fp32: 32x32x2, one element of a lane, k = lane >> 5. A lane's 16-byte chunk serves four
 // instructions: which k slot stands for which element is free as long as both operands agree.
 template <int DP>
 struct Mma<float, DP> {
-  static constexpr int KF = DP / 16, NDT = DP / 16, LDW = DP + 4;
+  static constexpr int KF = DP / 8, NDT = DP / 32, LDW = DP + 4;
   typedef f4 Frag;
   template <int NC>
-  static __device__ inline void scores(const float* lds, int rt, const Frag (&x)[NC][KF], f4 (&s)[NC],
-                                       f4 from, int lane) {
+  static __device__ inline void scores(const float* lds, int rt, const Frag (&x)[NC][KF], f16v (&s)[NC],
+                                       f16v from, int lane) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) s[c] = from;
-    const float* p = lds + (rt * 16 + (lane & 15)) * LDW + 4 * (lane >> 4);
+    const float* p = lds + (rt * 32 + (lane & 31)) * LDW + 4 * (lane >> 5);
 #pragma unroll
     for (int k = 0; k < KF; ++k) {
-      const f4 a = *(const f4*)(p + 16 * k);
+      const f4 a = *(const f4*)(p + 8 * k);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int c = 0; c < NC; ++c)
-          s[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], x[c][k][j], s[c], 0, 0, 0);
+          s[c] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], x[c][k][j], s[c], 0, 0, 0);
     }
   }
   static __device__ inline void load_cols(Frag (&f)[KF], const float* row, bool ok, int D, bool vec,
@@ -217,7 +237,7 @@ struct Mma<float, DP> {
 #pragma unroll
     for (int k = 0; k < KF; ++k) {
       u4 c = {0u, 0u, 0u, 0u};
-      if (ok) c = load_chunk(row, 16 * k + 4 * (lane >> 4), D, vec);
+      if (ok) c = load_chunk(row, 8 * k + 4 * (lane >> 5), D, vec);
       f[k] = __builtin_bit_cast(f4, c);
     }
   }
@@ -230,21 +250,19 @@ struct Mma<float, DP> {
     return t;
   }
   template <int NC>
-  static __device__ inline void accumulate(const float* lds, int rt, const f4 (&p)[2][NC], f4 (&acc)[NDT][NC],
+  static __device__ inline void accumulate(const float* lds, int rt, const f16v (&p)[NC], f16v (&acc)[NDT][NC],
                                            int lane) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int r = 0; r < 16; ++r) {
+      const float* z = lds + (32 * rt + tile_row(r, lane)) * LDW + (lane & 31);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float* z = lds + (16 * (rt + t) + 4 * (lane >> 4) + r) * LDW + (lane & 15);
+      for (int d = 0; d < NDT; ++d) {
+        const float a = z[32 * d];
 #pragma unroll
-        for (int d = 0; d < NDT; ++d) {
-          const float a = z[16 * d];
-#pragma unroll
-          for (int c = 0; c < NC; ++c)
-            acc[d][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, p[t][c][r], acc[d][c], 0, 0, 0);
-        }
+        for (int c = 0; c < NC; ++c)
+          acc[d][c] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[c][r], acc[d][c], 0, 0, 0);
       }
+    }
   }
 };
 
@@ -267,6 +285,21 @@ __device__ inline void store4(T* row, int d0, int D, f4 v, bool vec) {
     for (int i = 0; i < 4; ++i)
       if (d0 + i < D) row[d0 + i] = (T)v[i];
   }
+}
+
+// column c of acc, times f, as a row of D elements
+template <typename T, int NDT, int NC>
+__device__ inline void store_col(T* row, int D, const f16v (&acc)[NDT][NC], int c, float f, bool vec, int lane) {
+#pragma unroll
+  for (int d = 0; d < NDT; ++d)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int d0 = 32 * d + 8 * q + 4 * (lane >> 5);
+      f4 v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = acc[d][c][4 * q + i] * f;
+      if (d0 < D) store4(row, d0, D, v, vec);
+    }
 }
 
 }  // namespace seq

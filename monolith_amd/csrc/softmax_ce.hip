@@ -26,7 +26,7 @@ struct Args {
 
 template <typename T>
 struct Tile {
-  static constexpr int BN = sizeof(T) == 2 ? 64 : 32, NR = BN / 16;
+  static constexpr int BN = sizeof(T) == 2 ? 64 : 32, NR = BN / 32;
 };
 
 // what the products of a candidate start from: its bias in units of scale
@@ -41,9 +41,9 @@ __device__ inline void range_of(int n, int nsplit, int split, int BN, int* beg, 
 
 // ---- forward: running maximum and sum of a tile of queries over one piece of the vocabulary ----
 template <typename T, int DP, int NC>
-__global__ __launch_bounds__(256, 2) void k_ce_fwd(Args a) {
+__global__ __launch_bounds__(256, DP <= 128 || sizeof(T) == 2 ? 2 : 1) void k_ce_fwd(Args a) {
   typedef Mma<T, DP> M;
-  constexpr int BM = NC * 64, BN = Tile<T>::BN, NR = Tile<T>::NR;
+  constexpr int BM = NC * 128, BN = Tile<T>::BN, NR = Tile<T>::NR;
   typedef Stage<T, DP, BN, 256> St;
   __shared__ __align__(16) T lw[BN * St::LDW];
   __shared__ __align__(16) float lb[BN];
@@ -53,7 +53,7 @@ __global__ __launch_bounds__(256, 2) void k_ce_fwd(Args a) {
   float m[NC], l[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    col[c] = blockIdx.x * BM + (wave * NC + c) * 16 + (lane & 15);
+    col[c] = blockIdx.x * BM + (wave * NC + c) * 32 + (lane & 31);
     const bool ok = col[c] < a.n;
     M::load_cols(qf[c], (const T*)a.q + (int64_t)(ok ? col[c] : 0) * a.qs, ok, a.D, a.vec_q, lane);
     m[c] = neg_inf();
@@ -76,11 +76,14 @@ __global__ __launch_bounds__(256, 2) void k_ce_fwd(Args a) {
     if (tid < BN) lb[tid] = eb;
     __syncthreads();
     if (y0 + BN < vend) fetch(y0 + BN);
-    f4 s[NR][NC];
+    f16v s[NR][NC];
 #pragma unroll
-    for (int rt = 0; rt < NR; ++rt)
-      M::template scores<NC>(lw, rt, qf, s[rt], *(const f4*)(lb + 16 * rt + 4 * (lane >> 4)), lane);
-    // every lane keeps the maximum and sum of the candidates that it holds itself; the four lanes
+    for (int rt = 0; rt < NR; ++rt) {
+      f16v from = all_of(0.f);
+      if (a.bias || y0 + BN > vend) from = by_rows(lb + 32 * rt, lane);
+      M::template scores<NC>(lw, rt, qf, s[rt], from, lane);
+    }
+    // every lane keeps the maximum and sum of the candidates that it holds itself; the two lanes
     // of a query are joined once, behind the loop. m is in units of scale (scale > 0).
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -88,14 +91,14 @@ __global__ __launch_bounds__(256, 2) void k_ce_fwd(Args a) {
 #pragma unroll
       for (int rt = 0; rt < NR; ++rt)
 #pragma unroll
-        for (int r = 0; r < 4; r += 2) mx = fmaxf(fmaxf(mx, s[rt][c][r]), s[rt][c][r + 1]);
+        for (int r = 0; r < 16; r += 2) mx = fmaxf(fmaxf(mx, s[rt][c][r]), s[rt][c][r + 1]);
       const float base = mx == neg_inf() ? 0.f : mx * a.scale2;
-      float sum = 0.f;
+      float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int rt = 0; rt < NR; ++rt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sum += exp2_hw(fmaf(s[rt][c][r], a.scale2, -base));
-      l[c] = fmaf(l[c], exp2_hw(fmaf(m[c], a.scale2, -base)), sum);
+        for (int r = 0; r < 16; ++r) sum[r & 1] += exp2_hw(fmaf(s[rt][c][r], a.scale2, -base));
+      l[c] = fmaf(l[c], exp2_hw(fmaf(m[c], a.scale2, -base)), sum[0] + sum[1]);
       m[c] = mx;
     }
   }
@@ -103,7 +106,7 @@ __global__ __launch_bounds__(256, 2) void k_ce_fwd(Args a) {
   for (int c = 0; c < NC; ++c) {
     const float mx = col_max(m[c]) * a.scale2, base = mx == neg_inf() ? 0.f : mx;
     const float sum = col_sum(l[c] * exp2_hw(fmaf(m[c], a.scale2, -base)));
-    if (lane < 16 && col[c] < a.n) {
+    if (lane < 32 && col[c] < a.n) {
       a.part[(int64_t)blockIdx.y * a.n + col[c]] = mx;
       a.part2[(int64_t)blockIdx.y * a.n + col[c]] = sum;
     }
@@ -161,9 +164,9 @@ __device__ inline f4 minus_label(const Args& a, int i, int d0, f4 t) {
 }
 
 template <typename T, int DP, int NC>
-__global__ __launch_bounds__(256, 2) void k_ce_dq(Args a) {
+__global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void k_ce_dq(Args a) {
   typedef Mma<T, DP> M;
-  constexpr int BM = NC * 64, BN = Tile<T>::BN, NR = Tile<T>::NR;
+  constexpr int BM = NC * 128, BN = Tile<T>::BN, NR = Tile<T>::NR;
   typedef Stage<T, DP, BN, 256> St;
   __shared__ __align__(16) T lw[BN * St::LDW];
   __shared__ __align__(16) float lb[BN];
@@ -171,15 +174,15 @@ __global__ __launch_bounds__(256, 2) void k_ce_dq(Args a) {
   int col[NC];
   typename M::Frag qf[NC][M::KF];
   float lse[NC];
-  f4 acc[M::NDT][NC];
+  f16v acc[M::NDT][NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    col[c] = blockIdx.x * BM + (wave * NC + c) * 16 + (lane & 15);
+    col[c] = blockIdx.x * BM + (wave * NC + c) * 32 + (lane & 31);
     const bool ok = col[c] < a.n;
     M::load_cols(qf[c], (const T*)a.q + (int64_t)(ok ? col[c] : 0) * a.qs, ok, a.D, a.vec_q, lane);
     lse[c] = ok ? a.lse[col[c]] : __builtin_inff();
 #pragma unroll
-    for (int d = 0; d < M::NDT; ++d) acc[d][c] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < M::NDT; ++d) acc[d][c] = all_of(0.f);
   }
   int vbeg, vend;
   range_of(a.v, a.nsplit, blockIdx.y, BN, &vbeg, &vend);
@@ -199,31 +202,33 @@ __global__ __launch_bounds__(256, 2) void k_ce_dq(Args a) {
     __syncthreads();
     if (y0 + BN < vend) fetch(y0 + BN);
 #pragma unroll
-    for (int rt = 0; rt < NR; rt += 2) {
-      f4 s[2][NC];
+    for (int rt = 0; rt < NR; ++rt) {
+      f16v s[NC], from = all_of(0.f);
+      if (a.bias || y0 + BN > vend) from = by_rows(lb + 32 * rt, lane);
+      M::template scores<NC>(lw, rt, qf, s, from, lane);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        M::template scores<NC>(lw, rt + t, qf, s[t], *(const f4*)(lb + 16 * (rt + t) + 4 * (lane >> 4)), lane);
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s[t][c][r] = exp2_hw(fmaf(s[t][c][r], a.scale2, -lse[c]));
-      }
+        for (int r = 0; r < 16; ++r) s[c][r] = exp2_hw(fmaf(s[c][r], a.scale2, -lse[c]));
       M::template accumulate<NC>(lw, rt, s, acc, lane);
     }
   }
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     if (col[c] >= a.n) continue;
-#pragma unroll
-    for (int d = 0; d < M::NDT; ++d) {
-      const int d0 = 16 * d + 4 * (lane >> 4);
-      if (a.part) {
-        store4(a.part + ((int64_t)blockIdx.y * a.n + col[c]) * a.D, d0, a.D, acc[d][c], a.vec_o);
-      } else if (d0 < a.D) {
-        store4((T*)a.dq + (int64_t)col[c] * a.D, d0, a.D, minus_label<T>(a, col[c], d0, acc[d][c]), a.vec_o);
-      }
+    if (a.part) {
+      store_col(a.part + ((int64_t)blockIdx.y * a.n + col[c]) * a.D, a.D, acc, c, 1.f, a.vec_o, lane);
+      continue;
     }
+#pragma unroll
+    for (int d = 0; d < M::NDT; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int d0 = 32 * d + 8 * q + 4 * (lane >> 5);
+        const f4 t = {acc[d][c][4 * q], acc[d][c][4 * q + 1], acc[d][c][4 * q + 2], acc[d][c][4 * q + 3]};
+        if (d0 < a.D)
+          store4((T*)a.dq + (int64_t)col[c] * a.D, d0, a.D, minus_label<T>(a, col[c], d0, t), a.vec_o);
+      }
   }
 }
 
@@ -249,29 +254,28 @@ __global__ __launch_bounds__(256) void k_ce_dq_join(Args a) {
 // a tile of candidates keeps its sums while all queries stream by. The label's share is rare: one
 // ballot per tile of queries says whether any label falls into the candidates of the workgroup.
 template <typename T, int DP, int NC>
-__global__ __launch_bounds__(256, 2) void k_ce_dw(Args a) {
+__global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void k_ce_dw(Args a) {
   typedef Mma<T, DP> M;
-  constexpr int BM = NC * 64, BN = Tile<T>::BN, NR = Tile<T>::NR;
+  constexpr int BM = NC * 128, BN = Tile<T>::BN, NR = Tile<T>::NR;
   typedef Stage<T, DP, BN, 256> St;
   __shared__ __align__(16) T lq[BN * St::LDW];
   __shared__ __align__(16) float ll[BN], lg[BN];
   __shared__ __align__(16) int lab[BN];
-  typedef int i4 __attribute__((ext_vector_type(4)));
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int v0 = blockIdx.x * BM;
   int col[NC];
   typename M::Frag wf[NC][M::KF];
   float b2[NC], sb[NC];
-  f4 acc[M::NDT][NC];
+  f16v acc[M::NDT][NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    col[c] = v0 + (wave * NC + c) * 16 + (lane & 15);
+    col[c] = v0 + (wave * NC + c) * 32 + (lane & 31);
     const bool ok = col[c] < a.v;
     b2[c] = !ok ? neg_inf() : a.bias ? a.bias[col[c]] * kLog2e : 0.f;
     M::load_cols(wf[c], (const T*)a.w + (int64_t)(ok ? col[c] : 0) * a.ws, b2[c] != neg_inf(), a.D, a.vec_w, lane);
     sb[c] = 0.f;
 #pragma unroll
-    for (int d = 0; d < M::NDT; ++d) acc[d][c] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < M::NDT; ++d) acc[d][c] = all_of(0.f);
   }
   int nbeg, nend;
   range_of(a.n, a.nsplit, blockIdx.y, BN, &nbeg, &nend);
@@ -309,31 +313,30 @@ __global__ __launch_bounds__(256, 2) void k_ce_dw(Args a) {
     const int mine = lab[lane & (BN - 1)];
     const bool hits = __any(mine >= v0 && mine < v0 + BM);
 #pragma unroll
-    for (int rt = 0; rt < NR; rt += 2) {
-      f4 s[2][NC];
+    for (int rt = 0; rt < NR; ++rt) {
+      f16v s[NC];
+      M::template scores<NC>(lq, rt, wf, s, by_rows(ll + 32 * rt, lane), lane);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int y = 16 * (rt + t) + 4 * (lane >> 4);
-        M::template scores<NC>(lq, rt + t, wf, s[t], *(const f4*)(ll + y), lane);
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[c][r] = exp2_hw(fmaf(s[c][r], a.scale2, b2[c]));
+      if (hits) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int label = lab[32 * rt + tile_row(r, lane)];
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+            if (label == col[c]) s[c][r] -= 1.f;
+        }
+      }
+      const f16v g = by_rows(lg + 32 * rt, lane);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) s[c] *= g;
+      if (a.db) {
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s[t][c][r] = exp2_hw(fmaf(s[t][c][r], a.scale2, b2[c]));
-        if (hits) {
-          const i4 lbl = *(const i4*)(lab + y);
-#pragma unroll
-          for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (lbl[r] == col[c]) s[t][c][r] -= 1.f;
-        }
-        const f4 g = *(const f4*)(lg + y);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) s[t][c] *= g;
-        if (a.db) {
-#pragma unroll
-          for (int c = 0; c < NC; ++c) sb[c] += (s[t][c][0] + s[t][c][1]) + (s[t][c][2] + s[t][c][3]);
-        }
+          for (int r = 0; r < 16; ++r) sb[c] += s[c][r];
       }
       M::template accumulate<NC>(lq, rt, s, acc, lane);
     }
@@ -343,14 +346,10 @@ __global__ __launch_bounds__(256, 2) void k_ce_dw(Args a) {
     const float b = col_sum(sb[c]);
     if (col[c] >= a.v) continue;
     const int64_t row = (a.nsplit > 1 ? (int64_t)blockIdx.y * a.v : 0) + col[c];
-    if (a.db && lane < 16) (a.nsplit > 1 ? a.part2 : a.db)[row] = b;
+    if (a.db && lane < 32) (a.nsplit > 1 ? a.part2 : a.db)[row] = b;
     if (!a.dw) continue;
-#pragma unroll
-    for (int d = 0; d < M::NDT; ++d) {
-      const int d0 = 16 * d + 4 * (lane >> 4);
-      if (a.nsplit > 1) store4(a.part + row * a.D, d0, a.D, acc[d][c] * a.scale, a.vec_o);
-      else store4((T*)a.dw + row * a.D, d0, a.D, acc[d][c] * a.scale, a.vec_o);
-    }
+    if (a.nsplit > 1) store_col(a.part + row * a.D, a.D, acc, c, a.scale, a.vec_o, lane);
+    else store_col((T*)a.dw + row * a.D, a.D, acc, c, a.scale, a.vec_o, lane);
   }
 }
 
@@ -364,10 +363,12 @@ __global__ __launch_bounds__(256) void k_ce_sum(const float* part, int n_part, i
 }
 
 // ---- host ----------------------------------------------------------------------------------
-int cols_of(const mono_softmax_ce_args* p) { return p->dtype == MONO_ROW_BF16 && p->dim <= 128 ? 2 : 1; }
+int cols_of(const mono_softmax_ce_args* p) {
+  return p->dtype == MONO_ROW_BF16 && p->dim <= 64 ? 2 : 1;
+}
 // tiles of `kept` rows, and pieces of the streamed rows that fill the card when there are few tiles
 int64_t tiles_of(const mono_softmax_ce_args* p, int64_t kept) {
-  const int bm = 64 * cols_of(p);
+  const int bm = 128 * cols_of(p);
   return (kept + bm - 1) / bm;
 }
 int pieces_of(const mono_softmax_ce_args* p, int64_t kept, int64_t streamed) {
@@ -414,10 +415,9 @@ int launch(int dtype, const Args& a, int64_t tiles, hipStream_t st) {
   if (dtype == MONO_ROW_BF16) {
     if (a.D <= 32) return launch1<W, bf16, 32, 2>(a, tiles, st);
     if (a.D <= 64) return launch1<W, bf16, 64, 2>(a, tiles, st);
-    if (a.D <= 128) return launch1<W, bf16, 128, 2>(a, tiles, st);
+    if (a.D <= 128) return launch1<W, bf16, 128, 1>(a, tiles, st);
     return launch1<W, bf16, 256, 1>(a, tiles, st);
   }
-  if (a.D <= 16) return launch1<W, float, 16, 1>(a, tiles, st);
   if (a.D <= 32) return launch1<W, float, 32, 1>(a, tiles, st);
   if (a.D <= 64) return launch1<W, float, 64, 1>(a, tiles, st);
   if (a.D <= 128) return launch1<W, float, 128, 1>(a, tiles, st);
