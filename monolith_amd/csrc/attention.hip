@@ -249,26 +249,59 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(Args a) {
   }
 }
 
-// out = sum of the splits' results, each weighted by its share of the softmax's sum
-template <typename T>
+// out = sum of the splits' results, each weighted by its share of the softmax's sum. W = 1: a thread
+// takes four elements of a row through all splits. Many splits of few rows (W = 4): a workgroup takes a
+// row, its 256 threads as 256 / ceil(D / 4) groups that each sum every so many-th split; joined in LDS.
+template <typename T, int W>
 __global__ __launch_bounds__(256) void k_attn_join(const float* part, const float* part_lse, int n_part,
-                                                   int64_t rows, int D, T* out, float* lse) {
-  const int64_t total = rows * D;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / D;
-    float m = neg_inf();
+                                                   int64_t rows, int D, T* out, float* lse, int vec) {
+  const int d4 = (D + 3) / 4;
+  __shared__ f4 sums[W == 1 ? 1 : 256];
+  __shared__ float zs[W == 1 ? 1 : 256];
+  const int groups = W == 1 ? 1 : 256 / d4;
+  const int64_t i = W == 1 ? (int64_t)blockIdx.x * 256 + threadIdx.x : blockIdx.x;
+  const int64_t row = W == 1 ? i / d4 : i;
+  const int d0 = (W == 1 ? (int)(i % d4) : threadIdx.x % d4) * 4, group = W == 1 ? 0 : threadIdx.x / d4;
+  if (row >= rows) return;  // (W = 4: the whole workgroup)
+  f4 t = {0.f, 0.f, 0.f, 0.f};
+  float z = 0.f, m = neg_inf();
+  if (W == 1) {
     for (int s = 0; s < n_part; ++s) m = fmaxf(m, part_lse[(int64_t)s * rows + row]);
-    float z = 0.f, t = 0.f;
-    for (int s = 0; s < n_part; ++s) {
+  } else {
+    for (int s = threadIdx.x; s < n_part; s += 256) m = fmaxf(m, part_lse[(int64_t)s * rows + row]);
+    for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+    if ((threadIdx.x & 63) == 0) zs[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(zs[0], zs[1]), fmaxf(zs[2], zs[3]));
+    __syncthreads();
+  }
+  if (group < groups)
+    for (int s = group; s < n_part; s += groups) {
       const float e = part_lse[(int64_t)s * rows + row];
       if (e == neg_inf()) continue;  // a split without a key: nothing was summed
       const float w = exp2_hw(e - m);
+      const float* p = part + ((int64_t)s * rows + row) * D + d0;
       z += w;
-      t = fmaf(w, part[(int64_t)s * total + i], t);
+      if (vec) {
+        t += w * *(const f4*)p;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (d0 + j < D) t[j] = fmaf(w, p[j], t[j]);
+      }
     }
-    out[i] = (T)(z == 0.f ? 0.f : t / z);
-    if (lse && i % D == 0) lse[row] = z == 0.f ? neg_inf() : m + __log2f(z);
+  if (W > 1) {
+    sums[threadIdx.x] = t;
+    zs[threadIdx.x] = z;
+    __syncthreads();
+    if (group) return;
+    for (int g = 1; g < groups; ++g) {
+      t += sums[g * d4 + threadIdx.x];
+      z += zs[g * d4 + threadIdx.x];
+    }
   }
+  store4(out + row * D, d0, D, t * (z == 0.f ? 0.f : 1.f / z), vec);
+  if (lse && d0 == 0) lse[row] = z == 0.f ? neg_inf() : m + __log2f(z);
 }
 
 // ---- backward ------------------------------------------------------------------------------
@@ -531,6 +564,265 @@ __global__ __launch_bounds__(256) void k_sum_parts(const float* part, int n_part
   }
 }
 
+// ---- one query per sequence -------------------------------------------------------------------
+// A pooled row reads every key once and computes 4 D operations for it: memory bound, and a matrix tile
+// would hold one column. One wave walks the keys of a sequence (or of its split): LPR lanes hold a key's
+// row, 16 bytes each, so a wave takes R = 64 / LPR keys at once and U times that per turn; every group
+// of LPR lanes keeps softmax statistics of its own, joined behind the loop. GT query heads of the key
+// head share what is read.
+template <typename T>
+struct Chunk {
+  static constexpr int E = 16 / sizeof(T);
+  float x[E];
+  __device__ inline void set(u4 w) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t t = w[i];
+      if constexpr (sizeof(T) == 4) {
+        x[i] = __uint_as_float(t);
+      } else {
+        x[2 * i] = __uint_as_float(t << 16);
+        x[2 * i + 1] = __uint_as_float(t & 0xffff0000u);
+      }
+    }
+  }
+  __device__ inline void clear() {
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] = 0.f;
+  }
+  __device__ inline float dot(const Chunk& o) const {
+    float t = x[0] * o.x[0];
+#pragma unroll
+    for (int i = 1; i < E; ++i) t = fmaf(x[i], o.x[i], t);
+    return t;
+  }
+  __device__ inline void add(float w, const Chunk& o) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] = fmaf(w, o.x[i], x[i]);
+  }
+  template <typename O>
+  __device__ inline void store(O* row, int e0, int D, bool vec, float f) const {
+#pragma unroll
+    for (int i = 0; i < E; i += 4)
+      if (e0 + i < D) store4(row, e0 + i, D, f4{x[i] * f, x[i + 1] * f, x[i + 2] * f, x[i + 3] * f}, vec);
+  }
+};
+template <int LPR>
+__device__ inline float row_sum(float t) {
+#pragma unroll
+  for (int x = 1; x < LPR; x <<= 1) t += __shfl_xor(t, x);
+  return t;
+}
+
+// the keys of a split
+__device__ inline void split_range(int n, int nsplit, int split, int step, int* beg, int* end) {
+  const int chunk = ((n + nsplit - 1) / nsplit + step - 1) / step * step;
+  *beg = (int)min((int64_t)n, (int64_t)split * chunk);
+  *end = (int)min((int64_t)n, (int64_t)*beg + chunk);
+}
+
+template <typename T, int DP, int GT>
+__global__ __launch_bounds__(256) void k_pool_fwd(Args a) {
+  constexpr int E = 16 / sizeof(T), LPR = DP / E, R = 64 / LPR, U = sizeof(T) == 4 ? 4 : 2;
+  const int lane = threadIdx.x & 63;
+  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (item >= (int64_t)a.B * a.Hkv * a.nsplit) return;
+  const int split = (int)(item % a.nsplit), kvh = (int)(item / a.nsplit % a.Hkv);
+  const int b = (int)(item / a.nsplit / a.Hkv);
+  const int sub = lane / LPR, e0 = lane % LPR * E;
+  const Seg sk = segment(a.ksp, kSplits, b, a.nk);
+  int beg, end;
+  split_range(sk.n, a.nsplit, split, R, &beg, &end);
+  const T* kb = (const T*)a.k + (int64_t)sk.lo * a.ks + (int64_t)kvh * a.kh;
+  const T* vb = (const T*)a.v + (int64_t)sk.lo * a.vs + (int64_t)kvh * a.vh;
+  const uint8_t* mb = a.mask ? a.mask + sk.lo : nullptr;
+  const bool same = a.k == a.v && a.ks == a.vs && a.kh == a.vh;
+  Chunk<T> q[GT], acc[GT];
+  float m[GT], l[GT];
+#pragma unroll
+  for (int g = 0; g < GT; ++g) {
+    const int head = kvh * a.G + g;
+    q[g].set(load_chunk((const T*)a.q + (int64_t)b * a.qs + (int64_t)head * a.qh, e0, a.D, a.vec_q));
+    acc[g].clear();
+    m[g] = neg_inf();
+    l[g] = 0.f;
+  }
+  for (int j0 = beg; j0 < end; j0 += R * U) {
+    u4 kw[U], vw[U];
+    bool in[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * R + sub;
+      in[u] = j < end && (!mb || mb[j]);
+      kw[u] = vw[u] = u4{0u, 0u, 0u, 0u};
+      if (in[u]) {
+        kw[u] = load_chunk(kb + (int64_t)j * a.ks, e0, a.D, a.vec_k);
+        if (!same) vw[u] = load_chunk(vb + (int64_t)j * a.vs, e0, a.D, a.vec_v);
+      }
+    }
+    Chunk<T> kc[U], vc[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      kc[u].set(kw[u]);
+      vc[u].set(same ? kw[u] : vw[u]);
+    }
+#pragma unroll
+    for (int g = 0; g < GT; ++g) {
+      float s[U], mx = m[g];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float t = row_sum<LPR>(q[g].dot(kc[u]));
+        s[u] = in[u] ? t : neg_inf();
+        mx = fmaxf(mx, s[u]);
+      }
+      const float base = mx == neg_inf() ? 0.f : mx * a.scale2;
+      const float alpha = exp2_hw(fmaf(m[g], a.scale2, -base));
+      m[g] = mx;
+      l[g] *= alpha;
+#pragma unroll
+      for (int i = 0; i < E; ++i) acc[g].x[i] *= alpha;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float p = exp2_hw(fmaf(s[u], a.scale2, -base));
+        l[g] += p;
+        acc[g].add(p, vc[u]);
+      }
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < GT; ++g) {
+    float mx = m[g];
+#pragma unroll
+    for (int x = LPR; x < 64; x <<= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
+    const float base = mx == neg_inf() ? 0.f : mx * a.scale2;
+    const float w = exp2_hw(fmaf(m[g], a.scale2, -base));
+    float lt = l[g] * w;
+#pragma unroll
+    for (int i = 0; i < E; ++i) acc[g].x[i] *= w;
+#pragma unroll
+    for (int x = LPR; x < 64; x <<= 1) {
+      lt += __shfl_xor(lt, x);
+#pragma unroll
+      for (int i = 0; i < E; ++i) acc[g].x[i] += __shfl_xor(acc[g].x[i], x);
+    }
+    if (sub) continue;
+    const float inv = lt == 0.f ? 0.f : 1.f / lt;
+    const float lse = lt == 0.f ? neg_inf() : fmaf(mx, a.scale2, __log2f(lt));
+    const int64_t row = (int64_t)b * a.H + kvh * a.G + g;
+    if (a.part) {
+      const int64_t at = (int64_t)(a.slot0 + split) * a.nq * a.H + row;
+      if (lane == 0) a.part_lse[at] = lse;
+      acc[g].store(a.part + at * a.D, e0, a.D, a.vec_o, inv);
+    } else {
+      if (a.lse && lane == 0) a.lse[row] = lse;
+      acc[g].store((T*)a.out + row * a.D, e0, a.D, a.vec_o, inv);
+    }
+  }
+}
+
+// The gradient in one pass over the keys: a wave that holds the query and its output's gradient makes
+// a key's weight again and writes the key's and value's gradients at once, which no other row shares;
+// the query's gradient is summed on the way. All GT = G heads of the key head together.
+template <typename T, int DP, int GT>
+__global__ __launch_bounds__(256) void k_pool_bwd(Args a) {
+  constexpr int E = 16 / sizeof(T), LPR = DP / E, R = 64 / LPR, U = 2;
+  const int lane = threadIdx.x & 63;
+  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t items = (int64_t)a.B * a.Hkv * a.nsplit;
+  const int sub = lane / LPR, e0 = lane % LPR * E;
+  Chunk<T> zero;
+  zero.clear();
+  if (item >= items) {  // the waves behind the last: rows of no sequence get zeros
+    if (!a.dk) return;
+    const int first = split_at(a.ksp, 0, a.nk), last = split_at(a.ksp, a.B, a.nk);
+    const int64_t others = ((int64_t)first + max(0, a.nk - last)) * a.Hkv, step = ((int64_t)gridDim.x * 4 - items) * R;
+    for (int64_t i = (item - items) * R + sub; i < others; i += step) {
+      const int64_t at = i < (int64_t)first * a.Hkv ? i : i - (int64_t)first * a.Hkv + (int64_t)last * a.Hkv;
+      zero.store((T*)a.dk + at * a.D, e0, a.D, a.vec_o, 0.f);
+      if (!a.shared) zero.store((T*)a.dv + at * a.D, e0, a.D, a.vec_o, 0.f);
+    }
+    return;
+  }
+  const int split = (int)(item % a.nsplit), kvh = (int)(item / a.nsplit % a.Hkv);
+  const int b = (int)(item / a.nsplit / a.Hkv);
+  const Seg sk = segment(a.ksp, kSplits, b, a.nk);
+  int beg, end;
+  split_range(sk.n, a.nsplit, split, R, &beg, &end);
+  const T* kb = (const T*)a.k + (int64_t)sk.lo * a.ks + (int64_t)kvh * a.kh;
+  const T* vb = (const T*)a.v + (int64_t)sk.lo * a.vs + (int64_t)kvh * a.vh;
+  const uint8_t* mb = a.mask ? a.mask + sk.lo : nullptr;
+  const bool same = a.k == a.v && a.ks == a.vs && a.kh == a.vh;
+  Chunk<T> q[GT], go[GT], dq[GT];
+  float lse[GT], delta[GT];
+#pragma unroll
+  for (int g = 0; g < GT; ++g) {
+    const int head = kvh * a.G + g;
+    const int64_t row = (int64_t)b * a.H + head;
+    Chunk<T> o;
+    q[g].set(load_chunk((const T*)a.q + (int64_t)b * a.qs + (int64_t)head * a.qh, e0, a.D, a.vec_q));
+    go[g].set(load_chunk((const T*)a.go + (int64_t)b * a.gs + (int64_t)head * a.gh, e0, a.D, a.vec_g));
+    o.set(load_chunk((const T*)a.o + row * a.D, e0, a.D, a.vec_o));
+    delta[g] = row_sum<LPR>(go[g].dot(o));
+    const float e = a.lse[row];
+    lse[g] = e == neg_inf() ? __builtin_inff() : e;
+    dq[g].clear();
+  }
+  for (int j0 = beg; j0 < end; j0 += R * U) {
+    u4 kw[U], vw[U];
+    bool in[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * R + sub;
+      in[u] = j < end && (!mb || mb[j]);
+      kw[u] = vw[u] = u4{0u, 0u, 0u, 0u};
+      if (in[u]) {
+        kw[u] = load_chunk(kb + (int64_t)j * a.ks, e0, a.D, a.vec_k);
+        if (!same) vw[u] = load_chunk(vb + (int64_t)j * a.vs, e0, a.D, a.vec_v);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * R + sub;
+      Chunk<T> kc, vc, dk, dv;
+      kc.set(kw[u]);
+      vc.set(same ? kw[u] : vw[u]);
+      dk.clear();
+      dv.clear();
+#pragma unroll
+      for (int g = 0; g < GT; ++g) {
+        const float s = row_sum<LPR>(q[g].dot(kc)), dp = row_sum<LPR>(go[g].dot(vc));
+        const float p = in[u] ? exp2_hw(fmaf(s, a.scale2, -lse[g])) : 0.f;
+        const float ds = p * (dp - delta[g]) * a.scale;
+        if (in[u]) {
+          dq[g].add(ds, kc);
+          dk.add(ds, q[g]);
+          if (a.shared) dk.add(p, go[g]);
+          else dv.add(p, go[g]);
+        }
+      }
+      if (a.dk && j < end) {
+        const int64_t at = ((int64_t)(sk.lo + j) * a.Hkv + kvh) * a.D;
+        dk.store((T*)a.dk + at, e0, a.D, a.vec_o, 1.f);
+        if (!a.shared) dv.store((T*)a.dv + at, e0, a.D, a.vec_o, 1.f);
+      }
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < GT; ++g) {
+#pragma unroll
+    for (int x = LPR; x < 64; x <<= 1)
+#pragma unroll
+      for (int i = 0; i < E; ++i) dq[g].x[i] += __shfl_xor(dq[g].x[i], x);
+    if (sub) continue;
+    const int64_t row = (int64_t)b * a.H + kvh * a.G + g;
+    if (a.part) {
+      dq[g].store(a.part + ((int64_t)split * a.nq * a.H + row) * a.D, e0, a.D, a.vec_o, 1.f);
+    } else {
+      dq[g].store((T*)a.dq + row * a.D, e0, a.D, a.vec_o, 1.f);
+    }
+  }
+}
+
 // ---- host ----------------------------------------------------------------------------------
 struct Shape {
   int nc, nw, bm;
@@ -601,6 +893,7 @@ Args base_args(const mono_attention_args* p) {
 
 // how one kernel's work is cut
 struct Plan {
+  bool pool;  // one query per sequence, by the kernels of their own
   Shape sh;
   int64_t tiles;
   int nsplit;
@@ -608,6 +901,7 @@ struct Plan {
 Plan plan_tiles(int dtype, int D, int mode, int64_t B, int64_t n, int64_t G, int64_t heads,
                 double stream_rows) {
   Plan pl;
+  pl.pool = false;
   const double per = mode == kWhole ? (double)n * G : (double)n * G / std::max<int64_t>(1, B);
   pl.sh = shape_for(dtype, D, per);
   pl.tiles = tiles_for(mode, B, n, G, pl.sh.bm);
@@ -616,7 +910,19 @@ Plan plan_tiles(int dtype, int D, int mode, int64_t B, int64_t n, int64_t G, int
 }
 double average(int64_t n, int64_t B) { return (double)n / std::max<int64_t>(1, B); }
 
+// One query per sequence: a wave per sequence and key head while a few heads share the keys; a group of
+// more than 4 heads fills enough of a matrix tile.
+bool is_pool(const mono_attention_args* p) { return !p->query_splits && p->heads / p->kv_heads <= 4; }
 Plan plan_fwd(const mono_attention_args* p) {
+  if (is_pool(p)) {
+    Plan pl{};
+    pl.pool = true;
+    pl.tiles = p->batch;
+    const int64_t waves = p->batch * p->kv_heads, want = 256 * 16;
+    const int64_t by_len = (int64_t)(average(p->n_key, p->batch) / 128);
+    pl.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want / std::max<int64_t>(1, waves), by_len), 256));
+    return pl;
+  }
   return plan_tiles(p->dtype, p->dim, p->query_splits ? kSplits : kOnePerSeq, p->batch, p->n_query,
                     p->heads / p->kv_heads, p->kv_heads, average(p->n_key, p->batch));
 }
@@ -635,6 +941,37 @@ int launch1(const Args& a, const Plan& pl, hipStream_t st) {
   MONO_HIP(hipGetLastError());
   return 0;
 }
+// the pooled kernels; backward: 64 more workgroups for the rows of no sequence
+template <int W, typename T, int DP, int GT>
+int launch_pool2(const Args& a, hipStream_t st) {
+  const int64_t wgs = ((int64_t)a.B * a.Hkv * a.nsplit + 3) / 4;
+  MONO_REQUIRE(wgs < (1LL << 31) - 64, "attention: too many sequences");
+  if (W == kFwd) k_pool_fwd<T, DP, GT><<<(unsigned)wgs, 256, 0, st>>>(a);
+  else k_pool_bwd<T, DP, GT><<<(unsigned)wgs + 64, 256, 0, st>>>(a);
+  MONO_HIP(hipGetLastError());
+  return 0;
+}
+template <int W, typename T, int DP>
+int launch_pool1(const Args& a, hipStream_t st) {
+  if (W == kFwd && a.B == 0) return 0;
+  if (a.G == 1) return launch_pool2<W, T, DP, 1>(a, st);
+  if (a.G == 2) return launch_pool2<W, T, DP, 2>(a, st);
+  if (a.G == 3) return launch_pool2<W, T, DP, 3>(a, st);
+  return launch_pool2<W, T, DP, 4>(a, st);
+}
+template <int W>
+int launch_pool(int dtype, const Args& a, hipStream_t st) {
+  if (dtype == MONO_ROW_BF16) {
+    if (a.D <= 16) return launch_pool1<W, bf16, 16>(a, st);
+    if (a.D <= 32) return launch_pool1<W, bf16, 32>(a, st);
+    if (a.D <= 64) return launch_pool1<W, bf16, 64>(a, st);
+    return launch_pool1<W, bf16, 128>(a, st);
+  }
+  if (a.D <= 16) return launch_pool1<W, float, 16>(a, st);
+  if (a.D <= 32) return launch_pool1<W, float, 32>(a, st);
+  if (a.D <= 64) return launch_pool1<W, float, 64>(a, st);
+  return launch_pool1<W, float, 128>(a, st);
+}
 template <int W, typename T, int DP>
 int launch2(const Args& a, const Plan& pl, hipStream_t st) {
   if (pl.tiles * a.Hkv == 0) return 0;
@@ -646,6 +983,7 @@ int launch2(const Args& a, const Plan& pl, hipStream_t st) {
 }
 template <int W>
 int launch(int dtype, const Args& a, const Plan& pl, hipStream_t st) {
+  if (pl.pool) return launch_pool<W>(dtype, a, st);
   if (dtype == MONO_ROW_BF16) {
     if (a.D <= 32) return launch2<W, bf16, 32>(a, pl, st);
     if (a.D <= 64) return launch2<W, bf16, 64>(a, pl, st);
@@ -664,11 +1002,19 @@ int64_t parts_bytes(int64_t n_part, int64_t rows, int64_t D) {
 int join(const mono_attention_args* p, const float* part, const float* part_lse, int n_part, hipStream_t st) {
   const int64_t rows = p->n_query * p->heads;
   if (rows == 0) return 0;
-  const int grid = grid_for(rows * p->dim, 256);
-  if (p->dtype == MONO_ROW_BF16)
-    k_attn_join<bf16><<<grid, 256, 0, st>>>(part, part_lse, n_part, rows, p->dim, (bf16*)p->out, p->lse);
+  const int vec = p->dim % 4 == 0 && ((uintptr_t)p->out & 15) == 0;
+  // a row's splits in one thread's turn cost a memory latency each: from 16 splits on a workgroup per row
+  const bool wide = n_part >= 16;
+  const unsigned grid = (unsigned)(wide ? rows : (rows * ((p->dim + 3) / 4) + 255) / 256);
+  const bool half = p->dtype == MONO_ROW_BF16;
+  if (half && wide)
+    k_attn_join<bf16, 4><<<grid, 256, 0, st>>>(part, part_lse, n_part, rows, p->dim, (bf16*)p->out, p->lse, vec);
+  else if (half)
+    k_attn_join<bf16, 1><<<grid, 256, 0, st>>>(part, part_lse, n_part, rows, p->dim, (bf16*)p->out, p->lse, vec);
+  else if (wide)
+    k_attn_join<float, 4><<<grid, 256, 0, st>>>(part, part_lse, n_part, rows, p->dim, (float*)p->out, p->lse, vec);
   else
-    k_attn_join<float><<<grid, 256, 0, st>>>(part, part_lse, n_part, rows, p->dim, (float*)p->out, p->lse);
+    k_attn_join<float, 1><<<grid, 256, 0, st>>>(part, part_lse, n_part, rows, p->dim, (float*)p->out, p->lse, vec);
   MONO_HIP(hipGetLastError());
   return 0;
 }
@@ -754,7 +1100,7 @@ int mono_ragged_attention_gradient(const mono_attention_args* p, void* stream) {
   a.part = plq.nsplit > 1 ? scratch : nullptr;
   MONO_TRY(launch<kDq>(p->dtype, a, plq, st));
   if (a.part) MONO_TRY(sum_parts(p->dtype, a.part, plq.nsplit, rows * p->dim, p->grad_query, st));
-  if (!p->grad_key) return 0;
+  if (!p->grad_key || plq.pool) return 0;  // (the pooled pass has written the keys' gradients)
   a.nsplit = plk.nsplit;
   a.part = plk.nsplit > 1 ? scratch : nullptr;
   a.part2 = a.part ? (float*)((char*)scratch + round16(plk.nsplit * krows * p->dim * 4)) : nullptr;
