@@ -96,3 +96,11 @@ def vp(x):
 def stream_ptr(device=None):
   import torch
   return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def launch(fn, args, device):
+  """fn(&args, current stream of `device`), with `device` the current one (a launch goes to it)."""
+  if device.index == torch.cuda.current_device():
+    return check(fn(C.byref(args), stream_ptr(device)))
+  with torch.cuda.device(device):
+    check(fn(C.byref(args), stream_ptr(device)))

@@ -129,8 +129,7 @@ def _call(fn, workspace, a: _lib.AttentionArgs, device) -> None:
   if n:
     ws = torch.empty(n, dtype=torch.uint8, device=device)
     a.workspace, a.workspace_bytes = ws.data_ptr(), n
-  with torch.cuda.device(device):
-    _lib.check(fn(C.byref(a), _lib.stream_ptr(device)))
+  _lib.launch(fn, a, device)
 
 
 def _forward(q, k, v, key_splits, query_splits, key_mask, causal, scale, with_lse):

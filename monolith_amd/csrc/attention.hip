@@ -609,9 +609,7 @@ struct Chunk {
 };
 template <int LPR>
 __device__ inline float row_sum(float t) {
-#pragma unroll
-  for (int x = 1; x < LPR; x <<= 1) t += __shfl_xor(t, x);
-  return t;
+  return over_lanes<1, LPR, Sum>(t);
 }
 
 // the keys of a split
@@ -691,20 +689,12 @@ __global__ __launch_bounds__(256) void k_pool_fwd(Args a) {
   }
 #pragma unroll
   for (int g = 0; g < GT; ++g) {
-    float mx = m[g];
-#pragma unroll
-    for (int x = LPR; x < 64; x <<= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
+    const float mx = over_lanes<LPR, 64, Max>(m[g]);
     const float base = mx == neg_inf() ? 0.f : mx * a.scale2;
     const float w = exp2_hw(fmaf(m[g], a.scale2, -base));
-    float lt = l[g] * w;
+    const float lt = over_lanes<LPR, 64, Sum>(l[g] * w);
 #pragma unroll
-    for (int i = 0; i < E; ++i) acc[g].x[i] *= w;
-#pragma unroll
-    for (int x = LPR; x < 64; x <<= 1) {
-      lt += __shfl_xor(lt, x);
-#pragma unroll
-      for (int i = 0; i < E; ++i) acc[g].x[i] += __shfl_xor(acc[g].x[i], x);
-    }
+    for (int i = 0; i < E; ++i) acc[g].x[i] = over_lanes<LPR, 64, Sum>(acc[g].x[i] * w);
     if (sub) continue;
     const float inv = lt == 0.f ? 0.f : 1.f / lt;
     const float lse = lt == 0.f ? neg_inf() : fmaf(mx, a.scale2, __log2f(lt));
@@ -810,9 +800,7 @@ __global__ __launch_bounds__(256) void k_pool_bwd(Args a) {
 #pragma unroll
   for (int g = 0; g < GT; ++g) {
 #pragma unroll
-    for (int x = LPR; x < 64; x <<= 1)
-#pragma unroll
-      for (int i = 0; i < E; ++i) dq[g].x[i] += __shfl_xor(dq[g].x[i], x);
+    for (int i = 0; i < E; ++i) dq[g].x[i] = over_lanes<LPR, 64, Sum>(dq[g].x[i]);
     if (sub) continue;
     const int64_t row = (int64_t)b * a.H + kvh * a.G + g;
     if (a.part) {
@@ -834,14 +822,13 @@ Shape shape_for(int dtype, int D, double rows_per_seq) {
   if (rows_per_seq <= 64 && (dtype == MONO_ROW_BF16 || D <= 32)) return {1, 1, 32};
   return {1, 4, 128};
 }
-// Workgroups that fill the card some times over: few tiles are split along the streamed axis, down
-// to pieces of `least` rows.
-int splits_for(int64_t tiles, int nw, double stream_rows, int least) {
-  const int64_t want = nw == 1 ? 256 * 12 : 256 * 3;
+// Few tiles are split along the streamed axis into as many workgroups as the card holds at once (a
+// rest would run alone on it: prefix_lifelong took 256 us in 768 workgroups of which it holds 512), in
+// pieces of 64 rows or more.
+int splits_for(int64_t tiles, int nw, int D, double stream_rows) {
+  const int64_t want = 256 * (nw == 1 ? 12 : D <= 32 ? 4 : D <= 64 ? 3 : 2);
   if (tiles <= 0 || tiles >= want) return 1;
-  const int64_t by_len = (int64_t)(stream_rows / least);
-  int64_t n = std::min((want + tiles - 1) / tiles, by_len);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(n, 256));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want / tiles, (int64_t)(stream_rows / 64)), 256));
 }
 
 bool aligned_rows(const mono_rows& r, int dtype, int D) {
@@ -905,7 +892,7 @@ Plan plan_tiles(int dtype, int D, int mode, int64_t B, int64_t n, int64_t G, int
   const double per = mode == kWhole ? (double)n * G : (double)n * G / std::max<int64_t>(1, B);
   pl.sh = shape_for(dtype, D, per);
   pl.tiles = tiles_for(mode, B, n, G, pl.sh.bm);
-  pl.nsplit = splits_for(pl.tiles * heads, pl.sh.nw, stream_rows, 256);
+  pl.nsplit = splits_for(pl.tiles * heads, pl.sh.nw, D, stream_rows);
   return pl;
 }
 double average(int64_t n, int64_t B) { return (double)n / std::max<int64_t>(1, B); }

@@ -32,9 +32,51 @@ constexpr float kLn2 = 0.6931471805599453f;
 __device__ inline float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ inline float neg_inf() { return -__builtin_inff(); }
 
-// reductions over the two lanes that hold one column
-__device__ inline float col_max(float x) { return fmaxf(x, __shfl_xor(x, 32)); }
-__device__ inline float col_sum(float x) { return x + __shfl_xor(x, 32); }
+// x of the lane with the other bit 5 (16) or 4 of its number, and both values in every lane: the lane
+// swaps and row permutations of the vector unit, not the LDS permutation that __shfl_xor takes
+__device__ inline float swap32(float x, float* other) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  *other = __uint_as_float(p[1]);
+  return __uint_as_float(p[0]);
+}
+__device__ inline float swap16(float x, float* other) {
+  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  *other = __uint_as_float(p[1]);
+  return __uint_as_float(p[0]);
+}
+template <int CTRL>
+__device__ inline float dpp(float x) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+struct Sum {
+  static __device__ inline float of(float a, float b) { return a + b; }
+};
+struct Max {
+  static __device__ inline float of(float a, float b) { return fmaxf(a, b); }
+};
+// Op over groups of lanes, the result in every lane: over lanes FROM apart and more, up to TO lanes.
+// From 1 on the partners hold equal values by the time that halves and rows are mirrored; lanes that
+// stay apart need the exact partner.
+template <int FROM, int TO, typename Op>
+__device__ inline float over_lanes(float x) {
+  float y;
+  if constexpr (FROM <= 1 && TO > 1) x = Op::of(x, dpp<0xB1>(x));
+  if constexpr (FROM <= 2 && TO > 2) x = Op::of(x, dpp<0x4E>(x));
+  if constexpr (FROM <= 4 && TO > 4) x = Op::of(x, FROM > 1 ? __shfl_xor(x, 4) : dpp<0x141>(x));
+  if constexpr (FROM <= 8 && TO > 8) x = Op::of(x, FROM > 1 ? dpp<0x128>(x) : dpp<0x140>(x));
+  if constexpr (FROM <= 16 && TO > 16) {
+    x = swap16(x, &y);
+    x = Op::of(x, y);
+  }
+  if constexpr (FROM <= 32 && TO > 32) {
+    x = swap32(x, &y);
+    x = Op::of(x, y);
+  }
+  return x;
+}
+// over the two lanes that hold one column
+__device__ inline float col_max(float x) { return over_lanes<32, 64, Max>(x); }
+__device__ inline float col_sum(float x) { return over_lanes<32, 64, Sum>(x); }
 
 // Where a row of D elements starts, and how it may be read: `vec` rows start on 16 bytes and hold
 // whole 16-byte chunks.

@@ -374,7 +374,7 @@ int64_t tiles_of(const mono_softmax_ce_args* p, int64_t kept) {
 int pieces_of(const mono_softmax_ce_args* p, int64_t kept, int64_t streamed) {
   const int64_t tiles = tiles_of(p, kept), want = 256 * 4;
   if (tiles >= want) return 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>((want + tiles - 1) / std::max<int64_t>(1, tiles), streamed / 256));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(want / std::max<int64_t>(1, tiles), streamed / 64));
 }
 
 int check(const mono_softmax_ce_args* p, const char* who) {

@@ -38,8 +38,7 @@ def _call(fn, workspace, a, device) -> None:
   if n:
     ws = torch.empty(n, dtype=torch.uint8, device=device)
     a.workspace, a.workspace_bytes = ws.data_ptr(), n
-  with torch.cuda.device(device):
-    _lib.check(fn(C.byref(a), _lib.stream_ptr(device)))
+  _lib.launch(fn, a, device)
 
 
 def _forward(query, rows, labels, bias, scale):
