@@ -85,10 +85,10 @@ int64_t tiles_for(int mode, int64_t B, int64_t n, int64_t G, int BM) {
   return n * G / BM + B + 2;
 }
 
-// rows of a streamed tile: fewer where the registers that hold it on its way to LDS are few
+// rows of a streamed tile: 64 where one takes the registers of 64 bytes a thread or less on its way to LDS
 template <typename T, int DP, int NW>
 struct Tile {
-  static constexpr int BN = sizeof(T) == 2 && NW > 1 && DP <= 64 ? 64 : 32, NR = BN / 32;
+  static constexpr int BN = NW > 1 && DP * sizeof(T) <= 128 ? 64 : 32, NR = BN / 32;
 };
 
 // v where a column's key (rows y of a tile, from its row 0 on) is not below lim or not alive
@@ -105,12 +105,12 @@ __device__ inline void hide(f16v& s, int lim, const uint8_t* alive, float v, int
 
 // ---- forward -------------------------------------------------------------------------------
 template <typename T, int DP, int NC, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(Args a) {
-  typedef Mma<T, DP> M;
+__global__ __launch_bounds__(NW * 64, DP * sizeof(T) <= 256 ? 2 : 1) void k_attn_fwd(Args a) {
   constexpr int BM = NC * NW * 32, BN = Tile<T, DP, NW>::BN, NR = Tile<T, DP, NW>::NR, NT = NW * 64;
   typedef Stage<T, DP, BN, NT> St;
-  __shared__ __align__(16) T lk[BN * St::LDW];
-  __shared__ __align__(16) T lv[BN * St::LDW];
+  typedef Mma<T, DP, St::PLANE> M;
+  __shared__ __align__(16) bf16 lk[St::LDS];
+  __shared__ __align__(16) bf16 lv[St::LDS];
   __shared__ __align__(16) uint8_t lm[BN];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int kvh = blockIdx.x % a.Hkv, split = blockIdx.y;
@@ -309,11 +309,11 @@ __global__ __launch_bounds__(256) void k_attn_join(const float* part, const floa
 // delta = g.o, ds = p (g.v - delta), dq = scale sum ds k. Also writes delta for the pass over keys.
 template <typename T, int DP, int NC, int NW>
 __global__ __launch_bounds__(NW * 64, DP <= 64 || (sizeof(T) == 2 && NW > 1) ? 2 : 1) void k_attn_dq(Args a) {
-  typedef Mma<T, DP> M;
   constexpr int BM = NC * NW * 32, BN = Tile<T, DP, NW>::BN, NR = Tile<T, DP, NW>::NR, NT = NW * 64;
   typedef Stage<T, DP, BN, NT> St;
-  __shared__ __align__(16) T lk[BN * St::LDW];
-  __shared__ __align__(16) T lv[BN * St::LDW];
+  typedef Mma<T, DP, St::PLANE> M;
+  __shared__ __align__(16) bf16 lk[St::LDS];
+  __shared__ __align__(16) bf16 lv[St::LDS];
   __shared__ __align__(16) uint8_t lm[BN];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int kvh = blockIdx.x % a.Hkv, split = blockIdx.y;
@@ -426,11 +426,11 @@ __global__ __launch_bounds__(NW * 64, DP <= 64 || (sizeof(T) == 2 && NW > 1) ? 2
 // the group one after the other, so a shared key head's gradient is one sum in one order.
 template <typename T, int DP, int NC, int NW>
 __global__ __launch_bounds__(NW * 64, DP * sizeof(T) <= 128 ? 2 : 1) void k_attn_dkv(Args a) {
-  typedef Mma<T, DP> M;
   constexpr int BM = NC * NW * 32, BN = Tile<T, DP, NW>::BN, NR = Tile<T, DP, NW>::NR, NT = NW * 64;
   typedef Stage<T, DP, BN, NT> St;
-  __shared__ __align__(16) T lq[BN * St::LDW];
-  __shared__ __align__(16) T lg[BN * St::LDW];
+  typedef Mma<T, DP, St::PLANE> M;
+  __shared__ __align__(16) bf16 lq[St::LDS];
+  __shared__ __align__(16) bf16 lg[St::LDS];
   __shared__ __align__(16) float ll[BN], ld[BN];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int kvh = blockIdx.x % a.Hkv, split = blockIdx.y;
@@ -972,10 +972,12 @@ template <int W>
 int launch(int dtype, const Args& a, const Plan& pl, hipStream_t st) {
   if (pl.pool) return launch_pool<W>(dtype, a, st);
   if (dtype == MONO_ROW_BF16) {
+    if (a.D <= 16) return launch2<W, bf16, 16>(a, pl, st);
     if (a.D <= 32) return launch2<W, bf16, 32>(a, pl, st);
     if (a.D <= 64) return launch2<W, bf16, 64>(a, pl, st);
     return launch2<W, bf16, 128>(a, pl, st);
   }
+  if (a.D <= 16) return launch2<W, float, 16>(a, pl, st);
   if (a.D <= 32) return launch2<W, float, 32>(a, pl, st);
   if (a.D <= 64) return launch2<W, float, 64>(a, pl, st);
   return launch2<W, float, 128>(a, pl, st);

@@ -8,7 +8,7 @@
 // weights P = f(S) lie in the lanes exactly as the B operand of the second product
 // Z^T P = sum over y of Z[y][d] P[y][x] wants them, up to an order of the summation index y that
 // the A operand Z^T follows: P never goes through LDS. Z^T comes out of the row-major LDS tile by
-// the transposing LDS read (bf16) or by 4-byte reads (fp32).
+// the transposing LDS read.
 #ifndef MONO_SEQ_DEV_H_
 #define MONO_SEQ_DEV_H_
 
@@ -102,17 +102,38 @@ struct Rows {
   bool vec;         // rows start on 16 bytes and are whole 16-byte chunks
 };
 
+// fp32 rows go through the bf16 matrix instructions as three bf16 numbers each, x = hi + mid + lo, every
+// one the rounded rest of those before: 24 bits, as many as x has. Of the nine products of two such
+// sums the six that reach 2^-24 of the whole are taken (hi hi, hi mid, mid hi, mid mid, hi lo, lo hi),
+// so a product is off by about 2^-25 of its size, less than the 32-bit sum it goes into, at 6/16 of the
+// fp32 matrix instructions' time. (An infinite element gives NaN; the hi of a number within 2^-9 of the
+// largest is infinite.)
+template <typename T>
+constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
+
+__device__ inline void split3(const float* x, int n, bf16* hi, bf16* mid, bf16* lo) {
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    hi[i] = (bf16)x[i];
+    const float r = x[i] - (float)hi[i];
+    mid[i] = (bf16)r;
+    lo[i] = (bf16)(r - (float)mid[i]);
+  }
+}
+
 // A tile of BN rows on its way from global memory to LDS: load() takes the thread's chunks into
-// registers, store() writes them. Rows outside [0, n) and rows that are not alive(row) become zeros,
-// so that nothing that lies in such a row reaches a product; what alive() reads is read beside the
-// row and needed only by store().
+// registers, store() writes them, one plane of bf16 behind the other. Rows outside [0, n) and rows that
+// are not alive(row) become zeros, so that nothing that lies in such a row reaches a product; what
+// alive() reads is read beside the row and needed only by store().
 template <typename T, int DP, int BN, int NT>
 struct Stage {
   static constexpr int E = 16 / sizeof(T);   // elements of a chunk
   static constexpr int CH = DP / E;          // chunks of a row
   static constexpr int PER = (BN * CH + NT - 1) / NT;
   static constexpr int STEP = NT / CH;       // rows between a thread's chunks
-  static constexpr int LDW = DP + E;         // LDS row: 16 bytes of padding against bank conflicts
+  static constexpr int LDW = DP + 8;         // LDS row: 16 bytes of padding against bank conflicts
+  // (16 more elements: the transposing read of rows of 16 takes 32 columns, of which it uses 16)
+  static constexpr int PLANE = BN * LDW + (DP < 32 ? 16 : 0), LDS = kPlanes<T> * PLANE;
   static_assert(NT % CH == 0 && (PER == 1 || BN * CH % NT == 0), "every thread holds one column of chunks");
   u4 r[PER];
   bool live[PER];
@@ -145,12 +166,25 @@ struct Stage {
       for (int i = 0; i < PER; ++i)
         if (mine && row + i * STEP < n) live[i] = alive(row + i * STEP);
   }
-  __device__ inline void store(T* lds, int tid, bool filter) const {
+  __device__ inline void store(bf16* lds, int tid, bool filter) const {
     if (PER > 1 || tid < BN * CH) {
-      T* p = lds + tid / CH * LDW + tid % CH * E;
+      bf16* p = lds + tid / CH * LDW + tid % CH * E;
 #pragma unroll
-      for (int i = 0; i < PER; ++i)
-        *(u4*)(p + i * STEP * LDW) = !filter || live[i] ? r[i] : u4{0u, 0u, 0u, 0u};
+      for (int i = 0; i < PER; ++i) {
+        const u4 w = !filter || live[i] ? r[i] : u4{0u, 0u, 0u, 0u};
+        bf16* to = p + i * STEP * LDW;
+        if constexpr (sizeof(T) == 2) {
+          *(u4*)to = w;
+        } else {
+          const f4 x = __builtin_bit_cast(f4, w);
+          const float v[4] = {x[0], x[1], x[2], x[3]};
+          bf16 h[4], m[4], l[4];
+          split3(v, 4, h, m, l);
+          *(bf4*)to = bf4{h[0], h[1], h[2], h[3]};
+          *(bf4*)(to + PLANE) = bf4{m[0], m[1], m[2], m[3]};
+          *(bf4*)(to + 2 * PLANE) = bf4{l[0], l[1], l[2], l[3]};
+        }
+      }
     }
   }
 };
@@ -179,14 +213,21 @@ __device__ inline f16v all_of(float x) {
   return v;
 }
 
-template <typename T, int DP>
-struct Mma;
-
-// bf16: 32x32x16, the operands' 8 elements of a lane are k = 8 * (lane >> 5) + j.
-template <int DP>
-struct Mma<bf16, DP> {
-  static constexpr int KF = DP / 16, NDT = DP / 32, LDW = DP + 8;
-  typedef bf8 Frag;
+// 32x32x16: the operands' 8 elements of a lane are k = 8 * (lane >> 5) + j.
+template <typename T, int DP, int PLANE>
+struct Mma {
+  static constexpr int PL = kPlanes<T>, KF = DP / 16, NDT = (DP + 31) / 32, LDW = DP + 8;
+  struct Frag {
+    bf8 p[PL];
+  };
+  static __device__ inline f16v product(const Frag& a, const Frag& b, f16v c) {
+#pragma unroll
+    for (int i = PL - 1; i >= 0; --i)  // the small ones first
+#pragma unroll
+      for (int j = 0; j < PL; ++j)
+        if (i + j < PL) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[i], b.p[j], c, 0, 0, 0);
+    return c;
+  }
   // s[c] = from + rows 32 rt .. of the tile times the columns' rows
   template <int NC>
   static __device__ inline void scores(const bf16* lds, int rt, const Frag (&x)[NC][KF], f16v (&s)[NC],
@@ -196,113 +237,89 @@ struct Mma<bf16, DP> {
     const bf16* p = lds + (rt * 32 + (lane & 31)) * LDW + 8 * (lane >> 5);
 #pragma unroll
     for (int k = 0; k < KF; ++k) {
-      const bf8 a = *(const bf8*)(p + 16 * k);
+      Frag a;
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-        s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, x[c][k], s[c], 0, 0, 0);
+      for (int i = 0; i < PL; ++i) a.p[i] = *(const bf8*)(p + i * PLANE + 16 * k);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) s[c] = product(a, x[c][k], s[c]);
     }
   }
-  static __device__ inline void load_cols(Frag (&f)[KF], const bf16* row, bool ok, int D, bool vec,
-                                          int lane) {
+  static __device__ inline void load_cols(Frag (&f)[KF], const T* row, bool ok, int D, bool vec, int lane) {
 #pragma unroll
     for (int k = 0; k < KF; ++k) {
-      u4 c = {0u, 0u, 0u, 0u};
-      if (ok) c = load_chunk(row, 16 * k + 8 * (lane >> 5), D, vec);
-      f[k] = __builtin_bit_cast(bf8, c);
+      const int e0 = 16 * k + 8 * (lane >> 5);
+      u4 c[2] = {{0u, 0u, 0u, 0u}, {0u, 0u, 0u, 0u}};
+      if (ok) c[0] = load_chunk(row, e0, D, vec);
+      if constexpr (PL == 1) {
+        f[k].p[0] = __builtin_bit_cast(bf8, c[0]);
+      } else {
+        if (ok) c[1] = load_chunk(row, e0 + 4, D, vec);
+        const f4 x = __builtin_bit_cast(f4, c[0]), y = __builtin_bit_cast(f4, c[1]);
+        const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        f[k] = frag(v);
+      }
     }
+  }
+  static __device__ inline Frag frag(const float* v) {
+    Frag f;
+    if constexpr (PL == 1) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f.p[0][j] = (bf16)v[j];
+    } else {
+      bf16 h[8], m[8], l[8];
+      split3(v, 8, h, m, l);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f.p[0][j] = h[j], f.p[1][j] = m[j], f.p[2][j] = l[j];
+    }
+    return f;
+  }
+  static __device__ inline float whole(const Frag& f, int j) {
+    float t = (float)f.p[0][j];
+#pragma unroll
+    for (int i = 1; i < PL; ++i) t += (float)f.p[i][j];
+    return t;
   }
   static __device__ inline float dot(const Frag (&a)[KF], const Frag (&b)[KF]) {
     float t = 0.f;
 #pragma unroll
     for (int k = 0; k < KF; ++k)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) t = fmaf((float)a[k][j], (float)b[k][j], t);
+      for (int j = 0; j < 8; ++j) t = fmaf(whole(a[k], j), whole(b[k], j), t);
     return t;
   }
   // Four rows from y on of columns d0 .. d0 + 31 of a row-major tile, transposed: in every group of 16
   // lanes, lane i addresses 8 bytes (row i / 4, columns 4 * (i % 4)..) and receives column i.
-  static __device__ inline s4 read_tr(const bf16* lds, int y, int d0, int lane) {
+  static __device__ inline bf4 read_tr(const bf16* lds, int y, int d0, int lane) {
     const bf16* p = lds + (y + ((lane & 15) >> 2)) * LDW + d0 + (lane & 16) + 4 * (lane & 3);
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p);
+    return __builtin_bit_cast(bf4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p));
   }
-  // acc[dt][c] += sum over the 32 rows from 32 rt on of Z[y][32 dt + ..] P[y][x]. P is rounded to bf16
-  // here: half a step of 2^-8 of every weight, independent from weight to weight, beside the one
-  // rounding of the result to the same type.
+  // acc[dt][c] += sum over the 32 rows from 32 rt on of Z[y][32 dt + ..] P[y][x]. For bf16 rows P is
+  // rounded to bf16 here: half a step of 2^-8 of every weight, independent from weight to weight, beside
+  // the one rounding of the result to the same type.
   template <int NC>
   static __device__ inline void accumulate(const bf16* lds, int rt, const f16v (&p)[NC], f16v (&acc)[NDT][NC],
                                            int lane) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      bf8 b[NC];
+      Frag b[NC];
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
+      for (int c = 0; c < NC; ++c) {
+        float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) b[c][j] = (bf16)p[c][8 * k + j];
+        for (int j = 0; j < 8; ++j) v[j] = p[c][8 * k + j];
+        b[c] = frag(v);
+      }
       const int y = 32 * rt + 16 * k + 4 * (lane >> 5);
 #pragma unroll
       for (int d = 0; d < NDT; ++d) {
-        const bf4 l = __builtin_bit_cast(bf4, read_tr(lds, y, 32 * d, lane));
-        const bf4 h = __builtin_bit_cast(bf4, read_tr(lds, y + 8, 32 * d, lane));
-        const bf8 a = {l[0], l[1], l[2], l[3], h[0], h[1], h[2], h[3]};
+        Frag a;
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
-          acc[d][c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[c], acc[d][c], 0, 0, 0);
-      }
-    }
-  }
-};
-
-// fp32: 32x32x2, one element of a lane, k = lane >> 5. A lane's 16-byte chunk serves four
-// instructions: which k slot stands for which element is free as long as both operands agree.
-template <int DP>
-struct Mma<float, DP> {
-  static constexpr int KF = DP / 8, NDT = DP / 32, LDW = DP + 4;
-  typedef f4 Frag;
-  template <int NC>
-  static __device__ inline void scores(const float* lds, int rt, const Frag (&x)[NC][KF], f16v (&s)[NC],
-                                       f16v from, int lane) {
+        for (int i = 0; i < PL; ++i) {
+          const bf4 l = read_tr(lds + i * PLANE, y, 32 * d, lane), h = read_tr(lds + i * PLANE, y + 8, 32 * d, lane);
+          a.p[i] = bf8{l[0], l[1], l[2], l[3], h[0], h[1], h[2], h[3]};
+        }
 #pragma unroll
-    for (int c = 0; c < NC; ++c) s[c] = from;
-    const float* p = lds + (rt * 32 + (lane & 31)) * LDW + 4 * (lane >> 5);
-#pragma unroll
-    for (int k = 0; k < KF; ++k) {
-      const f4 a = *(const f4*)(p + 8 * k);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-          s[c] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], x[c][k][j], s[c], 0, 0, 0);
-    }
-  }
-  static __device__ inline void load_cols(Frag (&f)[KF], const float* row, bool ok, int D, bool vec,
-                                          int lane) {
-#pragma unroll
-    for (int k = 0; k < KF; ++k) {
-      u4 c = {0u, 0u, 0u, 0u};
-      if (ok) c = load_chunk(row, 8 * k + 4 * (lane >> 5), D, vec);
-      f[k] = __builtin_bit_cast(f4, c);
-    }
-  }
-  static __device__ inline float dot(const Frag (&a)[KF], const Frag (&b)[KF]) {
-    float t = 0.f;
-#pragma unroll
-    for (int k = 0; k < KF; ++k)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) t = fmaf(a[k][j], b[k][j], t);
-    return t;
-  }
-  template <int NC>
-  static __device__ inline void accumulate(const float* lds, int rt, const f16v (&p)[NC], f16v (&acc)[NDT][NC],
-                                           int lane) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const float* z = lds + (32 * rt + tile_row(r, lane)) * LDW + (lane & 31);
-#pragma unroll
-      for (int d = 0; d < NDT; ++d) {
-        const float a = z[32 * d];
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-          acc[d][c] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[c][r], acc[d][c], 0, 0, 0);
+        for (int c = 0; c < NC; ++c) acc[d][c] = product(a, b[c], acc[d][c]);
       }
     }
   }

@@ -24,9 +24,9 @@ struct Args {
   int vec_q, vec_w, vec_o;
 };
 
-template <typename T>
+template <typename T, int DP>
 struct Tile {
-  static constexpr int BN = sizeof(T) == 2 ? 64 : 32, NR = BN / 32;
+  static constexpr int BN = DP * sizeof(T) <= 256 ? 64 : 32, NR = BN / 32;
 };
 
 // what the products of a candidate start from: its bias in units of scale
@@ -42,10 +42,10 @@ __device__ inline void range_of(int n, int nsplit, int split, int BN, int* beg, 
 // ---- forward: running maximum and sum of a tile of queries over one piece of the vocabulary ----
 template <typename T, int DP, int NC>
 __global__ __launch_bounds__(256, DP <= 128 || sizeof(T) == 2 ? 2 : 1) void k_ce_fwd(Args a) {
-  typedef Mma<T, DP> M;
-  constexpr int BM = NC * 128, BN = Tile<T>::BN, NR = Tile<T>::NR;
+  constexpr int BM = NC * 128, BN = Tile<T, DP>::BN, NR = Tile<T, DP>::NR;
   typedef Stage<T, DP, BN, 256> St;
-  __shared__ __align__(16) T lw[BN * St::LDW];
+  typedef Mma<T, DP, St::PLANE> M;
+  __shared__ __align__(16) bf16 lw[St::LDS];
   __shared__ __align__(16) float lb[BN];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int col[NC];
@@ -165,10 +165,10 @@ __device__ inline f4 minus_label(const Args& a, int i, int d0, f4 t) {
 
 template <typename T, int DP, int NC>
 __global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void k_ce_dq(Args a) {
-  typedef Mma<T, DP> M;
-  constexpr int BM = NC * 128, BN = Tile<T>::BN, NR = Tile<T>::NR;
+  constexpr int BM = NC * 128, BN = Tile<T, DP>::BN, NR = Tile<T, DP>::NR;
   typedef Stage<T, DP, BN, 256> St;
-  __shared__ __align__(16) T lw[BN * St::LDW];
+  typedef Mma<T, DP, St::PLANE> M;
+  __shared__ __align__(16) bf16 lw[St::LDS];
   __shared__ __align__(16) float lb[BN];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int col[NC];
@@ -255,10 +255,10 @@ __global__ __launch_bounds__(256) void k_ce_dq_join(Args a) {
 // ballot per tile of queries says whether any label falls into the candidates of the workgroup.
 template <typename T, int DP, int NC>
 __global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void k_ce_dw(Args a) {
-  typedef Mma<T, DP> M;
-  constexpr int BM = NC * 128, BN = Tile<T>::BN, NR = Tile<T>::NR;
+  constexpr int BM = NC * 128, BN = Tile<T, DP>::BN, NR = Tile<T, DP>::NR;
   typedef Stage<T, DP, BN, 256> St;
-  __shared__ __align__(16) T lq[BN * St::LDW];
+  typedef Mma<T, DP, St::PLANE> M;
+  __shared__ __align__(16) bf16 lq[St::LDS];
   __shared__ __align__(16) float ll[BN], lg[BN];
   __shared__ __align__(16) int lab[BN];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -413,11 +413,13 @@ int launch1(const Args& a, int64_t tiles, hipStream_t st) {
 template <int W>
 int launch(int dtype, const Args& a, int64_t tiles, hipStream_t st) {
   if (dtype == MONO_ROW_BF16) {
+    if (a.D <= 16) return launch1<W, bf16, 16, 2>(a, tiles, st);
     if (a.D <= 32) return launch1<W, bf16, 32, 2>(a, tiles, st);
     if (a.D <= 64) return launch1<W, bf16, 64, 2>(a, tiles, st);
     if (a.D <= 128) return launch1<W, bf16, 128, 1>(a, tiles, st);
     return launch1<W, bf16, 256, 1>(a, tiles, st);
   }
+  if (a.D <= 16) return launch1<W, float, 16, 1>(a, tiles, st);
   if (a.D <= 32) return launch1<W, float, 32, 1>(a, tiles, st);
   if (a.D <= 64) return launch1<W, float, 64, 1>(a, tiles, st);
   if (a.D <= 128) return launch1<W, float, 128, 1>(a, tiles, st);
