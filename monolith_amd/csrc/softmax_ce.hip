@@ -18,8 +18,11 @@ struct Args {
   float *lse, *loss;
   void *dq, *dw;
   float* db;
-  float *part, *part2;  // forward: maximum and sum of every split; backward: partial gradients
-  int n, v, D, nsplit;
+  float *part, *part2;         // forward: maximum and sum of every piece
+  float *q_part, *w_part, *b_part;  // backward: partial gradients of every piece
+  int n, v, D;
+  int nsplit, q_split, w_split;     // pieces of the streamed rows: forward, and the gradient's two halves
+  int q_tiles, w_tiles;
   float scale, scale2;
   int vec_q, vec_w, vec_o;
 };
@@ -79,9 +82,8 @@ __global__ __launch_bounds__(256, DP <= 128 || sizeof(T) == 2 ? 2 : 1) void k_ce
     f16v s[NR][NC];
 #pragma unroll
     for (int rt = 0; rt < NR; ++rt) {
-      f16v from = all_of(0.f);
-      if (a.bias || y0 + BN > vend) from = by_rows(lb + 32 * rt, lane);
-      M::template scores<NC>(lw, rt, qf, s[rt], from, lane);
+      if (a.bias || y0 + BN > vend) M::template scores<NC>(lw, rt, qf, s[rt], by_rows(lb + 32 * rt, lane), lane);
+      else M::template scores<NC>(lw, rt, qf, s[rt], all_of(0.f), lane);
     }
     // every lane keeps the maximum and sum of the candidates that it holds itself; the two lanes
     // of a query are joined once, behind the loop. m is in units of scale (scale > 0).
@@ -164,12 +166,10 @@ __device__ inline f4 minus_label(const Args& a, int i, int d0, f4 t) {
 }
 
 template <typename T, int DP, int NC>
-__global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void k_ce_dq(Args a) {
+__device__ inline void query_half(const Args& a, int tile, int piece, bf16* lw, float* lb) {
   constexpr int BM = NC * 128, BN = Tile<T, DP>::BN, NR = Tile<T, DP>::NR;
   typedef Stage<T, DP, BN, 256> St;
   typedef Mma<T, DP, St::PLANE> M;
-  __shared__ __align__(16) bf16 lw[St::LDS];
-  __shared__ __align__(16) float lb[BN];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int col[NC];
   typename M::Frag qf[NC][M::KF];
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void k_ce_dq(Ar
   f16v acc[M::NDT][NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    col[c] = blockIdx.x * BM + (wave * NC + c) * 32 + (lane & 31);
+    col[c] = tile * BM + (wave * NC + c) * 32 + (lane & 31);
     const bool ok = col[c] < a.n;
     M::load_cols(qf[c], (const T*)a.q + (int64_t)(ok ? col[c] : 0) * a.qs, ok, a.D, a.vec_q, lane);
     lse[c] = ok ? a.lse[col[c]] : __builtin_inff();
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void k_ce_dq(Ar
     for (int d = 0; d < M::NDT; ++d) acc[d][c] = all_of(0.f);
   }
   int vbeg, vend;
-  range_of(a.v, a.nsplit, blockIdx.y, BN, &vbeg, &vend);
+  range_of(a.v, a.q_split, piece, BN, &vbeg, &vend);
   St st;
   float eb = 0.f;
   const float inv_scale = 1.f / a.scale;
@@ -203,9 +203,9 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void k_ce_dq(Ar
     if (y0 + BN < vend) fetch(y0 + BN);
 #pragma unroll
     for (int rt = 0; rt < NR; ++rt) {
-      f16v s[NC], from = all_of(0.f);
-      if (a.bias || y0 + BN > vend) from = by_rows(lb + 32 * rt, lane);
-      M::template scores<NC>(lw, rt, qf, s, from, lane);
+      f16v s[NC];
+      if (a.bias || y0 + BN > vend) M::template scores<NC>(lw, rt, qf, s, by_rows(lb + 32 * rt, lane), lane);
+      else M::template scores<NC>(lw, rt, qf, s, all_of(0.f), lane);
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -216,8 +216,8 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void k_ce_dq(Ar
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     if (col[c] >= a.n) continue;
-    if (a.part) {
-      store_col(a.part + ((int64_t)blockIdx.y * a.n + col[c]) * a.D, a.D, acc, c, 1.f, a.vec_o, lane);
+    if (a.q_split > 1) {
+      store_col(a.q_part + ((int64_t)piece * a.n + col[c]) * a.D, a.D, acc, c, 1.f, a.vec_o, lane);
       continue;
     }
 #pragma unroll
@@ -232,37 +232,16 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void k_ce_dq(Ar
   }
 }
 
-// dquery from the splits' partial sums, four elements of a row per thread
-template <typename T>
-__global__ __launch_bounds__(256) void k_ce_dq_join(Args a) {
-  const int per = (a.D + 3) / 4;
-  const int64_t total = (int64_t)a.n * per;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int row = (int)(i / per), d0 = (int)(i % per) * 4;
-    f4 t = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.nsplit; ++s) {
-      const float* p = a.part + ((int64_t)s * a.n + row) * a.D;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (d0 + r < a.D) t[r] += p[d0 + r];
-    }
-    store4((T*)a.dq + (int64_t)row * a.D, d0, a.D, minus_label<T>(a, row, d0, t), a.vec_o);
-  }
-}
-
 // drows_v = scale sum_i g_i (p_iv - [v = label_i]) query_i, dbias_v the same without scale and query:
 // a tile of candidates keeps its sums while all queries stream by. The label's share is rare: one
 // ballot per tile of queries says whether any label falls into the candidates of the workgroup.
 template <typename T, int DP, int NC>
-__global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void k_ce_dw(Args a) {
+__device__ inline void rows_half(const Args& a, int tile, int piece, bf16* lq, float* ll, float* lg, int* lab) {
   constexpr int BM = NC * 128, BN = Tile<T, DP>::BN, NR = Tile<T, DP>::NR;
   typedef Stage<T, DP, BN, 256> St;
   typedef Mma<T, DP, St::PLANE> M;
-  __shared__ __align__(16) bf16 lq[St::LDS];
-  __shared__ __align__(16) float ll[BN], lg[BN];
-  __shared__ __align__(16) int lab[BN];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int v0 = blockIdx.x * BM;
+  const int v0 = tile * BM;
   int col[NC];
   typename M::Frag wf[NC][M::KF];
   float b2[NC], sb[NC];
@@ -278,7 +257,7 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void k_ce_dw(Ar
     for (int d = 0; d < M::NDT; ++d) acc[d][c] = all_of(0.f);
   }
   int nbeg, nend;
-  range_of(a.n, a.nsplit, blockIdx.y, BN, &nbeg, &nend);
+  range_of(a.n, a.w_split, piece, BN, &nbeg, &nend);
   St st;
   const Rows<T> qr = {(const T*)a.q, a.qs, a.D, a.vec_q != 0};
   const float inv_scale2 = 1.f / a.scale2;
@@ -345,20 +324,56 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void k_ce_dw(Ar
   for (int c = 0; c < NC; ++c) {
     const float b = col_sum(sb[c]);
     if (col[c] >= a.v) continue;
-    const int64_t row = (a.nsplit > 1 ? (int64_t)blockIdx.y * a.v : 0) + col[c];
-    if (a.db && lane < 32) (a.nsplit > 1 ? a.part2 : a.db)[row] = b;
+    const int64_t row = (a.w_split > 1 ? (int64_t)piece * a.v : 0) + col[c];
+    if (a.db && lane < 32) (a.w_split > 1 ? a.b_part : a.db)[row] = b;
     if (!a.dw) continue;
-    if (a.nsplit > 1) store_col(a.part + row * a.D, a.D, acc, c, a.scale, a.vec_o, lane);
+    if (a.w_split > 1) store_col(a.w_part + row * a.D, a.D, acc, c, a.scale, a.vec_o, lane);
     else store_col((T*)a.dw + row * a.D, a.D, acc, c, a.scale, a.vec_o, lane);
   }
 }
 
+// Both halves of the gradient in one launch: they share nothing, the queries' half first.
+template <typename T, int DP, int NC>
+__global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void k_ce_bwd(Args a) {
+  constexpr int BN = Tile<T, DP>::BN;
+  __shared__ __align__(16) bf16 rows[Stage<T, DP, BN, 256>::LDS];
+  __shared__ __align__(16) float first[BN], second[BN];
+  __shared__ __align__(16) int labels[BN];
+  const int of_queries = a.q_tiles * a.q_split, i = blockIdx.x - of_queries;
+  if (i < 0) query_half<T, DP, NC>(a, blockIdx.x % a.q_tiles, blockIdx.x / a.q_tiles, rows, first);
+  else rows_half<T, DP, NC>(a, i % a.w_tiles, i / a.w_tiles, rows, first, second, labels);
+}
+
+// out[four elements from 4 i on] = the pieces' partial sums, first to last
+__device__ inline f4 sum_parts(const float* part, int n_part, int64_t total, int64_t at, int n) {
+  f4 t = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < n_part; ++s) {
+    const float* p = part + (int64_t)s * total + at;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (r < n) t[r] += p[r];
+  }
+  return t;
+}
+// what of the gradient came in pieces: dquery and drows by four elements of a row, dbias by candidates
 template <typename T>
-__global__ __launch_bounds__(256) void k_ce_sum(const float* part, int n_part, int64_t total, T* out) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    float t = 0.f;
-    for (int s = 0; s < n_part; ++s) t += part[(int64_t)s * total + i];
-    out[i] = (T)t;
+__global__ __launch_bounds__(256) void k_ce_join(Args a) {
+  const int per = (a.D + 3) / 4;
+  const int64_t nq = a.dq && a.q_split > 1 ? (int64_t)a.n * per : 0;
+  const int64_t nw = a.dw && a.w_split > 1 ? (int64_t)a.v * per : 0;
+  const int64_t nb = a.db && a.w_split > 1 ? a.v : 0;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < nq + nw + nb; i += (int64_t)gridDim.x * 256) {
+    if (i < nq) {
+      const int row = (int)(i / per), d0 = (int)(i % per) * 4;
+      const f4 t = sum_parts(a.q_part, a.q_split, (int64_t)a.n * a.D, (int64_t)row * a.D + d0, a.D - d0);
+      store4((T*)a.dq + (int64_t)row * a.D, d0, a.D, minus_label<T>(a, row, d0, t), a.vec_o);
+    } else if (i < nq + nw) {
+      const int row = (int)((i - nq) / per), d0 = (int)((i - nq) % per) * 4;
+      const f4 t = sum_parts(a.w_part, a.w_split, (int64_t)a.v * a.D, (int64_t)row * a.D + d0, a.D - d0);
+      store4((T*)a.dw + (int64_t)row * a.D, d0, a.D, t, a.vec_o);
+    } else {
+      a.db[i - nq - nw] = sum_parts(a.b_part, a.w_split, a.v, i - nq - nw, 1)[0];
+    }
   }
 }
 
@@ -366,16 +381,24 @@ __global__ __launch_bounds__(256) void k_ce_sum(const float* part, int n_part, i
 int cols_of(const mono_softmax_ce_args* p) {
   return p->dtype == MONO_ROW_BF16 && p->dim <= 64 ? 2 : 1;
 }
-// tiles of `kept` rows, and pieces of the streamed rows that fill the card when there are few tiles
 int64_t tiles_of(const mono_softmax_ce_args* p, int64_t kept) {
   const int bm = 128 * cols_of(p);
   return (kept + bm - 1) / bm;
 }
-int pieces_of(const mono_softmax_ce_args* p, int64_t kept, int64_t streamed) {
-  const int64_t tiles = tiles_of(p, kept), want = 256 * 4;
-  if (tiles >= want) return 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(want / std::max<int64_t>(1, tiles), streamed / 64));
+// Few tiles of kept rows: the streamed rows are cut into pieces of 64 or more, as many as make `rounds`
+// rounds of the workgroups that the card holds at once (with 1024 workgroups where it holds 768 the last
+// 256 run alone: 138 us instead of 124 for 8192 queries against 16385 rows of 64 floats). The forward's
+// partial results are two numbers a query, so it takes several rounds; the backward's are whole rows, so
+// each of its halves takes one.
+int pieces_of(const mono_softmax_ce_args* p, int64_t kept, int64_t streamed, int rounds) {
+  const int row = p->dim * (p->dtype == MONO_ROW_BF16 ? 2 : 4);
+  const int64_t want = 256 * rounds * (row > 256 ? 1 : cols_of(p) == 2 && p->dim > 32 ? 2 : 3);
+  const int64_t tiles = std::max<int64_t>(1, tiles_of(p, kept));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(want / tiles, streamed / 64));
 }
+int fwd_pieces(const mono_softmax_ce_args* p) { return pieces_of(p, p->n, p->vocab, 4); }
+int query_pieces(const mono_softmax_ce_args* p) { return pieces_of(p, p->n, p->vocab, 1); }
+int rows_pieces(const mono_softmax_ce_args* p) { return pieces_of(p, p->vocab, p->n, 1); }
 
 int check(const mono_softmax_ce_args* p, const char* who) {
   MONO_REQUIRE(p != nullptr, "%s: args is NULL", who);
@@ -400,38 +423,34 @@ Args base_args(const mono_softmax_ce_args* p) {
   return a;
 }
 
-enum Which { kFwd, kDq, kDw };
+enum Which { kFwd, kBwd };
 template <int W, typename T, int DP, int NC>
-int launch1(const Args& a, int64_t tiles, hipStream_t st) {
-  const dim3 grid((unsigned)tiles, (unsigned)a.nsplit);
-  if (W == kFwd) k_ce_fwd<T, DP, NC><<<grid, 256, 0, st>>>(a);
-  else if (W == kDq) k_ce_dq<T, DP, NC><<<grid, 256, 0, st>>>(a);
-  else k_ce_dw<T, DP, NC><<<grid, 256, 0, st>>>(a);
+int launch1(const Args& a, hipStream_t st) {
+  if (W == kFwd) {
+    k_ce_fwd<T, DP, NC><<<dim3((unsigned)a.q_tiles, (unsigned)a.nsplit), 256, 0, st>>>(a);
+  } else {
+    const int64_t wgs = (int64_t)a.q_tiles * a.q_split + (int64_t)a.w_tiles * a.w_split;
+    k_ce_bwd<T, DP, NC><<<(unsigned)wgs, 256, 0, st>>>(a);
+  }
   MONO_HIP(hipGetLastError());
   return 0;
 }
 template <int W>
-int launch(int dtype, const Args& a, int64_t tiles, hipStream_t st) {
+int launch(int dtype, const Args& a, hipStream_t st) {
   if (dtype == MONO_ROW_BF16) {
-    if (a.D <= 16) return launch1<W, bf16, 16, 2>(a, tiles, st);
-    if (a.D <= 32) return launch1<W, bf16, 32, 2>(a, tiles, st);
-    if (a.D <= 64) return launch1<W, bf16, 64, 2>(a, tiles, st);
-    if (a.D <= 128) return launch1<W, bf16, 128, 1>(a, tiles, st);
-    return launch1<W, bf16, 256, 1>(a, tiles, st);
+    if (a.D <= 16) return launch1<W, bf16, 16, 2>(a, st);
+    if (a.D <= 32) return launch1<W, bf16, 32, 2>(a, st);
+    if (a.D <= 64) return launch1<W, bf16, 64, 2>(a, st);
+    if (a.D <= 128) return launch1<W, bf16, 128, 1>(a, st);
+    return launch1<W, bf16, 256, 1>(a, st);
   }
-  if (a.D <= 16) return launch1<W, float, 16, 1>(a, tiles, st);
-  if (a.D <= 32) return launch1<W, float, 32, 1>(a, tiles, st);
-  if (a.D <= 64) return launch1<W, float, 64, 1>(a, tiles, st);
-  if (a.D <= 128) return launch1<W, float, 128, 1>(a, tiles, st);
-  return launch1<W, float, 256, 1>(a, tiles, st);
+  if (a.D <= 16) return launch1<W, float, 16, 1>(a, st);
+  if (a.D <= 32) return launch1<W, float, 32, 1>(a, st);
+  if (a.D <= 64) return launch1<W, float, 64, 1>(a, st);
+  if (a.D <= 128) return launch1<W, float, 128, 1>(a, st);
+  return launch1<W, float, 256, 1>(a, st);
 }
 int64_t round16(int64_t b) { return (b + 15) & ~(int64_t)15; }
-template <typename T>
-int sum_parts(const float* part, int n_part, int64_t total, T* out, hipStream_t st) {
-  k_ce_sum<T><<<grid_for(total, 256), 256, 0, st>>>(part, n_part, total, out);
-  MONO_HIP(hipGetLastError());
-  return 0;
-}
 }  // namespace
 }  // namespace mono
 
@@ -440,7 +459,7 @@ using namespace mono;
 
 int64_t mono_softmax_cross_entropy_workspace(const mono_softmax_ce_args* p) {
   if (check(p, "mono_softmax_cross_entropy_workspace")) return -1;
-  return 2 * round16((int64_t)pieces_of(p, p->n, p->vocab) * p->n * 4);
+  return 2 * round16((int64_t)fwd_pieces(p) * p->n * 4);
 }
 
 int mono_softmax_cross_entropy(const mono_softmax_ce_args* p, void* stream) {
@@ -450,10 +469,11 @@ int mono_softmax_cross_entropy(const mono_softmax_ce_args* p, void* stream) {
                "mono_softmax_cross_entropy: workspace of %lld bytes is too small", (long long)p->workspace_bytes);
   hipStream_t st = (hipStream_t)stream;
   Args a = base_args(p);
-  a.nsplit = pieces_of(p, p->n, p->vocab);
+  a.nsplit = fwd_pieces(p);
+  a.q_tiles = (int)tiles_of(p, p->n);
   a.part = (float*)p->workspace;
   a.part2 = (float*)((char*)p->workspace + round16((int64_t)a.nsplit * p->n * 4));
-  MONO_TRY(launch<kFwd>(p->dtype, a, tiles_of(p, p->n), st));
+  MONO_TRY(launch<kFwd>(p->dtype, a, st));
   const unsigned grid = (unsigned)((p->n + 3) / 4);
   if (p->dtype == MONO_ROW_BF16) k_ce_loss<bf16><<<grid, 256, 0, st>>>(a);
   else k_ce_loss<float><<<grid, 256, 0, st>>>(a);
@@ -461,43 +481,48 @@ int mono_softmax_cross_entropy(const mono_softmax_ce_args* p, void* stream) {
   return 0;
 }
 
+namespace {
+// where the partial gradients lie in the workspace; returns its bytes
+int64_t place_parts(const mono_softmax_ce_args* p, Args* a) {
+  const bool rows = p->grad_rows || p->grad_bias;
+  a->q_split = p->grad_query ? query_pieces(p) : 1;
+  a->w_split = rows ? rows_pieces(p) : 1;
+  a->q_tiles = p->grad_query ? (int)tiles_of(p, p->n) : 0;
+  a->w_tiles = rows ? (int)tiles_of(p, p->vocab) : 0;
+  int64_t at = 0;
+  const auto take = [&](int n_part, int64_t each) {
+    float* to = (float*)((char*)p->workspace + at);
+    if (n_part > 1) at += round16(n_part * each * 4);
+    return to;
+  };
+  a->q_part = take(a->q_split, p->n * p->dim);
+  a->w_part = take(p->grad_rows ? a->w_split : 1, p->vocab * p->dim);
+  a->b_part = take(p->grad_bias ? a->w_split : 1, p->vocab);
+  return at;
+}
+}  // namespace
+
 int64_t mono_softmax_cross_entropy_gradient_workspace(const mono_softmax_ce_args* p) {
   if (check(p, "mono_softmax_cross_entropy_gradient_workspace")) return -1;
-  const int64_t sq = pieces_of(p, p->n, p->vocab), sw = pieces_of(p, p->vocab, p->n);
-  return std::max(sq <= 1 ? 0 : round16(sq * p->n * p->dim * 4),
-                  sw <= 1 ? 0 : round16(sw * p->vocab * p->dim * 4) + round16(sw * p->vocab * 4));
+  Args a;
+  return place_parts(p, &a);
 }
 
 int mono_softmax_cross_entropy_gradient(const mono_softmax_ce_args* p, void* stream) {
   MONO_TRY(check(p, "mono_softmax_cross_entropy_gradient"));
-  MONO_REQUIRE(p->workspace_bytes >= mono_softmax_cross_entropy_gradient_workspace(p),
+  Args a = base_args(p);
+  MONO_REQUIRE(p->workspace_bytes >= place_parts(p, &a),
                "mono_softmax_cross_entropy_gradient: workspace of %lld bytes is too small",
                (long long)p->workspace_bytes);
   hipStream_t st = (hipStream_t)stream;
-  const bool half = p->dtype == MONO_ROW_BF16;
-  Args a = base_args(p);
-  if (p->grad_query && p->n) {
-    a.nsplit = pieces_of(p, p->n, p->vocab);
-    a.part = a.nsplit > 1 ? (float*)p->workspace : nullptr;
-    MONO_TRY(launch<kDq>(p->dtype, a, tiles_of(p, p->n), st));
-    if (a.part) {
-      const int grid = grid_for(p->n * ((p->dim + 3) / 4), 256);
-      if (half) k_ce_dq_join<bf16><<<grid, 256, 0, st>>>(a);
-      else k_ce_dq_join<float><<<grid, 256, 0, st>>>(a);
-      MONO_HIP(hipGetLastError());
-    }
-  }
-  if (p->grad_rows || p->grad_bias) {
-    a.nsplit = pieces_of(p, p->vocab, p->n);
-    const int64_t total = p->vocab * p->dim;
-    a.part = (float*)p->workspace;
-    a.part2 = (float*)((char*)p->workspace + round16((int64_t)a.nsplit * total * 4));
-    MONO_TRY(launch<kDw>(p->dtype, a, tiles_of(p, p->vocab), st));
-    if (a.nsplit > 1) {
-      if (p->grad_rows && half) MONO_TRY(sum_parts(a.part, a.nsplit, total, (bf16*)p->grad_rows, st));
-      if (p->grad_rows && !half) MONO_TRY(sum_parts(a.part, a.nsplit, total, (float*)p->grad_rows, st));
-      if (p->grad_bias) MONO_TRY(sum_parts(a.part2, a.nsplit, p->vocab, p->grad_bias, st));
-    }
+  if (a.q_tiles + a.w_tiles == 0) return 0;
+  MONO_TRY(launch<kBwd>(p->dtype, a, st));
+  if (a.q_split > 1 || a.w_split > 1) {
+    const int64_t per = (p->dim + 3) / 4;
+    const int grid = grid_for((a.q_split > 1 ? p->n * per : 0) + (a.w_split > 1 ? p->vocab * (per + 1) : 0), 256);
+    if (p->dtype == MONO_ROW_BF16) k_ce_join<bf16><<<grid, 256, 0, st>>>(a);
+    else k_ce_join<float><<<grid, 256, 0, st>>>(a);
+    MONO_HIP(hipGetLastError());
   }
   return 0;
 }
