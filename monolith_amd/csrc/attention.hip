@@ -7,6 +7,7 @@
 // the rule that sequence b's tiles start at floor(start_b / BM) + b: that leaves every sequence room
 // for ceil(length / BM) tiles, needs no pass over the splits and no copy of them to the host.
 #include <algorithm>
+#include <type_traits>
 
 #include "mono_common.h"
 #include "seq_dev.h"
@@ -27,6 +28,7 @@ struct Args {
   const uint8_t* mask;
   int B, nq, nk, H, Hkv, G, D, qmode, kmode, causal, shared;
   int nsplit, slot0;
+  int chunk;                       // pooled rows: keys of a wave, 0 = a split of a sequence's keys
   float scale, scale2;
   int vec_q, vec_k, vec_v, vec_g, vec_o;
 };
@@ -249,59 +251,111 @@ __global__ __launch_bounds__(NW * 64, DP * sizeof(T) <= 256 ? 2 : 1) void k_attn
   }
 }
 
-// out = sum of the splits' results, each weighted by its share of the softmax's sum. W = 1: a thread
-// takes four elements of a row through all splits. Many splits of few rows (W = 4): a workgroup takes a
-// row, its 256 threads as 256 / ceil(D / 4) groups that each sum every so many-th split; joined in LDS.
-template <typename T, int W>
-__global__ __launch_bounds__(256) void k_attn_join(const float* part, const float* part_lse, int n_part,
+// Where the parts of a row lie: part s at first + s * step.
+struct Parts {
+  int n;                // parts of a row (chunk = 0)
+  int64_t rows;         // rows of a part
+  const int64_t* ksp;   // chunk > 0: the parts of the pooled rows, by the splits
+  int chunk, B, nk, H;
+  __device__ inline int of(int64_t row, int64_t* first, int64_t* step) const {
+    if (!chunk) {
+      *first = row;
+      *step = rows;
+      return n;
+    }
+    const int b = (int)(row / H), lo = split_at(ksp, b, nk), hi = split_at(ksp, b + 1, nk);
+    *first = (int64_t)(lo / chunk + b + 1) * H + row % H;
+    *step = H;
+    return hi > lo ? (hi - lo + chunk - 1) / chunk : 1;
+  }
+};
+// out = sum of the parts' results, each weighted by its share of the softmax's sum (a part without a key
+// holds zeros and a statistic of -inf: its weight is 0). A thread takes four elements of a row through
+// all parts.
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_join(const float* part, const float* part_lse, Parts parts,
                                                    int64_t rows, int D, T* out, float* lse, int vec) {
   const int d4 = (D + 3) / 4;
-  __shared__ f4 sums[W == 1 ? 1 : 256];
-  __shared__ float zs[W == 1 ? 1 : 256];
-  const int groups = W == 1 ? 1 : 256 / d4;
-  const int64_t i = W == 1 ? (int64_t)blockIdx.x * 256 + threadIdx.x : blockIdx.x;
-  const int64_t row = W == 1 ? i / d4 : i;
-  const int d0 = (W == 1 ? (int)(i % d4) : threadIdx.x % d4) * 4, group = W == 1 ? 0 : threadIdx.x / d4;
-  if (row >= rows) return;  // (W = 4: the whole workgroup)
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / d4;
+  const int d0 = (int)(i % d4) * 4;
+  if (row >= rows) return;
+  int64_t first, step;
+  const int n = parts.of(row, &first, &step);
+  float m = neg_inf();
+  for (int s = 0; s < n; ++s) m = fmaxf(m, part_lse[first + s * step]);
+  const float base = m == neg_inf() ? 0.f : m;
   f4 t = {0.f, 0.f, 0.f, 0.f};
-  float z = 0.f, m = neg_inf();
-  if (W == 1) {
-    for (int s = 0; s < n_part; ++s) m = fmaxf(m, part_lse[(int64_t)s * rows + row]);
-  } else {
-    for (int s = threadIdx.x; s < n_part; s += 256) m = fmaxf(m, part_lse[(int64_t)s * rows + row]);
-    for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
-    if ((threadIdx.x & 63) == 0) zs[threadIdx.x >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(zs[0], zs[1]), fmaxf(zs[2], zs[3]));
-    __syncthreads();
-  }
-  if (group < groups)
-    for (int s = group; s < n_part; s += groups) {
-      const float e = part_lse[(int64_t)s * rows + row];
-      if (e == neg_inf()) continue;  // a split without a key: nothing was summed
-      const float w = exp2_hw(e - m);
-      const float* p = part + ((int64_t)s * rows + row) * D + d0;
-      z += w;
-      if (vec) {
-        t += w * *(const f4*)p;
-      } else {
+  float z = 0.f;
+  for (int s = 0; s < n; ++s) {
+    const float w = exp2_hw(part_lse[first + s * step] - base);
+    const float* p = part + (first + s * step) * D + d0;
+    z += w;
+    if (vec) {
+      t += w * *(const f4*)p;
+    } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (d0 + j < D) t[j] = fmaf(w, p[j], t[j]);
-      }
-    }
-  if (W > 1) {
-    sums[threadIdx.x] = t;
-    zs[threadIdx.x] = z;
-    __syncthreads();
-    if (group) return;
-    for (int g = 1; g < groups; ++g) {
-      t += sums[g * d4 + threadIdx.x];
-      z += zs[g * d4 + threadIdx.x];
+      for (int j = 0; j < 4; ++j)
+        if (d0 + j < D) t[j] = fmaf(w, p[j], t[j]);
     }
   }
   store4(out + row * D, d0, D, t * (z == 0.f ? 0.f : 1.f / z), vec);
   if (lse && d0 == 0) lse[row] = z == 0.f ? neg_inf() : m + __log2f(z);
+}
+
+// The same for many parts of few rows: a workgroup per row, its threads as groups of d4 that take every
+// so many-th part. The weights come first, 1024 parts at a time, so that the parts' rows are loads that
+// wait for nothing: one thread after the other through 625 parts, each behind its weight, took 30 us.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(1024) void k_attn_join_many(const float* part, const float* part_lse, Parts parts,
+                                                         int D, T* out, float* lse) {
+  __shared__ f4 sums[1024];
+  __shared__ float ws[1024], red[16];
+  const int tid = threadIdx.x, d4 = (D + 3) / 4, groups = 1024 / d4, group = tid / d4, d0 = tid % d4 * 4;
+  const int64_t row = blockIdx.x;
+  int64_t first, step;
+  const int n = parts.of(row, &first, &step);
+  float m = neg_inf();
+  for (int s = tid; s < n; s += 1024) m = fmaxf(m, part_lse[first + s * step]);
+  m = over_lanes<1, 64, Max>(m);
+  if ((tid & 63) == 0) red[tid >> 6] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = fmaxf(m, red[i]);
+  const float base = m == neg_inf() ? 0.f : m;
+  f4 t = {0.f, 0.f, 0.f, 0.f};
+  float z = 0.f;
+  for (int s0 = 0; s0 < n; s0 += 1024) {
+    const int here = min(1024, n - s0);
+    __syncthreads();
+    ws[tid] = tid < here ? exp2_hw(part_lse[first + (s0 + tid) * step] - base) : 0.f;
+    z += ws[tid];
+    __syncthreads();
+    const float* p = part + (first + s0 * step) * D + d0;
+    if (group < groups) {
+#pragma unroll 8
+      for (int s = group; s < here; s += groups) {
+        if (VEC) {
+          t += ws[s] * *(const f4*)(p + s * step * D);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (d0 + j < D) t[j] = fmaf(ws[s], p[s * step * D + j], t[j]);
+        }
+      }
+    }
+  }
+  z = over_lanes<1, 64, Sum>(z);
+  __syncthreads();
+  if ((tid & 63) == 0) red[tid >> 6] = z;
+  sums[tid] = t;
+  __syncthreads();
+  if (group) return;
+  z = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z += red[i];
+  for (int g = 1; g < groups; ++g) t += sums[g * d4 + tid];
+  store4(out + row * D, d0, D, t * (z == 0.f ? 0.f : 1.f / z), VEC);
+  if (lse && tid == 0) lse[row] = z == 0.f ? neg_inf() : m + __log2f(z);
 }
 
 // ---- backward ------------------------------------------------------------------------------
@@ -554,12 +608,16 @@ __global__ __launch_bounds__(NW * 64, DP * sizeof(T) <= 128 ? 2 : 1) void k_attn
   }
 }
 
-// out = the splits' partial sums, first to last
+// out = the parts' sums, first to last
 template <typename T>
-__global__ __launch_bounds__(256) void k_sum_parts(const float* part, int n_part, int64_t total, T* out) {
+__global__ __launch_bounds__(256) void k_sum_parts(const float* part, Parts parts, int64_t total, int D, T* out) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    int64_t first, step;
+    const int n = parts.of(i / D, &first, &step);
+    const float* p = part + first * D + i % D;
     float t = 0.f;
-    for (int s = 0; s < n_part; ++s) t += part[(int64_t)s * total + i];
+#pragma unroll 8
+    for (int s = 0; s < n; ++s) t += p[s * step * D];
     out[i] = (T)t;
   }
 }
@@ -619,18 +677,50 @@ __device__ inline void split_range(int n, int nsplit, int split, int step, int* 
   *end = (int)min((int64_t)n, (int64_t)*beg + chunk);
 }
 
+// A wave's work: a key head of a sequence, or a part of its keys. With chunk = 0 every sequence has
+// nsplit equal parts, and part p of row b lies at p * n_query + b. Otherwise a part is `chunk` keys, so that
+// long sequences have more of them, and the parts are numbered like tiles of `chunk` rows.
+struct PoolItem {
+  Seg sk;
+  int kvh, beg, end;
+  int64_t part;  // times heads: the row of the partial results
+};
+__device__ __host__ inline int64_t pool_tiles(int64_t B, int64_t nk, int chunk) { return nk / chunk + B + 2; }
+__device__ inline int64_t pool_items(const Args& a) {
+  return (a.chunk ? pool_tiles(a.B, a.nk, a.chunk) : (int64_t)a.B * a.nsplit) * a.Hkv;
+}
+__device__ inline PoolItem pool_item(const Args& a, int64_t item, int step) {
+  PoolItem w;
+  w.kvh = (int)(item % a.Hkv);
+  item /= a.Hkv;
+  if (a.chunk) {
+    int local;
+    w.sk = find_tile(a.ksp, kSplits, a.B, a.nk, 1, a.chunk, (int)item, &local);
+    const int64_t beg = (int64_t)local * a.chunk;
+    if (local > 0 && beg >= w.sk.n) w.sk.b = -1;  // (a tile that the rule leaves free)
+    w.beg = (int)min(beg, (int64_t)w.sk.n);
+    w.end = (int)min(beg + a.chunk, (int64_t)w.sk.n);
+    w.part = item;
+  } else {
+    const int split = (int)(item % a.nsplit), b = (int)(item / a.nsplit);
+    w.sk = segment(a.ksp, kSplits, b, a.nk);
+    split_range(w.sk.n, a.nsplit, split, step, &w.beg, &w.end);
+    w.part = (int64_t)split * a.nq + b;
+  }
+  return w;
+}
+
 template <typename T, int DP, int GT>
 __global__ __launch_bounds__(256) void k_pool_fwd(Args a) {
   constexpr int E = 16 / sizeof(T), LPR = DP / E, R = 64 / LPR, U = sizeof(T) == 4 ? 4 : 2;
   const int lane = threadIdx.x & 63;
   const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (item >= (int64_t)a.B * a.Hkv * a.nsplit) return;
-  const int split = (int)(item % a.nsplit), kvh = (int)(item / a.nsplit % a.Hkv);
-  const int b = (int)(item / a.nsplit / a.Hkv);
+  if (item >= pool_items(a)) return;
+  const PoolItem w = pool_item(a, item, R);
+  if (w.sk.b < 0) return;
+  const int kvh = w.kvh, b = w.sk.b, beg = w.beg, end = w.end;
+  const Seg sk = w.sk;
   const int sub = lane / LPR, e0 = lane % LPR * E;
-  const Seg sk = segment(a.ksp, kSplits, b, a.nk);
-  int beg, end;
-  split_range(sk.n, a.nsplit, split, R, &beg, &end);
   const T* kb = (const T*)a.k + (int64_t)sk.lo * a.ks + (int64_t)kvh * a.kh;
   const T* vb = (const T*)a.v + (int64_t)sk.lo * a.vs + (int64_t)kvh * a.vh;
   const uint8_t* mb = a.mask ? a.mask + sk.lo : nullptr;
@@ -691,16 +781,16 @@ __global__ __launch_bounds__(256) void k_pool_fwd(Args a) {
   for (int g = 0; g < GT; ++g) {
     const float mx = over_lanes<LPR, 64, Max>(m[g]);
     const float base = mx == neg_inf() ? 0.f : mx * a.scale2;
-    const float w = exp2_hw(fmaf(m[g], a.scale2, -base));
-    const float lt = over_lanes<LPR, 64, Sum>(l[g] * w);
+    const float share = exp2_hw(fmaf(m[g], a.scale2, -base));
+    const float lt = over_lanes<LPR, 64, Sum>(l[g] * share);
 #pragma unroll
-    for (int i = 0; i < E; ++i) acc[g].x[i] = over_lanes<LPR, 64, Sum>(acc[g].x[i] * w);
+    for (int i = 0; i < E; ++i) acc[g].x[i] = over_lanes<LPR, 64, Sum>(acc[g].x[i] * share);
     if (sub) continue;
     const float inv = lt == 0.f ? 0.f : 1.f / lt;
     const float lse = lt == 0.f ? neg_inf() : fmaf(mx, a.scale2, __log2f(lt));
     const int64_t row = (int64_t)b * a.H + kvh * a.G + g;
     if (a.part) {
-      const int64_t at = (int64_t)(a.slot0 + split) * a.nq * a.H + row;
+      const int64_t at = (a.chunk ? 0 : (int64_t)a.slot0 * a.nq * a.H) + w.part * a.H + kvh * a.G + g;
       if (lane == 0) a.part_lse[at] = lse;
       acc[g].store(a.part + at * a.D, e0, a.D, a.vec_o, inv);
     } else {
@@ -718,7 +808,7 @@ __global__ __launch_bounds__(256) void k_pool_bwd(Args a) {
   constexpr int E = 16 / sizeof(T), LPR = DP / E, R = 64 / LPR, U = 2;
   const int lane = threadIdx.x & 63;
   const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t items = (int64_t)a.B * a.Hkv * a.nsplit;
+  const int64_t items = pool_items(a);
   const int sub = lane / LPR, e0 = lane % LPR * E;
   Chunk<T> zero;
   zero.clear();
@@ -733,11 +823,10 @@ __global__ __launch_bounds__(256) void k_pool_bwd(Args a) {
     }
     return;
   }
-  const int split = (int)(item % a.nsplit), kvh = (int)(item / a.nsplit % a.Hkv);
-  const int b = (int)(item / a.nsplit / a.Hkv);
-  const Seg sk = segment(a.ksp, kSplits, b, a.nk);
-  int beg, end;
-  split_range(sk.n, a.nsplit, split, R, &beg, &end);
+  const PoolItem w = pool_item(a, item, R);
+  if (w.sk.b < 0) return;
+  const int kvh = w.kvh, b = w.sk.b, beg = w.beg, end = w.end;
+  const Seg sk = w.sk;
   const T* kb = (const T*)a.k + (int64_t)sk.lo * a.ks + (int64_t)kvh * a.kh;
   const T* vb = (const T*)a.v + (int64_t)sk.lo * a.vs + (int64_t)kvh * a.vh;
   const uint8_t* mb = a.mask ? a.mask + sk.lo : nullptr;
@@ -804,7 +893,7 @@ __global__ __launch_bounds__(256) void k_pool_bwd(Args a) {
     if (sub) continue;
     const int64_t row = (int64_t)b * a.H + kvh * a.G + g;
     if (a.part) {
-      dq[g].store(a.part + ((int64_t)split * a.nq * a.H + row) * a.D, e0, a.D, a.vec_o, 1.f);
+      dq[g].store(a.part + (w.part * a.H + kvh * a.G + g) * a.D, e0, a.D, a.vec_o, 1.f);
     } else {
       dq[g].store((T*)a.dq + row * a.D, e0, a.D, a.vec_o, 1.f);
     }
@@ -884,11 +973,15 @@ struct Plan {
   Shape sh;
   int64_t tiles;
   int nsplit;
+  int chunk;  // pool: keys of a wave where long sequences are cut
+  int64_t part_rows(int64_t rows, int64_t heads) const { return chunk ? tiles * heads : nsplit > 1 ? nsplit * rows : 0; }
+  bool parted() const { return chunk || nsplit > 1; }
 };
 Plan plan_tiles(int dtype, int D, int mode, int64_t B, int64_t n, int64_t G, int64_t heads,
                 double stream_rows) {
   Plan pl;
   pl.pool = false;
+  pl.chunk = 0;
   const double per = mode == kWhole ? (double)n * G : (double)n * G / std::max<int64_t>(1, B);
   pl.sh = shape_for(dtype, D, per);
   pl.tiles = tiles_for(mode, B, n, G, pl.sh.bm);
@@ -898,18 +991,27 @@ Plan plan_tiles(int dtype, int D, int mode, int64_t B, int64_t n, int64_t G, int
 double average(int64_t n, int64_t B) { return (double)n / std::max<int64_t>(1, B); }
 
 // One query per sequence: a wave per sequence and key head while a few heads share the keys; a group of
-// more than 4 heads fills enough of a matrix tile.
+// more than 4 heads fills enough of a matrix tile. Too few waves for the card's 4096 at a time: long
+// sequences are cut, into `chunk` keys (the 7 histories of pool_lifelong are of 9411 to 120000 keys: equal
+// numbers of parts left the longest alone at the end) or, behind a prefix, into equal parts.
 bool is_pool(const mono_attention_args* p) { return !p->query_splits && p->heads / p->kv_heads <= 4; }
-Plan plan_fwd(const mono_attention_args* p) {
-  if (is_pool(p)) {
-    Plan pl{};
-    pl.pool = true;
-    pl.tiles = p->batch;
-    const int64_t waves = p->batch * p->kv_heads, want = 256 * 16;
-    const int64_t by_len = (int64_t)(average(p->n_key, p->batch) / 128);
-    pl.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want / std::max<int64_t>(1, waves), by_len), 256));
+Plan plan_pool(const mono_attention_args* p, bool equal) {
+  Plan pl{};
+  pl.pool = true;
+  pl.nsplit = 1;
+  const int64_t waves = std::max<int64_t>(1, p->batch * p->kv_heads), want = 256 * 16;
+  const int64_t by_len = (int64_t)(average(p->n_key, p->batch) / 128);
+  if (waves >= want || by_len < 2) return pl;
+  if (equal) {
+    pl.nsplit = (int)std::min<int64_t>(std::min<int64_t>(want / waves, by_len), 256);
     return pl;
   }
+  pl.chunk = (int)((std::max<int64_t>(128, p->n_key * p->kv_heads / want) + 63) / 64 * 64);
+  pl.tiles = pool_tiles(p->batch, p->n_key, pl.chunk);
+  return pl;
+}
+Plan plan_fwd(const mono_attention_args* p, bool behind_prefix = false) {
+  if (is_pool(p)) return plan_pool(p, behind_prefix);
   return plan_tiles(p->dtype, p->dim, p->query_splits ? kSplits : kOnePerSeq, p->batch, p->n_query,
                     p->heads / p->kv_heads, p->kv_heads, average(p->n_key, p->batch));
 }
@@ -931,7 +1033,7 @@ int launch1(const Args& a, const Plan& pl, hipStream_t st) {
 // the pooled kernels; backward: 64 more workgroups for the rows of no sequence
 template <int W, typename T, int DP, int GT>
 int launch_pool2(const Args& a, hipStream_t st) {
-  const int64_t wgs = ((int64_t)a.B * a.Hkv * a.nsplit + 3) / 4;
+  const int64_t wgs = ((a.chunk ? pool_tiles(a.B, a.nk, a.chunk) : (int64_t)a.B * a.nsplit) * a.Hkv + 3) / 4;
   MONO_REQUIRE(wgs < (1LL << 31) - 64, "attention: too many sequences");
   if (W == kFwd) k_pool_fwd<T, DP, GT><<<(unsigned)wgs, 256, 0, st>>>(a);
   else k_pool_bwd<T, DP, GT><<<(unsigned)wgs + 64, 256, 0, st>>>(a);
@@ -984,34 +1086,35 @@ int launch(int dtype, const Args& a, const Plan& pl, hipStream_t st) {
 }
 
 int64_t round16(int64_t b) { return (b + 15) & ~(int64_t)15; }
-int64_t parts_bytes(int64_t n_part, int64_t rows, int64_t D) {
-  return n_part <= 1 ? 0 : round16(n_part * rows * D * 4) + round16(n_part * rows * 4);
-}
+// partial rows and their statistics
+int64_t parts_bytes(int64_t rows, int64_t D) { return round16(rows * D * 4) + round16(rows * 4); }
 
-int join(const mono_attention_args* p, const float* part, const float* part_lse, int n_part, hipStream_t st) {
+Parts parts_of(const mono_attention_args* p, int n, int64_t rows, int chunk) {
+  return Parts{n, rows, p->key_splits, chunk, (int)p->batch, (int)p->n_key, p->heads};
+}
+int join(const mono_attention_args* p, const float* part, const float* part_lse, int n_part, int chunk, hipStream_t st) {
   const int64_t rows = p->n_query * p->heads;
   if (rows == 0) return 0;
   const int vec = p->dim % 4 == 0 && ((uintptr_t)p->out & 15) == 0;
-  // a row's splits in one thread's turn cost a memory latency each: from 16 splits on a workgroup per row
-  const bool wide = n_part >= 16;
-  const unsigned grid = (unsigned)(wide ? rows : (rows * ((p->dim + 3) / 4) + 255) / 256);
-  const bool half = p->dtype == MONO_ROW_BF16;
-  if (half && wide)
-    k_attn_join<bf16, 4><<<grid, 256, 0, st>>>(part, part_lse, n_part, rows, p->dim, (bf16*)p->out, p->lse, vec);
-  else if (half)
-    k_attn_join<bf16, 1><<<grid, 256, 0, st>>>(part, part_lse, n_part, rows, p->dim, (bf16*)p->out, p->lse, vec);
-  else if (wide)
-    k_attn_join<float, 4><<<grid, 256, 0, st>>>(part, part_lse, n_part, rows, p->dim, (float*)p->out, p->lse, vec);
-  else
-    k_attn_join<float, 1><<<grid, 256, 0, st>>>(part, part_lse, n_part, rows, p->dim, (float*)p->out, p->lse, vec);
+  const bool many = chunk || n_part >= 16;
+  const unsigned grid = (unsigned)(many ? rows : (rows * ((p->dim + 3) / 4) + 255) / 256);
+  const Parts parts = parts_of(p, n_part, rows, chunk);
+  const auto go = [&](auto* out) {
+    typedef typename std::remove_pointer<decltype(out)>::type T;
+    if (!many) k_attn_join<T><<<grid, 256, 0, st>>>(part, part_lse, parts, rows, p->dim, out, p->lse, vec);
+    else if (vec) k_attn_join_many<T, true><<<grid, 1024, 0, st>>>(part, part_lse, parts, p->dim, out, p->lse);
+    else k_attn_join_many<T, false><<<grid, 1024, 0, st>>>(part, part_lse, parts, p->dim, out, p->lse);
+  };
+  if (p->dtype == MONO_ROW_BF16) go((bf16*)p->out);
+  else go((float*)p->out);
   MONO_HIP(hipGetLastError());
   return 0;
 }
-int sum_parts(int dtype, const float* part, int n_part, int64_t total, void* out, hipStream_t st) {
+int sum_parts(int dtype, const float* part, const Parts& parts, int64_t total, int D, void* out, hipStream_t st) {
   if (total == 0) return 0;
   const int grid = grid_for(total, 256);
-  if (dtype == MONO_ROW_BF16) k_sum_parts<bf16><<<grid, 256, 0, st>>>(part, n_part, total, (bf16*)out);
-  else k_sum_parts<float><<<grid, 256, 0, st>>>(part, n_part, total, (float*)out);
+  if (dtype == MONO_ROW_BF16) k_sum_parts<bf16><<<grid, 256, 0, st>>>(part, parts, total, D, (bf16*)out);
+  else k_sum_parts<float><<<grid, 256, 0, st>>>(part, parts, total, D, (float*)out);
   MONO_HIP(hipGetLastError());
   return 0;
 }
@@ -1028,7 +1131,7 @@ PrefixPlan plan_prefix(const mono_attention_args* p) {
   r.pre = plan_tiles(p->dtype, p->dim, kWhole, 1, p->n_query, G, p->kv_heads, (double)p->n_prefix);
   r.slots = r.pre.nsplit;
   if (p->key_splits) {
-    r.own = plan_fwd(p);
+    r.own = plan_fwd(p, true);
     r.slots += r.own.nsplit;
   }
   return r;
@@ -1041,7 +1144,7 @@ using namespace mono;
 
 int64_t mono_ragged_attention_workspace(const mono_attention_args* p) {
   if (check(p, "mono_ragged_attention_workspace")) return -1;
-  return parts_bytes(plan_fwd(p).nsplit, p->n_query * p->heads, p->dim);
+  return parts_bytes(plan_fwd(p).part_rows(p->n_query * p->heads, p->heads), p->dim);
 }
 
 int mono_ragged_attention(const mono_attention_args* p, void* stream) {
@@ -1049,17 +1152,18 @@ int mono_ragged_attention(const mono_attention_args* p, void* stream) {
   MONO_REQUIRE(p->key_splits, "mono_ragged_attention: key_splits is NULL");
   if (p->n_query == 0) return 0;
   const Plan pl = plan_fwd(p);
-  const int64_t rows = p->n_query * p->heads;
-  MONO_REQUIRE(p->workspace_bytes >= parts_bytes(pl.nsplit, rows, p->dim),
+  const int64_t rows = pl.part_rows(p->n_query * p->heads, p->heads);
+  MONO_REQUIRE(p->workspace_bytes >= parts_bytes(rows, p->dim),
                "mono_ragged_attention: workspace of %lld bytes is too small", (long long)p->workspace_bytes);
   Args a = base_args(p);
   a.nsplit = pl.nsplit;
-  if (pl.nsplit > 1) {
+  a.chunk = pl.chunk;
+  if (pl.parted()) {
     a.part = (float*)p->workspace;
-    a.part_lse = (float*)((char*)p->workspace + round16(pl.nsplit * rows * p->dim * 4));
+    a.part_lse = (float*)((char*)p->workspace + round16(rows * p->dim * 4));
   }
   MONO_TRY(launch<kFwd>(p->dtype, a, pl, (hipStream_t)stream));
-  return pl.nsplit > 1 ? join(p, a.part, a.part_lse, pl.nsplit, (hipStream_t)stream) : 0;
+  return pl.parted() ? join(p, a.part, a.part_lse, pl.nsplit, pl.chunk, (hipStream_t)stream) : 0;
 }
 
 int64_t mono_ragged_attention_gradient_workspace(const mono_attention_args* p) {
@@ -1067,8 +1171,8 @@ int64_t mono_ragged_attention_gradient_workspace(const mono_attention_args* p) {
   const Plan q = plan_fwd(p), k = plan_dkv(p);
   const int64_t nk = p->n_key * p->kv_heads;
   return round16(p->n_query * p->heads * 4) +
-         std::max(parts_bytes(q.nsplit, p->n_query * p->heads, p->dim),
-                  k.nsplit <= 1 ? 0 : 2 * round16(k.nsplit * nk * p->dim * 4));
+         std::max(round16(q.part_rows(p->n_query * p->heads, p->heads) * p->dim * 4),
+                  q.pool ? 0 : 2 * round16(k.part_rows(nk, 0) * p->dim * 4));
 }
 
 int mono_ragged_attention_gradient(const mono_attention_args* p, void* stream) {
@@ -1086,24 +1190,29 @@ int mono_ragged_attention_gradient(const mono_attention_args* p, void* stream) {
   Args a = base_args(p);
   a.delta = (float*)p->workspace;
   a.nsplit = plq.nsplit;
-  a.part = plq.nsplit > 1 ? scratch : nullptr;
+  a.chunk = plq.chunk;
+  a.part = plq.parted() ? scratch : nullptr;
   MONO_TRY(launch<kDq>(p->dtype, a, plq, st));
-  if (a.part) MONO_TRY(sum_parts(p->dtype, a.part, plq.nsplit, rows * p->dim, p->grad_query, st));
+  if (a.part)
+    MONO_TRY(sum_parts(p->dtype, a.part, parts_of(p, plq.nsplit, rows, plq.chunk), rows * p->dim, p->dim,
+                       p->grad_query, st));
   if (!p->grad_key || plq.pool) return 0;  // (the pooled pass has written the keys' gradients)
   a.nsplit = plk.nsplit;
   a.part = plk.nsplit > 1 ? scratch : nullptr;
   a.part2 = a.part ? (float*)((char*)scratch + round16(plk.nsplit * krows * p->dim * 4)) : nullptr;
   MONO_TRY(launch<kDkv>(p->dtype, a, plk, st));
   if (a.part) {
-    MONO_TRY(sum_parts(p->dtype, a.part, plk.nsplit, krows * p->dim, p->grad_key, st));
-    if (!p->kv_shared) MONO_TRY(sum_parts(p->dtype, a.part2, plk.nsplit, krows * p->dim, p->grad_value, st));
+    const Parts parts = parts_of(p, plk.nsplit, krows, 0);
+    MONO_TRY(sum_parts(p->dtype, a.part, parts, krows * p->dim, p->dim, p->grad_key, st));
+    if (!p->kv_shared) MONO_TRY(sum_parts(p->dtype, a.part2, parts, krows * p->dim, p->dim, p->grad_value, st));
   }
   return 0;
 }
 
 int64_t mono_shared_prefix_attention_workspace(const mono_attention_args* p) {
   if (check(p, "mono_shared_prefix_attention_workspace")) return -1;
-  return parts_bytes(plan_prefix(p).slots, p->n_query * p->heads, p->dim);
+  const int64_t slots = plan_prefix(p).slots;
+  return slots > 1 ? parts_bytes(slots * p->n_query * p->heads, p->dim) : 0;
 }
 
 int mono_shared_prefix_attention(const mono_attention_args* p, void* stream) {
@@ -1111,7 +1220,7 @@ int mono_shared_prefix_attention(const mono_attention_args* p, void* stream) {
   if (p->n_query == 0) return 0;
   const PrefixPlan pl = plan_prefix(p);
   const int64_t rows = p->n_query * p->heads;
-  MONO_REQUIRE(p->workspace_bytes >= parts_bytes(pl.slots, rows, p->dim),
+  MONO_REQUIRE(p->workspace_bytes >= (pl.slots > 1 ? parts_bytes(pl.slots * rows, p->dim) : 0),
                "mono_shared_prefix_attention: workspace of %lld bytes is too small",
                (long long)p->workspace_bytes);
   hipStream_t st = (hipStream_t)stream;
@@ -1137,6 +1246,6 @@ int mono_shared_prefix_attention(const mono_attention_args* p, void* stream) {
   a.nsplit = pl.pre.nsplit;
   a.slot0 = 0;
   MONO_TRY(launch<kFwd>(p->dtype, a, pl.pre, st));
-  return pl.slots > 1 ? join(p, a.part, a.part_lse, pl.slots, st) : 0;
+  return pl.slots > 1 ? join(p, a.part, a.part_lse, pl.slots, 0, st) : 0;
 }
 }

@@ -344,14 +344,17 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void k_ce_bwd(A
   else rows_half<T, DP, NC>(a, i % a.w_tiles, i / a.w_tiles, rows, first, second, labels);
 }
 
-// out[four elements from 4 i on] = the pieces' partial sums, first to last
-__device__ inline f4 sum_parts(const float* part, int n_part, int64_t total, int64_t at, int n) {
+// four elements from `at` on of the pieces' partial sums, first to last; several pieces' loads in flight
+__device__ inline f4 sum_parts(const float* part, int n_part, int64_t total, int64_t at, int n, bool vec) {
   f4 t = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < n_part; ++s) {
-    const float* p = part + (int64_t)s * total + at;
+  if (vec) {
+#pragma unroll 8
+    for (int s = 0; s < n_part; ++s) t += *(const f4*)(part + (int64_t)s * total + at);
+  } else {
+    for (int s = 0; s < n_part; ++s)
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (r < n) t[r] += p[r];
+      for (int r = 0; r < 4; ++r)
+        if (r < n) t[r] += part[(int64_t)s * total + at + r];
   }
   return t;
 }
@@ -359,20 +362,21 @@ __device__ inline f4 sum_parts(const float* part, int n_part, int64_t total, int
 template <typename T>
 __global__ __launch_bounds__(256) void k_ce_join(Args a) {
   const int per = (a.D + 3) / 4;
+  const bool vec = a.D % 4 == 0;
   const int64_t nq = a.dq && a.q_split > 1 ? (int64_t)a.n * per : 0;
   const int64_t nw = a.dw && a.w_split > 1 ? (int64_t)a.v * per : 0;
   const int64_t nb = a.db && a.w_split > 1 ? a.v : 0;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < nq + nw + nb; i += (int64_t)gridDim.x * 256) {
     if (i < nq) {
       const int row = (int)(i / per), d0 = (int)(i % per) * 4;
-      const f4 t = sum_parts(a.q_part, a.q_split, (int64_t)a.n * a.D, (int64_t)row * a.D + d0, a.D - d0);
+      const f4 t = sum_parts(a.q_part, a.q_split, (int64_t)a.n * a.D, (int64_t)row * a.D + d0, a.D - d0, vec);
       store4((T*)a.dq + (int64_t)row * a.D, d0, a.D, minus_label<T>(a, row, d0, t), a.vec_o);
     } else if (i < nq + nw) {
       const int row = (int)((i - nq) / per), d0 = (int)((i - nq) % per) * 4;
-      const f4 t = sum_parts(a.w_part, a.w_split, (int64_t)a.v * a.D, (int64_t)row * a.D + d0, a.D - d0);
+      const f4 t = sum_parts(a.w_part, a.w_split, (int64_t)a.v * a.D, (int64_t)row * a.D + d0, a.D - d0, vec);
       store4((T*)a.dw + (int64_t)row * a.D, d0, a.D, t, a.vec_o);
     } else {
-      a.db[i - nq - nw] = sum_parts(a.b_part, a.w_split, a.v, i - nq - nw, 1)[0];
+      a.db[i - nq - nw] = sum_parts(a.b_part, a.w_split, a.v, i - nq - nw, 1, false)[0];
     }
   }
 }
