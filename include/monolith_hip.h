@@ -486,6 +486,7 @@ typedef struct {
   /* contiguous [n_query, heads, dim]; lse float[n_query, heads] in units of log 2, written by the
    * forward (may be NULL there) and read by the backward */
   void* out;
+  void* out_rest; /* NULL, or like out: what its rounding to bf16 leaves, kept for the backward */
   float* lse;
   /* backward: grad_out like query, the gradients contiguous and shaped like their inputs */
   mono_rows grad_out;

@@ -47,7 +47,8 @@ class AttentionArgs(C.Structure):  # mono_attention_args
               ("query", Rows), ("key", Rows), ("value", Rows), ("query_splits", C.c_void_p),
               ("key_splits", C.c_void_p), ("key_mask", C.c_void_p), ("scale", C.c_float),
               ("n_prefix", C.c_int64), ("prefix_key", Rows), ("prefix_value", Rows),
-              ("prefix_mask", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+              ("prefix_mask", C.c_void_p), ("out", C.c_void_p), ("out_rest", C.c_void_p),
+              ("lse", C.c_void_p),
               ("grad_out", Rows), ("grad_query", C.c_void_p), ("grad_key", C.c_void_p),
               ("grad_value", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
 

@@ -132,15 +132,19 @@ def _call(fn, workspace, a: _lib.AttentionArgs, device) -> None:
   _lib.launch(fn, a, device)
 
 
-def _forward(q, k, v, key_splits, query_splits, key_mask, causal, scale, with_lse):
+def _forward(q, k, v, key_splits, query_splits, key_mask, causal, scale, for_backward):
   out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-  lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if with_lse else None
+  lse = rest = None
   a = _args(q, k, v, key_splits, query_splits, key_mask, causal, scale)
   a.out = out.data_ptr()
-  if with_lse:
+  if for_backward:
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
     a.lse = lse.data_ptr()
+    if q.dtype == torch.bfloat16:
+      rest = torch.empty_like(out)
+      a.out_rest = rest.data_ptr()
   _call(_lib.lib.mono_ragged_attention, _lib.lib.mono_ragged_attention_workspace, a, q.device)
-  return out, lse
+  return out, lse, rest
 
 
 class _RaggedAttention(torch.autograd.Function):
@@ -148,15 +152,15 @@ class _RaggedAttention(torch.autograd.Function):
   @staticmethod
   def forward(ctx, query, key, value, key_splits, query_splits, key_mask, causal, scale):
     v = key if value is None else value
-    out, lse = _forward(query, key, v, key_splits, query_splits, key_mask, causal, scale, True)
-    ctx.save_for_backward(query, key, value, key_splits, query_splits, key_mask, out, lse)
+    out, lse, rest = _forward(query, key, v, key_splits, query_splits, key_mask, causal, scale, True)
+    ctx.save_for_backward(query, key, value, key_splits, query_splits, key_mask, out, lse, rest)
     ctx.causal, ctx.scale = causal, scale
     return out
 
   @staticmethod
   @torch.autograd.function.once_differentiable
   def backward(ctx, grad):
-    query, key, value, key_splits, query_splits, key_mask, out, lse = ctx.saved_tensors
+    query, key, value, key_splits, query_splits, key_mask, out, lse, rest = ctx.saved_tensors
     shared = value is None
     a = _args(query, key, key if shared else value, key_splits, query_splits, key_mask, ctx.causal,
               ctx.scale)
@@ -166,6 +170,8 @@ class _RaggedAttention(torch.autograd.Function):
     a.kv_shared = int(shared)
     a.out, a.lse, a.grad_out = out.data_ptr(), lse.data_ptr(), _rows(grad)
     a.grad_query = dq.data_ptr()
+    if rest is not None:
+      a.out_rest = rest.data_ptr()
     dk = dv = None
     keys = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
     if keys:

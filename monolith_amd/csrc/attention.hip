@@ -21,7 +21,7 @@ enum Mode { kSplits = 0, kOnePerSeq = 1, kWhole = 2 };
 struct Args {
   const void *q, *k, *v, *go, *o;
   int64_t qs, qh, ks, kh, vs, vh, gs, gh;
-  void *out, *dq, *dk, *dv;
+  void *out, *rest, *dq, *dk, *dv;
   float *lse, *delta;
   float *part, *part2, *part_lse;  // split partials
   const int64_t *qsp, *ksp;
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(NW * 64, DP * sizeof(T) <= 256 ? 2 : 1) void k_attn
       store_col(a.part + at * a.D, a.D, acc, c, inv, a.vec_o, lane);
     } else {
       if (a.lse && lane < 32) a.lse[row] = lse;
-      store_col((T*)a.out + row * a.D, a.D, acc, c, inv, a.vec_o, lane);
+      store_col((T*)a.out + row * a.D, a.D, acc, c, inv, a.vec_o, lane, a.rest ? (T*)a.rest + row * a.D : nullptr);
     }
   }
 }
@@ -274,7 +274,7 @@ struct Parts {
 // all parts.
 template <typename T>
 __global__ __launch_bounds__(256) void k_attn_join(const float* part, const float* part_lse, Parts parts,
-                                                   int64_t rows, int D, T* out, float* lse, int vec) {
+                                                   int64_t rows, int D, T* out, T* rest, float* lse, int vec) {
   const int d4 = (D + 3) / 4;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / d4;
   const int d0 = (int)(i % d4) * 4;
@@ -298,7 +298,9 @@ __global__ __launch_bounds__(256) void k_attn_join(const float* part, const floa
         if (d0 + j < D) t[j] = fmaf(w, p[j], t[j]);
     }
   }
-  store4(out + row * D, d0, D, t * (z == 0.f ? 0.f : 1.f / z), vec);
+  t *= z == 0.f ? 0.f : 1.f / z;
+  store4(out + row * D, d0, D, t, vec);
+  if (rest) store4(rest + row * D, d0, D, rest_of<T>(t), vec);
   if (lse && d0 == 0) lse[row] = z == 0.f ? neg_inf() : m + __log2f(z);
 }
 
@@ -307,7 +309,7 @@ __global__ __launch_bounds__(256) void k_attn_join(const float* part, const floa
 // wait for nothing: one thread after the other through 625 parts, each behind its weight, took 30 us.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(1024) void k_attn_join_many(const float* part, const float* part_lse, Parts parts,
-                                                         int D, T* out, float* lse) {
+                                                         int D, T* out, T* rest, float* lse) {
   __shared__ f4 sums[1024];
   __shared__ float ws[1024], red[16];
   const int tid = threadIdx.x, d4 = (D + 3) / 4, groups = 1024 / d4, group = tid / d4, d0 = tid % d4 * 4;
@@ -354,13 +356,17 @@ __global__ __launch_bounds__(1024) void k_attn_join_many(const float* part, cons
 #pragma unroll
   for (int i = 0; i < 16; ++i) z += red[i];
   for (int g = 1; g < groups; ++g) t += sums[g * d4 + tid];
-  store4(out + row * D, d0, D, t * (z == 0.f ? 0.f : 1.f / z), VEC);
+  t *= z == 0.f ? 0.f : 1.f / z;
+  store4(out + row * D, d0, D, t, VEC);
+  if (rest) store4(rest + row * D, d0, D, rest_of<T>(t), VEC);
   if (lse && tid == 0) lse[row] = z == 0.f ? neg_inf() : m + __log2f(z);
 }
 
 // ---- backward ------------------------------------------------------------------------------
 // dQ: the forward's tiles again. With p = exp2(s - lse) from the forward's statistics and
-// delta = g.o, ds = p (g.v - delta), dq = scale sum ds k. Also writes delta for the pass over keys.
+// delta = g.o, ds = p (g.v - delta), dq = scale sum ds k. Also writes delta for the pass over keys. A bf16
+// result's rounding would shift delta, and with it every ds of the row the same way (gradients 2.5e-3 off
+// instead of 2.4e-3, of which their own rounding is 1.7e-3): o is taken with its rest.
 template <typename T, int DP, int NC, int NW>
 __global__ __launch_bounds__(NW * 64, DP <= 64 || (sizeof(T) == 2 && NW > 1) ? 2 : 1) void k_attn_dq(Args a) {
   constexpr int BM = NC * NW * 32, BN = Tile<T, DP, NW>::BN, NR = Tile<T, DP, NW>::NR, NT = NW * 64;
@@ -399,7 +405,12 @@ __global__ __launch_bounds__(NW * 64, DP <= 64 || (sizeof(T) == 2 && NW > 1) ? 2
     M::load_cols(gf[c], (const T*)a.go + t * a.gs + (int64_t)head[c] * a.gh, ok[c], a.D, a.vec_g, lane);
     typename M::Frag of[M::KF];
     M::load_cols(of, (const T*)a.o + row * a.D, ok[c], a.D, a.vec_o, lane);
-    delta[c] = col_sum(M::dot(gf[c], of));
+    delta[c] = M::dot(gf[c], of);
+    if (a.rest) {
+      M::load_cols(of, (const T*)a.rest + row * a.D, ok[c], a.D, a.vec_o, lane);
+      delta[c] += M::dot(gf[c], of);
+    }
+    delta[c] = col_sum(delta[c]);
     const float e = ok[c] ? a.lse[row] : neg_inf();
     lse[c] = e == neg_inf() ? __builtin_inff() : e;  // a row without keys: every weight is 0
     if (ok[c] && lane < 32 && split == 0) a.delta[row] = delta[c];
@@ -796,6 +807,12 @@ __global__ __launch_bounds__(256) void k_pool_fwd(Args a) {
     } else {
       if (a.lse && lane == 0) a.lse[row] = lse;
       acc[g].store((T*)a.out + row * a.D, e0, a.D, a.vec_o, inv);
+      if (a.rest) {
+        Chunk<T> rest;
+#pragma unroll
+        for (int i = 0; i < E; ++i) rest.x[i] = acc[g].x[i] * inv - (float)(T)(acc[g].x[i] * inv);
+        rest.store((T*)a.rest + row * a.D, e0, a.D, a.vec_o, 1.f);
+      }
     }
   }
 }
@@ -841,7 +858,12 @@ __global__ __launch_bounds__(256) void k_pool_bwd(Args a) {
     q[g].set(load_chunk((const T*)a.q + (int64_t)b * a.qs + (int64_t)head * a.qh, e0, a.D, a.vec_q));
     go[g].set(load_chunk((const T*)a.go + (int64_t)b * a.gs + (int64_t)head * a.gh, e0, a.D, a.vec_g));
     o.set(load_chunk((const T*)a.o + row * a.D, e0, a.D, a.vec_o));
-    delta[g] = row_sum<LPR>(go[g].dot(o));
+    delta[g] = go[g].dot(o);
+    if (a.rest) {
+      o.set(load_chunk((const T*)a.rest + row * a.D, e0, a.D, a.vec_o));
+      delta[g] += go[g].dot(o);
+    }
+    delta[g] = row_sum<LPR>(delta[g]);
     const float e = a.lse[row];
     lse[g] = e == neg_inf() ? __builtin_inff() : e;
     dq[g].clear();
@@ -948,7 +970,7 @@ Args base_args(const mono_attention_args* p) {
   a.k = p->key.ptr, a.ks = p->key.row_stride, a.kh = p->key.head_stride;
   a.v = p->value.ptr, a.vs = p->value.row_stride, a.vh = p->value.head_stride;
   a.go = p->grad_out.ptr, a.gs = p->grad_out.row_stride, a.gh = p->grad_out.head_stride;
-  a.o = p->out, a.out = p->out, a.lse = p->lse;
+  a.o = p->out, a.out = p->out, a.rest = p->out_rest, a.lse = p->lse;
   a.dq = p->grad_query, a.dk = p->grad_key, a.dv = p->grad_value;
   a.qsp = p->query_splits, a.ksp = p->key_splits, a.mask = p->key_mask;
   a.B = (int)p->batch, a.nq = (int)p->n_query, a.nk = (int)p->n_key;
@@ -962,7 +984,7 @@ Args base_args(const mono_attention_args* p) {
   a.vec_k = aligned_rows(p->key, p->dtype, p->dim);
   a.vec_v = aligned_rows(p->value, p->dtype, p->dim);
   a.vec_g = aligned_rows(p->grad_out, p->dtype, p->dim);
-  a.vec_o = p->dim % (p->dtype == MONO_ROW_BF16 ? 8 : 4) == 0 && (((uintptr_t)p->out | (uintptr_t)p->grad_query |
+  a.vec_o = p->dim % (p->dtype == MONO_ROW_BF16 ? 8 : 4) == 0 && (((uintptr_t)p->out | (uintptr_t)p->out_rest | (uintptr_t)p->grad_query |
              (uintptr_t)p->grad_key | (uintptr_t)p->grad_value) & 15) == 0;
   return a;
 }
@@ -1095,15 +1117,16 @@ Parts parts_of(const mono_attention_args* p, int n, int64_t rows, int chunk) {
 int join(const mono_attention_args* p, const float* part, const float* part_lse, int n_part, int chunk, hipStream_t st) {
   const int64_t rows = p->n_query * p->heads;
   if (rows == 0) return 0;
-  const int vec = p->dim % 4 == 0 && ((uintptr_t)p->out & 15) == 0;
+  const int vec = p->dim % 4 == 0 && (((uintptr_t)p->out | (uintptr_t)p->out_rest) & 15) == 0;
   const bool many = chunk || n_part >= 16;
   const unsigned grid = (unsigned)(many ? rows : (rows * ((p->dim + 3) / 4) + 255) / 256);
   const Parts parts = parts_of(p, n_part, rows, chunk);
   const auto go = [&](auto* out) {
     typedef typename std::remove_pointer<decltype(out)>::type T;
-    if (!many) k_attn_join<T><<<grid, 256, 0, st>>>(part, part_lse, parts, rows, p->dim, out, p->lse, vec);
-    else if (vec) k_attn_join_many<T, true><<<grid, 1024, 0, st>>>(part, part_lse, parts, p->dim, out, p->lse);
-    else k_attn_join_many<T, false><<<grid, 1024, 0, st>>>(part, part_lse, parts, p->dim, out, p->lse);
+    T* rest = (T*)p->out_rest;
+    if (!many) k_attn_join<T><<<grid, 256, 0, st>>>(part, part_lse, parts, rows, p->dim, out, rest, p->lse, vec);
+    else if (vec) k_attn_join_many<T, true><<<grid, 1024, 0, st>>>(part, part_lse, parts, p->dim, out, rest, p->lse);
+    else k_attn_join_many<T, false><<<grid, 1024, 0, st>>>(part, part_lse, parts, p->dim, out, rest, p->lse);
   };
   if (p->dtype == MONO_ROW_BF16) go((bf16*)p->out);
   else go((float*)p->out);

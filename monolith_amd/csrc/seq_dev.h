@@ -346,9 +346,18 @@ __device__ inline void store4(T* row, int d0, int D, f4 v, bool vec) {
   }
 }
 
-// column c of acc, times f, as a row of D elements
+// what a value's rounding to T leaves
+template <typename T>
+__device__ inline f4 rest_of(f4 v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] -= (float)(T)v[i];
+  return v;
+}
+
+// column c of acc, times f, as a row of D elements; rest (may be NULL) takes what the rounding leaves
 template <typename T, int NDT, int NC>
-__device__ inline void store_col(T* row, int D, const f16v (&acc)[NDT][NC], int c, float f, bool vec, int lane) {
+__device__ inline void store_col(T* row, int D, const f16v (&acc)[NDT][NC], int c, float f, bool vec, int lane,
+                                 T* rest = nullptr) {
 #pragma unroll
   for (int d = 0; d < NDT; ++d)
 #pragma unroll
@@ -357,7 +366,10 @@ __device__ inline void store_col(T* row, int D, const f16v (&acc)[NDT][NC], int 
       f4 v;
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = acc[d][c][4 * q + i] * f;
-      if (d0 < D) store4(row, d0, D, v, vec);
+      if (d0 < D) {
+        store4(row, d0, D, v, vec);
+        if (rest) store4(rest, d0, D, rest_of<T>(v), vec);
+      }
     }
 }
 

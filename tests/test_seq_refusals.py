@@ -153,7 +153,7 @@ def test_c_cross_entropy_refuses():
 
 
 def test_structures_have_the_header_s_size():
-  assert C.sizeof(_lib.AttentionArgs) == 296 and C.sizeof(_lib.SoftmaxCeArgs) == 144
+  assert C.sizeof(_lib.AttentionArgs) == 304 and C.sizeof(_lib.SoftmaxCeArgs) == 144
 
 
 def test_restated_gradients_against_differences():
