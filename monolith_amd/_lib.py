@@ -2,6 +2,7 @@
 library raises, and every non-zero status from the C ABI raises MonolithHipError."""
 import ctypes as C
 import os
+import struct
 
 # torch must load its HIP runtime before libmonolith_hip.so pulls in libamdhip64: with the order
 # reversed both end up sharing the system copy and torch then reports "No HIP GPUs are available".
@@ -62,6 +63,10 @@ class SoftmaxCeArgs(C.Structure):  # mono_softmax_ce_args
               ("grad_bias", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
 
 
+_SEQ = ("mono_ragged_attention", "mono_ragged_attention_gradient", "mono_shared_prefix_attention",
+        "mono_softmax_cross_entropy", "mono_softmax_cross_entropy_gradient")
+
+
 def _load():
   if not os.path.exists(LIB_PATH):
     raise ImportError(
@@ -70,14 +75,13 @@ def _load():
   lib = C.CDLL(LIB_PATH)
   lib.mono_last_error.restype = C.c_char_p
   lib.mono_fused_reorder_last_plan.restype = C.c_int64
-  for name in ("mono_ragged_attention", "mono_ragged_attention_gradient",
-               "mono_shared_prefix_attention", "mono_softmax_cross_entropy",
-               "mono_softmax_cross_entropy_gradient"):
+  for name in _SEQ:
     getattr(lib, name + "_workspace").restype = C.c_int64
   return lib
 
 
 lib = _load()
+_seq_fns = {n: (getattr(lib, n), getattr(lib, n + "_workspace")) for n in _SEQ}
 
 
 def check(rc):
@@ -99,9 +103,26 @@ def stream_ptr(device=None):
   return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-def launch(fn, args, device):
-  """fn(&args, current stream of `device`), with `device` the current one (a launch goes to it)."""
-  if device.index == torch.cuda.current_device():
-    return check(fn(C.byref(args), stream_ptr(device)))
+# The argument structures of the sequence operators, packed in one call: filling a ctypes.Structure field
+# by field costs more host time than the launch itself.
+pack_attention = struct.Struct("@6i3q" + 3 * "P2q" + "3Pfq" + 2 * "P2q" + "P3P" + "P2q" + "3PPq").pack
+pack_softmax_ce = struct.Struct("@2i2q" + 2 * "Pq" + "2Pf" + 2 * "P" + "PPPPPq").pack
+_raw_stream = torch._C._cuda_getCurrentRawStream  # (current_stream() builds an object on every call)
+
+
+def launch(name, pack, fields, device):
+  """The operator `name` on the current stream of `device`, with `device` the current one (a launch goes to
+  it), its arguments packed from `fields` and a workspace from torch's allocator behind them."""
+  fn, workspace = _seq_fns[name]
+  args = pack(*fields, 0, 0)
+  n = workspace(args)
+  if n:
+    if n < 0:
+      check(1)
+    ws = torch.empty(n, dtype=torch.uint8, device=device)
+    args = pack(*fields, ws.data_ptr(), n)
+  index = device.index
+  if index == torch.cuda.current_device():
+    return check(fn(args, C.c_void_p(_raw_stream(index))))
   with torch.cuda.device(device):
-    check(fn(C.byref(args), stream_ptr(device)))
+    check(fn(args, C.c_void_p(_raw_stream(index))))

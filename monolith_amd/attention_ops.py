@@ -11,14 +11,12 @@ no sequence: their outputs and gradients are zero. Splits that break this give w
 an access outside the tensors. Softmax statistics and sums are held in 32 bits; results have the
 rows' type and are the same bit for bit from call to call. Nothing synchronises the host, and
 scratch memory comes from torch's allocator, so every op can be captured into a HIP graph."""
-import ctypes as C
 import math
 from typing import Optional
 
 import torch
 
 from monolith_amd import _lib
-from monolith_amd._lib import vp
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}  # MONO_ROW_*
 MAX_DIM = 128
@@ -31,43 +29,6 @@ def _heads(x: torch.Tensor, name: str, who: str) -> torch.Tensor:
   if x.dim() == 2:
     x = x.unsqueeze(1)
   return x if x.stride(2) == 1 else x.contiguous()
-
-
-def _same(x: torch.Tensor, like: torch.Tensor, name: str, who: str):
-  if x.device != like.device or x.dtype != like.dtype:
-    raise ValueError("%s: %s is %s on %s, query is %s on %s" % (who, name, x.dtype, x.device,
-                                                                like.dtype, like.device))
-
-
-def _splits(x, n_batch, device, name: str, who: str) -> torch.Tensor:
-  if not isinstance(x, torch.Tensor) or x.dim() != 1 or x.numel() < 1 or \
-      x.dtype not in (torch.int64, torch.int32):
-    raise ValueError("%s: %s must be an int64 vector [batch + 1]" % (who, name))
-  if x.device != device:
-    raise ValueError("%s: %s is on %s, query on %s" % (who, name, x.device, device))
-  if n_batch is not None and x.numel() != n_batch + 1:
-    raise ValueError("%s: %s has %d entries for a batch of %d" % (who, name, x.numel(), n_batch))
-  return x.to(torch.int64).contiguous()
-
-
-def _mask(x, n, device, name: str, who: str) -> Optional[torch.Tensor]:
-  if x is None:
-    return None
-  if x.dtype != torch.bool or x.dim() != 1 or x.numel() != n or x.device != device:
-    raise ValueError("%s: %s must be a bool vector of %d entries on %s" % (who, name, n, device))
-  return x.contiguous()
-
-
-def _scale(scale, dim, who) -> float:
-  scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-  if not (math.isfinite(scale) and scale > 0):
-    raise ValueError("%s: scale must be a positive finite number, got %r" % (who, scale))
-  return scale
-
-
-def _on_gpu(x: torch.Tensor, who: str):
-  if not x.is_cuda:
-    raise _lib.MonolithHipError("%s: tensors must live on the GPU (no CPU fallback)" % who)
 
 
 def _query(query, who):
@@ -83,67 +44,93 @@ def _query(query, who):
 
 def _keys(q, key, value, who, name=""):
   k = _heads(key, name + "key", who)
-  _same(k, q, name + "key", who)
   v = k if value is None else _heads(value, name + "value", who)
-  _same(v, q, name + "value", who)
-  if v.shape != k.shape:
+  dtype, device = q.dtype, q.device
+  for x in (k,) if v is k else (k, v):
+    if x.dtype != dtype or x.device != device:
+      raise ValueError("%s: %s is %s on %s, query is %s on %s" % (
+          who, name + ("key" if x is k else "value"), x.dtype, x.device, dtype, device))
+  shape = k.shape
+  if v is not k and v.shape != shape:
     raise ValueError("%s: %svalue %s is not shaped like %skey %s" % (who, name, tuple(v.shape), name,
-                                                                   tuple(k.shape)))
-  if k.shape[2] != q.shape[2]:
-    raise ValueError("%s: %skey has dim %d, query %d" % (who, name, k.shape[2], q.shape[2]))
-  if k.shape[1] < 1 or q.shape[1] % k.shape[1]:
-    raise ValueError("%s: %d query heads are no multiple of %d key heads" % (who, q.shape[1],
-                                                                           k.shape[1]))
+                                                                   tuple(shape)))
+  if shape[2] != q.shape[2]:
+    raise ValueError("%s: %skey has dim %d, query %d" % (who, name, shape[2], q.shape[2]))
+  if shape[1] < 1 or q.shape[1] % shape[1]:
+    raise ValueError("%s: %d query heads are no multiple of %d key heads" % (who, q.shape[1], shape[1]))
   return k, v
 
 
-def _rows(x: torch.Tensor) -> _lib.Rows:
-  return _lib.Rows(x.data_ptr(), x.stride(0), x.stride(1))
+def _splits(x, n_batch, device, name: str, who: str) -> torch.Tensor:
+  if not isinstance(x, torch.Tensor) or x.dim() != 1 or x.numel() < 1 or \
+      x.dtype not in (torch.int64, torch.int32):
+    raise ValueError("%s: %s must be an int64 vector [batch + 1]" % (who, name))
+  if x.device != device:
+    raise ValueError("%s: %s is on %s, query on %s" % (who, name, x.device, device))
+  if n_batch is not None and x.numel() != n_batch + 1:
+    raise ValueError("%s: %s has %d entries for a batch of %d" % (who, name, x.numel(), n_batch))
+  return x if x.dtype == torch.int64 and x.is_contiguous() else x.to(torch.int64).contiguous()
 
 
-def _args(q, k, v, key_splits, query_splits, key_mask, causal, scale) -> _lib.AttentionArgs:
-  a = _lib.AttentionArgs()
-  a.dtype = _DTYPES[q.dtype]
-  a.heads, a.dim = q.shape[1], q.shape[2]
-  a.causal, a.scale = int(causal), scale
-  a.n_query, a.query = q.shape[0], _rows(q)
-  a.kv_heads = k.shape[1]
-  if key_splits is not None:
-    a.n_key, a.key, a.value = k.shape[0], _rows(k), _rows(v)
-    a.key_splits = key_splits.data_ptr()
-    a.batch = key_splits.numel() - 1
-  else:
-    a.batch = q.shape[0]
-  if query_splits is not None:
-    a.query_splits = query_splits.data_ptr()
-    a.batch = query_splits.numel() - 1
-  if key_mask is not None:
-    a.key_mask = key_mask.data_ptr()
-  return a
+def _mask(x, n, device, name: str, who: str) -> Optional[torch.Tensor]:
+  if x is None:
+    return None
+  if x.dtype != torch.bool or x.dim() != 1 or x.numel() != n or x.device != device:
+    raise ValueError("%s: %s must be a bool vector of %d entries on %s" % (who, name, n, device))
+  return x.contiguous()
 
 
-def _call(fn, workspace, a: _lib.AttentionArgs, device) -> None:
-  n = workspace(C.byref(a))
-  if n < 0:
-    _lib.check(1)
-  if n:
-    ws = torch.empty(n, dtype=torch.uint8, device=device)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), n
-  _lib.launch(fn, a, device)
+def _scale(scale, dim, who) -> float:
+  if scale is None:
+    return 1.0 / math.sqrt(dim)
+  scale = float(scale)
+  if not (math.isfinite(scale) and scale > 0):
+    raise ValueError("%s: scale must be a positive finite number, got %r" % (who, scale))
+  return scale
+
+
+def _on_gpu(x: torch.Tensor, who: str):
+  if not x.is_cuda:
+    raise _lib.MonolithHipError("%s: tensors must live on the GPU (no CPU fallback)" % who)
+
+
+_NO_ROWS = (0, 0, 0)
+
+
+def _rows(x: Optional[torch.Tensor]):
+  return _NO_ROWS if x is None else (x.data_ptr(), x.stride(0), x.stride(1))
+
+
+def _ptr(x: Optional[torch.Tensor]) -> int:
+  return 0 if x is None else x.data_ptr()
+
+
+def _fields(q, k, v, key_splits, query_splits, key_mask, causal, scale, out, rest, lse, kv_heads=None,
+            prefix=(0, _NO_ROWS, _NO_ROWS, 0), backward=(0, _NO_ROWS, 0, 0, 0)):
+  """The fields of mono_attention_args up to the workspace."""
+  nq, heads, dim = q.shape
+  splits = key_splits if key_splits is not None else query_splits
+  key = _rows(k)
+  shared, grad_out, dq, dk, dv = backward
+  n_prefix, prefix_key, prefix_value, prefix_mask = prefix
+  return (_DTYPES[q.dtype], heads, k.shape[1] if kv_heads is None else kv_heads, dim, causal, shared,
+          nq if splits is None else splits.numel() - 1, nq, 0 if k is None else k.shape[0],
+          *_rows(q), *key, *(key if v is k else _rows(v)),
+          _ptr(query_splits), _ptr(key_splits), _ptr(key_mask), scale,
+          n_prefix, *prefix_key, *prefix_value, prefix_mask, out.data_ptr(), _ptr(rest), _ptr(lse),
+          *grad_out, dq, dk, dv)
 
 
 def _forward(q, k, v, key_splits, query_splits, key_mask, causal, scale, for_backward):
-  out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+  device = q.device
+  out = torch.empty(q.shape, dtype=q.dtype, device=device)
   lse = rest = None
-  a = _args(q, k, v, key_splits, query_splits, key_mask, causal, scale)
-  a.out = out.data_ptr()
   if for_backward:
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-    a.lse = lse.data_ptr()
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=device)
     if q.dtype == torch.bfloat16:
       rest = torch.empty_like(out)
-      a.out_rest = rest.data_ptr()
-  _call(_lib.lib.mono_ragged_attention, _lib.lib.mono_ragged_attention_workspace, a, q.device)
+  _lib.launch("mono_ragged_attention", _lib.pack_attention,
+              _fields(q, k, v, key_splits, query_splits, key_mask, causal, scale, out, rest, lse), device)
   return out, lse, rest
 
 
@@ -162,26 +149,19 @@ class _RaggedAttention(torch.autograd.Function):
   def backward(ctx, grad):
     query, key, value, key_splits, query_splits, key_mask, out, lse, rest = ctx.saved_tensors
     shared = value is None
-    a = _args(query, key, key if shared else value, key_splits, query_splits, key_mask, ctx.causal,
-              ctx.scale)
     grad = grad if grad.stride(2) == 1 and grad.dtype == query.dtype else \
         grad.to(query.dtype).contiguous()
     dq = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    a.kv_shared = int(shared)
-    a.out, a.lse, a.grad_out = out.data_ptr(), lse.data_ptr(), _rows(grad)
-    a.grad_query = dq.data_ptr()
-    if rest is not None:
-      a.out_rest = rest.data_ptr()
     dk = dv = None
-    keys = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-    if keys:
+    if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
       dk = torch.empty(key.shape, dtype=key.dtype, device=key.device)
-      a.grad_key = dk.data_ptr()
-    if keys and not shared:
-      dv = torch.empty(value.shape, dtype=value.dtype, device=value.device)
-      a.grad_value = dv.data_ptr()
-    _call(_lib.lib.mono_ragged_attention_gradient,
-          _lib.lib.mono_ragged_attention_gradient_workspace, a, query.device)
+      if not shared:
+        dv = torch.empty(value.shape, dtype=value.dtype, device=value.device)
+    _lib.launch("mono_ragged_attention_gradient", _lib.pack_attention,
+                _fields(query, key, key if shared else value, key_splits, query_splits, key_mask,
+                        ctx.causal, ctx.scale, out, rest, lse,
+                        backward=(shared, _rows(grad), dq.data_ptr(), _ptr(dk), _ptr(dv))),
+                query.device)
     return dq, dk, dv, None, None, None, None, None
 
 
@@ -215,7 +195,7 @@ def ragged_attention(query: torch.Tensor, key: torch.Tensor, value: Optional[tor
     out = _RaggedAttention.apply(q, k, None if value is None else v, ks, qs, mask, bool(causal),
                                  scale)
   else:
-    out = _forward(q, k, v, ks, qs, mask, causal, scale, False)[0]
+    out = _forward(q, k, v, ks, qs, mask, bool(causal), scale, False)[0]
   return out.view(query.shape) if query.dim() == 2 else out
 
 
@@ -257,11 +237,7 @@ def shared_prefix_attention(query: torch.Tensor, prefix_key: torch.Tensor,
   pmask = _mask(prefix_mask, pk.shape[0], q.device, "prefix_mask", who)
   _on_gpu(q, who)
   out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-  a = _args(q, pk if k is None else k, pv if k is None else v, ks, qs, mask, causal, scale)
-  a.n_prefix, a.prefix_key, a.prefix_value = pk.shape[0], _rows(pk), _rows(pv)
-  if pmask is not None:
-    a.prefix_mask = pmask.data_ptr()
-  a.out = out.data_ptr()
-  _call(_lib.lib.mono_shared_prefix_attention, _lib.lib.mono_shared_prefix_attention_workspace, a,
-        q.device)
+  _lib.launch("mono_shared_prefix_attention", _lib.pack_attention,
+              _fields(q, k, v, ks, qs, mask, bool(causal), scale, out, None, None, kv_heads=pk.shape[1],
+                      prefix=(pk.shape[0], _rows(pk), _rows(pv), _ptr(pmask))), q.device)
   return out.view(query.shape) if query.dim() == 2 else out

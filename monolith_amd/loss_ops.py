@@ -7,7 +7,6 @@ the reference's op set.
 The logits [n, vocab] never exist in memory. Sums and statistics are held in 32 bits; results are the
 same bit for bit from call to call. Nothing synchronises the host and scratch memory comes from
 torch's allocator, so loss and gradient can be captured into a HIP graph."""
-import ctypes as C
 import math
 from typing import Optional
 
@@ -19,35 +18,19 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1}  # MONO_ROW_*
 MAX_DIM = 256
 
 
-def _args(query, rows, labels, bias, scale) -> _lib.SoftmaxCeArgs:
-  a = _lib.SoftmaxCeArgs()
-  a.dtype, a.dim = _DTYPES[query.dtype], query.shape[1]
-  a.n, a.vocab = query.shape[0], rows.shape[0]
-  a.query, a.query_stride = query.data_ptr(), query.stride(0)
-  a.rows, a.rows_stride = rows.data_ptr(), rows.stride(0)
-  a.labels, a.scale = labels.data_ptr(), scale
-  if bias is not None:
-    a.bias = bias.data_ptr()
-  return a
-
-
-def _call(fn, workspace, a, device) -> None:
-  n = workspace(C.byref(a))
-  if n < 0:
-    _lib.check(1)
-  if n:
-    ws = torch.empty(n, dtype=torch.uint8, device=device)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), n
-  _lib.launch(fn, a, device)
+def _fields(query, rows, labels, bias, scale, loss, lse, grad_loss=0, dq=0, dw=0, db=0):
+  """The fields of mono_softmax_ce_args up to the workspace."""
+  return (_DTYPES[query.dtype], query.shape[1], query.shape[0], rows.shape[0],
+          query.data_ptr(), query.stride(0), rows.data_ptr(), rows.stride(0),
+          labels.data_ptr(), 0 if bias is None else bias.data_ptr(), scale, loss, lse.data_ptr(),
+          grad_loss, dq, dw, db)
 
 
 def _forward(query, rows, labels, bias, scale):
   loss = torch.empty(query.shape[0], dtype=torch.float32, device=query.device)
   lse = torch.empty_like(loss)
-  a = _args(query, rows, labels, bias, scale)
-  a.loss, a.lse = loss.data_ptr(), lse.data_ptr()
-  _call(_lib.lib.mono_softmax_cross_entropy, _lib.lib.mono_softmax_cross_entropy_workspace, a,
-        query.device)
+  _lib.launch("mono_softmax_cross_entropy", _lib.pack_softmax_ce,
+              _fields(query, rows, labels, bias, scale, loss.data_ptr(), lse), query.device)
   return loss, lse
 
 
@@ -64,21 +47,22 @@ class _SoftmaxCrossEntropy(torch.autograd.Function):
   @torch.autograd.function.once_differentiable
   def backward(ctx, grad):
     query, rows, labels, bias, lse = ctx.saved_tensors
-    a = _args(query, rows, labels, bias, ctx.scale)
-    grad = grad.to(torch.float32).contiguous()
-    a.lse, a.grad_loss = lse.data_ptr(), grad.data_ptr()
+    if grad.dtype != torch.float32 or not grad.is_contiguous():
+      grad = grad.to(torch.float32).contiguous()
     dq = dw = db = None
+    ptrs = [0, 0, 0]
     if ctx.needs_input_grad[0]:
       dq = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-      a.grad_query = dq.data_ptr()
+      ptrs[0] = dq.data_ptr()
     if ctx.needs_input_grad[1]:
       dw = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
-      a.grad_rows = dw.data_ptr()
+      ptrs[1] = dw.data_ptr()
     if bias is not None and ctx.needs_input_grad[3]:
       db = torch.empty_like(bias)
-      a.grad_bias = db.data_ptr()
-    _call(_lib.lib.mono_softmax_cross_entropy_gradient,
-          _lib.lib.mono_softmax_cross_entropy_gradient_workspace, a, query.device)
+      ptrs[2] = db.data_ptr()
+    _lib.launch("mono_softmax_cross_entropy_gradient", _lib.pack_softmax_ce,
+                _fields(query, rows, labels, bias, ctx.scale, 0, lse, grad.data_ptr(), *ptrs),
+                query.device)
     return dq, dw, None, db, None
 
 

@@ -152,6 +152,23 @@ def test_c_cross_entropy_refuses():
   assert b"too small" in _lib.lib.mono_last_error()
 
 
+def test_packed_arguments_are_the_structures():
+  """The packed form that the operators pass is the ctypes.Structure's image, field by field."""
+  def image(cls, pack):
+    names, kinds = [], []
+    for n, t in cls._fields_:
+      for m, u in (t._fields_ if issubclass(t, C.Structure) else [(None, t)]):
+        names.append((n, m))
+        kinds.append(u)
+    values = [(0.5 * i if u is C.c_float else i + 1) for i, u in enumerate(kinds)]
+    a = cls()
+    for (n, m), v in zip(names, values):
+      setattr(getattr(a, n) if m else a, m or n, v)
+    assert bytes(a) == pack(*values)
+  image(_lib.AttentionArgs, _lib.pack_attention)
+  image(_lib.SoftmaxCeArgs, _lib.pack_softmax_ce)
+
+
 def test_structures_have_the_header_s_size():
   assert C.sizeof(_lib.AttentionArgs) == 304 and C.sizeof(_lib.SoftmaxCeArgs) == 144
 
