@@ -459,10 +459,11 @@ int mono_embedding_to_layout_grad(const mono_layout_slice* h_slices, int n_slice
  * No counterpart in the reference's op set. Row types: MONO_ROW_FP32, MONO_ROW_BF16; every sum,
  * softmax statistic and partial result is fp32. Nothing here allocates or synchronises (safe under
  * HIP graph capture): scratch is the caller's, sized by the *_workspace function for the same
- * arguments, and belongs to one call at a time. Ragged rows are given by splits int64[batch + 1],
+ * arguments, 16-byte aligned, and belongs to one call at a time. Ragged rows are given by splits int64[batch + 1],
  * non-decreasing, inside [0, rows]; rows in front of the first split and behind the last belong to
  * no sequence (their outputs and gradients are zero). Splits that break this give wrong values, but
- * no access outside the arrays. Rows are [rows, heads, dim] with the last dimension contiguous. */
+ * no access outside the arrays. fp32 rows are multiplied as three bf16 numbers each (24 bits): elements
+ * have to be finite where a query sees them, an infinite one gives NaN. Rows are [rows, heads, dim] with the last dimension contiguous. */
 enum { MONO_ROW_FP32 = 0, MONO_ROW_BF16 = 1 };
 typedef struct {
   const void* ptr;
@@ -478,7 +479,7 @@ typedef struct {
   const int64_t* query_splits;   /* NULL: one query per sequence (n_query == batch) */
   const int64_t* key_splits;
   const uint8_t* key_mask;       /* [n_key], 0 = no query sees this key; may be NULL */
-  float scale;                   /* of the products, before the softmax */
+  float scale;                   /* of the products, before the softmax: 1e-20 .. 1e20 */
   /* shared prefix (mono_shared_prefix_attention only) */
   int64_t n_prefix;
   mono_rows prefix_key, prefix_value;
@@ -512,14 +513,14 @@ int mono_shared_prefix_attention(const mono_attention_args* args, void* stream);
  * label is taken out has a loss of +inf and no gradient. */
 typedef struct {
   int32_t dtype, dim;            /* 1 <= dim <= 256 */
-  int64_t n, vocab;
+  int64_t n, vocab;              /* n < 2^26 */
   const void* query;             /* [n, dim], rows query_stride elements apart */
   int64_t query_stride;
   const void* rows;              /* [vocab, dim] */
   int64_t rows_stride;
   const int64_t* labels;         /* [n] */
   const float* bias;             /* [vocab], may be NULL */
-  float scale;
+  float scale;                   /* 1e-20 .. 1e20 */
   float* loss;                   /* [n] */
   float* lse;                    /* [n], in units of log 2; +inf: the row has no gradient */
   const float* grad_loss;        /* backward: [n] */

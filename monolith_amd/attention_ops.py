@@ -9,7 +9,8 @@ head); the sequences of a batch lie one behind the other and are given by int64 
 Rows in front of the first split and behind the last (the padding of a fixed-size buffer) belong to
 no sequence: their outputs and gradients are zero. Splits that break this give wrong values, never
 an access outside the tensors. Softmax statistics and sums are held in 32 bits; results have the
-rows' type and are the same bit for bit from call to call. Nothing synchronises the host, and
+rows' type and are the same bit for bit from call to call. Elements that a query sees have to be finite
+(float32 rows are multiplied as three bfloat16 numbers each; an infinite element gives NaN). Nothing synchronises the host, and
 scratch memory comes from torch's allocator, so every op can be captured into a HIP graph."""
 import math
 from typing import Optional
@@ -84,8 +85,8 @@ def _scale(scale, dim, who) -> float:
   if scale is None:
     return 1.0 / math.sqrt(dim)
   scale = float(scale)
-  if not (math.isfinite(scale) and scale > 0):
-    raise ValueError("%s: scale must be a positive finite number, got %r" % (who, scale))
+  if not 1e-20 <= scale <= 1e20:
+    raise ValueError("%s: scale must be in [1e-20, 1e20], got %r" % (who, scale))
   return scale
 
 

@@ -136,7 +136,7 @@ __global__ __launch_bounds__(NW * 64, DP * sizeof(T) <= 256 ? 2 : 1) void k_attn
     tok[c] = ok[c] ? (int)(r / a.G) : 0;
     head[c] = kvh * a.G + (ok[c] ? (int)(r % a.G) : 0);
     int lim = sk.n;
-    if (a.causal) lim = min(lim, max(0, tok[c] + 1 + sk.n - sq.n));
+    if (a.causal) lim = min(lim, max(0, sk.n - sq.n + tok[c] + 1));
     klim[c] = ok[c] ? lim : 0;
     if (ok[c]) kmin = min(kmin, lim), kmax = max(kmax, lim);
     M::load_cols(qf[c], (const T*)a.q + (int64_t)(sq.lo + tok[c]) * a.qs + (int64_t)head[c] * a.qh, ok[c],
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(NW * 64, DP * sizeof(T) <= 256 ? 2 : 1) void k_attn
   int kend = sk.n;
   if (a.causal) {
     const int last = (int)((min(r0 + BM, nrow) - 1) / a.G);
-    kend = min(kend, max(0, last + 1 + sk.n - sq.n));
+    kend = min(kend, max(0, sk.n - sq.n + last + 1));
   }
   int kbeg = 0;
   if (a.nsplit > 1) {
@@ -276,32 +276,33 @@ template <typename T>
 __global__ __launch_bounds__(256) void k_attn_join(const float* part, const float* part_lse, Parts parts,
                                                    int64_t rows, int D, T* out, T* rest, float* lse, int vec) {
   const int d4 = (D + 3) / 4;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / d4;
-  const int d0 = (int)(i % d4) * 4;
-  if (row >= rows) return;
-  int64_t first, step;
-  const int n = parts.of(row, &first, &step);
-  float m = neg_inf();
-  for (int s = 0; s < n; ++s) m = fmaxf(m, part_lse[first + s * step]);
-  const float base = m == neg_inf() ? 0.f : m;
-  f4 t = {0.f, 0.f, 0.f, 0.f};
-  float z = 0.f;
-  for (int s = 0; s < n; ++s) {
-    const float w = exp2_hw(part_lse[first + s * step] - base);
-    const float* p = part + (first + s * step) * D + d0;
-    z += w;
-    if (vec) {
-      t += w * *(const f4*)p;
-    } else {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * d4; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / d4;
+    const int d0 = (int)(i % d4) * 4;
+    int64_t first, step;
+    const int n = parts.of(row, &first, &step);
+    float m = neg_inf();
+    for (int s = 0; s < n; ++s) m = fmaxf(m, part_lse[first + s * step]);
+    const float base = m == neg_inf() ? 0.f : m;
+    f4 t = {0.f, 0.f, 0.f, 0.f};
+    float z = 0.f;
+    for (int s = 0; s < n; ++s) {
+      const float w = exp2_hw(part_lse[first + s * step] - base);
+      const float* p = part + (first + s * step) * D + d0;
+      z += w;
+      if (vec) {
+        t += w * *(const f4*)p;
+      } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (d0 + j < D) t[j] = fmaf(w, p[j], t[j]);
+        for (int j = 0; j < 4; ++j)
+          if (d0 + j < D) t[j] = fmaf(w, p[j], t[j]);
+      }
     }
+    t *= z == 0.f ? 0.f : 1.f / z;
+    store4(out + row * D, d0, D, t, vec);
+    if (rest) store4(rest + row * D, d0, D, rest_of<T>(t), vec);
+    if (lse && d0 == 0) lse[row] = z == 0.f ? neg_inf() : m + __log2f(z);
   }
-  t *= z == 0.f ? 0.f : 1.f / z;
-  store4(out + row * D, d0, D, t, vec);
-  if (rest) store4(rest + row * D, d0, D, rest_of<T>(t), vec);
-  if (lse && d0 == 0) lse[row] = z == 0.f ? neg_inf() : m + __log2f(z);
 }
 
 // The same for many parts of few rows: a workgroup per row, its threads as groups of d4 that take every
@@ -397,7 +398,7 @@ __global__ __launch_bounds__(NW * 64, DP <= 64 || (sizeof(T) == 2 && NW > 1) ? 2
     tok[c] = ok[c] ? (int)(r / a.G) : 0;
     head[c] = kvh * a.G + (ok[c] ? (int)(r % a.G) : 0);
     int lim = sk.n;
-    if (a.causal) lim = min(lim, max(0, tok[c] + 1 + sk.n - sq.n));
+    if (a.causal) lim = min(lim, max(0, sk.n - sq.n + tok[c] + 1));
     klim[c] = ok[c] ? lim : 0;
     if (ok[c]) kmin = min(kmin, lim), kmax = max(kmax, lim);
     const int64_t t = sq.lo + tok[c], row = t * a.H + head[c];
@@ -423,7 +424,7 @@ __global__ __launch_bounds__(NW * 64, DP <= 64 || (sizeof(T) == 2 && NW > 1) ? 2
   int kend = sk.n;
   if (a.causal) {
     const int last = (int)((min(r0 + BM, nrow) - 1) / a.G);
-    kend = min(kend, max(0, last + 1 + sk.n - sq.n));
+    kend = min(kend, max(0, sk.n - sq.n + last + 1));
   }
   int kbeg = 0;
   if (a.nsplit > 1) {
@@ -953,11 +954,14 @@ int check(const mono_attention_args* p, const char* who) {
   MONO_REQUIRE(p->dim >= 1 && p->dim <= 128, "%s: dim must be in [1, 128], got %d", who, p->dim);
   MONO_REQUIRE(p->heads >= 1 && p->kv_heads >= 1 && p->heads % p->kv_heads == 0,
                "%s: heads (%d) must be a positive multiple of kv_heads (%d)", who, p->heads, p->kv_heads);
-  MONO_REQUIRE(p->scale > 0.f && p->scale < __builtin_inff(), "%s: scale must be positive and finite", who);
+  MONO_REQUIRE(p->scale >= 1e-20f && p->scale <= 1e20f, "%s: scale must be in [1e-20, 1e20], got %g", who,
+               (double)p->scale);
   MONO_REQUIRE(p->batch >= 0 && p->n_query >= 0 && p->n_key >= 0 && p->n_prefix >= 0, "%s: negative size", who);
-  MONO_REQUIRE(p->n_query * p->heads < (1LL << 31) && p->n_key * p->kv_heads < (1LL << 31) &&
-                   p->n_prefix * p->kv_heads < (1LL << 31) && p->batch * p->kv_heads < (1LL << 31),
+  constexpr int64_t kMost = (1LL << 31) - 65536;
+  MONO_REQUIRE(p->n_query <= kMost / p->heads && p->n_key <= kMost / p->kv_heads &&
+                   p->n_prefix <= kMost / p->kv_heads && p->batch <= kMost / p->kv_heads,
                "%s: more than 2^31 rows", who);
+  MONO_REQUIRE(((uintptr_t)p->workspace & 15) == 0, "%s: workspace must be 16-byte aligned", who);
   MONO_REQUIRE(p->query_splits || p->n_query == p->batch,
                "%s: without query_splits there is one query per sequence (n_query %lld, batch %lld)", who,
                (long long)p->n_query, (long long)p->batch);
@@ -1056,7 +1060,7 @@ int launch1(const Args& a, const Plan& pl, hipStream_t st) {
 template <int W, typename T, int DP, int GT>
 int launch_pool2(const Args& a, hipStream_t st) {
   const int64_t wgs = ((a.chunk ? pool_tiles(a.B, a.nk, a.chunk) : (int64_t)a.B * a.nsplit) * a.Hkv + 3) / 4;
-  MONO_REQUIRE(wgs < (1LL << 31) - 64, "attention: too many sequences");
+  MONO_REQUIRE(wgs < (1LL << 24) - 64, "attention: too many sequences");
   if (W == kFwd) k_pool_fwd<T, DP, GT><<<(unsigned)wgs, 256, 0, st>>>(a);
   else k_pool_bwd<T, DP, GT><<<(unsigned)wgs + 64, 256, 0, st>>>(a);
   MONO_HIP(hipGetLastError());
@@ -1086,7 +1090,7 @@ int launch_pool(int dtype, const Args& a, hipStream_t st) {
 template <int W, typename T, int DP>
 int launch2(const Args& a, const Plan& pl, hipStream_t st) {
   if (pl.tiles * a.Hkv == 0) return 0;
-  MONO_REQUIRE(pl.tiles * a.Hkv < (1LL << 31), "attention: too many tiles");
+  MONO_REQUIRE(pl.tiles * a.Hkv < (1LL << 24), "attention: too many tiles");
   constexpr bool half = sizeof(T) == 2;
   if constexpr (half || DP <= 32)
     if (pl.sh.nw == 1) return launch1<W, T, DP, 1, 1>(a, pl, st);
@@ -1119,7 +1123,7 @@ int join(const mono_attention_args* p, const float* part, const float* part_lse,
   if (rows == 0) return 0;
   const int vec = p->dim % 4 == 0 && (((uintptr_t)p->out | (uintptr_t)p->out_rest) & 15) == 0;
   const bool many = chunk || n_part >= 16;
-  const unsigned grid = (unsigned)(many ? rows : (rows * ((p->dim + 3) / 4) + 255) / 256);
+  const unsigned grid = many ? (unsigned)rows : (unsigned)grid_for(rows * ((p->dim + 3) / 4), 256, 1 << 20);
   const Parts parts = parts_of(p, n_part, rows, chunk);
   const auto go = [&](auto* out) {
     typedef typename std::remove_pointer<decltype(out)>::type T;
@@ -1174,6 +1178,8 @@ int mono_ragged_attention(const mono_attention_args* p, void* stream) {
   MONO_TRY(check(p, "mono_ragged_attention"));
   MONO_REQUIRE(p->key_splits, "mono_ragged_attention: key_splits is NULL");
   if (p->n_query == 0) return 0;
+  MONO_REQUIRE(p->query.ptr && p->out && (p->n_key == 0 || (p->key.ptr && p->value.ptr)),
+               "mono_ragged_attention: a rows array is NULL");
   const Plan pl = plan_fwd(p);
   const int64_t rows = pl.part_rows(p->n_query * p->heads, p->heads);
   MONO_REQUIRE(p->workspace_bytes >= parts_bytes(rows, p->dim),
@@ -1206,6 +1212,9 @@ int mono_ragged_attention_gradient(const mono_attention_args* p, void* stream) {
   MONO_REQUIRE(p->workspace_bytes >= mono_ragged_attention_gradient_workspace(p),
                "mono_ragged_attention_gradient: workspace of %lld bytes is too small",
                (long long)p->workspace_bytes);
+  MONO_REQUIRE(p->n_query == 0 || (p->query.ptr && p->out && p->lse && p->grad_out.ptr && p->grad_query),
+               "mono_ragged_attention_gradient: a rows array of the queries is NULL");
+  MONO_REQUIRE(p->n_key == 0 || (p->key.ptr && p->value.ptr), "mono_ragged_attention_gradient: key or value is NULL");
   hipStream_t st = (hipStream_t)stream;
   const Plan plq = plan_fwd(p), plk = plan_dkv(p);
   const int64_t rows = p->n_query * p->heads, krows = p->n_key * p->kv_heads;
@@ -1241,6 +1250,9 @@ int64_t mono_shared_prefix_attention_workspace(const mono_attention_args* p) {
 int mono_shared_prefix_attention(const mono_attention_args* p, void* stream) {
   MONO_TRY(check(p, "mono_shared_prefix_attention"));
   if (p->n_query == 0) return 0;
+  MONO_REQUIRE(p->query.ptr && p->out && (!p->key_splits || p->n_key == 0 || (p->key.ptr && p->value.ptr)) &&
+                   (p->n_prefix == 0 || (p->prefix_key.ptr && p->prefix_value.ptr)),
+               "mono_shared_prefix_attention: a rows array is NULL");
   const PrefixPlan pl = plan_prefix(p);
   const int64_t rows = p->n_query * p->heads;
   MONO_REQUIRE(p->workspace_bytes >= (pl.slots > 1 ? parts_bytes(pl.slots * rows, p->dim) : 0),

@@ -119,7 +119,7 @@ __global__ __launch_bounds__(256, DP <= 128 || sizeof(T) == 2 ? 2 : 1) void k_ce
 template <typename T>
 __global__ __launch_bounds__(256) void k_ce_loss(Args a) {
   const int lane = threadIdx.x & 63;
-  const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (i >= a.n) return;
   float m = neg_inf();
   for (int s = lane; s < a.nsplit; s += 64) m = fmaxf(m, a.part[(int64_t)s * a.n + i]);
@@ -134,7 +134,7 @@ __global__ __launch_bounds__(256) void k_ce_loss(Args a) {
   float hit = 0.f;
   if (known)
     for (int d = lane; d < a.D; d += 64)
-      hit = fmaf((float)((const T*)a.q)[(int64_t)i * a.qs + d], (float)((const T*)a.w)[label * a.ws + d], hit);
+      hit = fmaf((float)((const T*)a.q)[i * a.qs + d], (float)((const T*)a.w)[label * a.ws + d], hit);
 #pragma unroll
   for (int x = 32; x; x >>= 1) {
     z += __shfl_xor(z, x);
@@ -408,9 +408,11 @@ int check(const mono_softmax_ce_args* p, const char* who) {
   MONO_REQUIRE(p != nullptr, "%s: args is NULL", who);
   MONO_REQUIRE(p->dtype == MONO_ROW_FP32 || p->dtype == MONO_ROW_BF16, "%s: unknown row type %d", who, p->dtype);
   MONO_REQUIRE(p->dim >= 1 && p->dim <= 256, "%s: dim must be in [1, 256], got %d", who, p->dim);
-  MONO_REQUIRE(p->scale > 0.f && p->scale < __builtin_inff(), "%s: scale must be positive and finite", who);
-  MONO_REQUIRE(p->n >= 0 && p->vocab >= 1 && p->n < (1LL << 31) - 65536 && p->vocab < (1LL << 31) - 65536,
+  MONO_REQUIRE(p->scale >= 1e-20f && p->scale <= 1e20f, "%s: scale must be in [1e-20, 1e20], got %g", who,
+               (double)p->scale);
+  MONO_REQUIRE(p->n >= 0 && p->vocab >= 1 && p->n < (1LL << 26) && p->vocab < (1LL << 31) - 65536,
                "%s: %lld queries and %lld rows are out of range", who, (long long)p->n, (long long)p->vocab);
+  MONO_REQUIRE(((uintptr_t)p->workspace & 15) == 0, "%s: workspace must be 16-byte aligned", who);
   return 0;
 }
 Args base_args(const mono_softmax_ce_args* p) {
@@ -469,6 +471,8 @@ int64_t mono_softmax_cross_entropy_workspace(const mono_softmax_ce_args* p) {
 int mono_softmax_cross_entropy(const mono_softmax_ce_args* p, void* stream) {
   MONO_TRY(check(p, "mono_softmax_cross_entropy"));
   if (p->n == 0) return 0;
+  MONO_REQUIRE(p->query && p->rows && p->labels && p->loss && p->lse,
+               "mono_softmax_cross_entropy: an array is NULL");
   MONO_REQUIRE(p->workspace_bytes >= mono_softmax_cross_entropy_workspace(p),
                "mono_softmax_cross_entropy: workspace of %lld bytes is too small", (long long)p->workspace_bytes);
   hipStream_t st = (hipStream_t)stream;
@@ -515,6 +519,8 @@ int64_t mono_softmax_cross_entropy_gradient_workspace(const mono_softmax_ce_args
 int mono_softmax_cross_entropy_gradient(const mono_softmax_ce_args* p, void* stream) {
   MONO_TRY(check(p, "mono_softmax_cross_entropy_gradient"));
   Args a = base_args(p);
+  MONO_REQUIRE(p->rows && (p->n == 0 || (p->query && p->labels && p->lse && p->grad_loss)),
+               "mono_softmax_cross_entropy_gradient: an array is NULL");
   MONO_REQUIRE(p->workspace_bytes >= place_parts(p, &a),
                "mono_softmax_cross_entropy_gradient: workspace of %lld bytes is too small",
                (long long)p->workspace_bytes);

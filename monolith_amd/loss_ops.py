@@ -7,7 +7,6 @@ the reference's op set.
 The logits [n, vocab] never exist in memory. Sums and statistics are held in 32 bits; results are the
 same bit for bit from call to call. Nothing synchronises the host and scratch memory comes from
 torch's allocator, so loss and gradient can be captured into a HIP graph."""
-import math
 from typing import Optional
 
 import torch
@@ -89,6 +88,8 @@ def softmax_cross_entropy(query: torch.Tensor, rows: torch.Tensor, labels: torch
         who, MAX_DIM, tuple(query.shape), tuple(rows.shape)))
   if rows.shape[0] < 1:
     raise ValueError("%s: there are no rows" % who)
+  if query.shape[0] >= 2 ** 26:
+    raise ValueError("%s: %d queries are too many for one call" % (who, query.shape[0]))
   if not isinstance(labels, torch.Tensor) or labels.dtype != torch.int64 or \
       labels.shape != query.shape[:1] or labels.device != query.device:
     raise ValueError("%s: labels must be an int64 vector [%d] on %s" % (who, query.shape[0],
@@ -98,8 +99,8 @@ def softmax_cross_entropy(query: torch.Tensor, rows: torch.Tensor, labels: torch
     raise ValueError("%s: bias must be a float32 vector [%d] on %s" % (who, rows.shape[0],
                                                                       query.device))
   scale = float(scale)
-  if not (math.isfinite(scale) and scale > 0):
-    raise ValueError("%s: scale must be a positive finite number, got %r" % (who, scale))
+  if not 1e-20 <= scale <= 1e20:
+    raise ValueError("%s: scale must be in [1e-20, 1e20], got %r" % (who, scale))
   if not query.is_cuda:
     raise _lib.MonolithHipError("%s: tensors must live on the GPU (no CPU fallback)" % who)
   query = query if query.stride(1) == 1 else query.contiguous()

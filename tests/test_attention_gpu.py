@@ -95,6 +95,16 @@ def test_long_histories_are_split(dtype, H, Hkv, D):
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_one_long_history_among_short_ones(dtype):
+  """Parts of equal keys: most sequences have one, some none, one has hundreds."""
+  rng = np.random.default_rng(30)
+  lens = [1, 0, 0, 700, 2, 150000, 0, 129, 1, 0]
+  run_both(rng, dtype, 2, 1, 16, None, lens, mask=0.2, pad=(3, 70))
+  run_both(rng, dtype, 3, 1, 8, None, lens, shared=True)
+  run_both(rng, dtype, 5, 1, 8, None, [1, 0, 9000, 3])
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_few_keys_under_many_queries(dtype):
   """The pass over keys splits the queries: the keys' gradients are joined from partial sums."""
   rng = np.random.default_rng(3)
@@ -362,7 +372,7 @@ def test_query_gradient_alone():
 @pytest.mark.parametrize("prefix,lq,lk", [
     (1, None, [0, 1, 3]), (300, None, None), (300, None, [0, 40, 7, 64, 1]), (0, None, [4, 0, 9]),
     (77, [1, 3, 2, 0, 70], [5, 3, 40, 6, 70]), (5000, [1, 2], [0, 2]), (5000, [3, 1, 2], None),
-    (2000, [50] * 6, [60] * 6)])
+    (2000, [50] * 6, [60] * 6), (40, None, [3000, 5, 0, 700]), (40, [2, 1, 3], [3000, 5, 700])])
 def test_shared_prefix(dtype, H, Hkv, D, prefix, lq, lk):
   """Every query over the prefix and its own keys: the restatement has both as one list of keys."""
   from monolith_amd import attention_ops

@@ -32,7 +32,7 @@ BAD_ATTENTION = [
     dict(query_splits=torch.tensor([0, 6])), dict(query_splits=None),
     dict(key_mask=torch.ones(8, dtype=torch.bool)), dict(key_mask=torch.ones(9)),
     dict(key_mask=torch.ones(9, 1, dtype=torch.bool)),
-    dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")),
+    dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=1e-21),
 ]
 
 
@@ -109,7 +109,8 @@ def _c_attention(**kw):
 
 BAD_C = [dict(dtype=2), dict(dtype=-1), dict(dim=0), dict(dim=129), dict(heads=0), dict(kv_heads=0),
          dict(heads=3, kv_heads=2), dict(batch=-1), dict(n_query=-1), dict(n_key=-1), dict(n_prefix=-1),
-         dict(n_query=3), dict(n_query=2 ** 31, query_splits=64), dict(n_key=2 ** 31)]
+         dict(n_query=3), dict(n_query=2 ** 31, query_splits=64), dict(n_key=2 ** 31), dict(scale=0.0),
+         dict(scale=float("nan")), dict(scale=-1.0), dict(scale=float("inf")), dict(workspace=8)]
 
 
 @pytest.mark.parametrize("i", range(len(BAD_C)))
@@ -124,21 +125,29 @@ def test_c_attention_refuses(i):
 def test_c_small_workspaces_and_missing_pointers_are_refused():
   long = _c_attention(batch=1, n_query=1, n_key=100000)
   assert _lib.lib.mono_ragged_attention_workspace(C.byref(long)) > 0
+  assert _lib.lib.mono_ragged_attention_gradient(C.byref(long), None) != 0
+  assert b"too small" in _lib.lib.mono_last_error()
   for name in ("mono_ragged_attention", "mono_ragged_attention_gradient"):
-    assert getattr(_lib.lib, name)(C.byref(long), None) != 0
-    assert b"too small" in _lib.lib.mono_last_error()
     assert getattr(_lib.lib, name)(None, None) != 0
     a = _c_attention(key_splits=None)
     assert getattr(_lib.lib, name)(C.byref(a), None) != 0
     assert b"key_splits" in _lib.lib.mono_last_error()
+  for name in ("mono_ragged_attention", "mono_ragged_attention_gradient", "mono_shared_prefix_attention"):
+    a = _c_attention(workspace=64, workspace_bytes=2 ** 30)
+    assert getattr(_lib.lib, name)(C.byref(a), None) != 0
+    assert b"NULL" in _lib.lib.mono_last_error()
   pre = _c_attention(n_prefix=100000)
+  pre.query.ptr = pre.out = pre.key.ptr = pre.value.ptr = pre.prefix_key.ptr = pre.prefix_value.ptr = 64
+  long.query.ptr = long.out = long.key.ptr = long.value.ptr = 64
+  assert _lib.lib.mono_ragged_attention(C.byref(long), None) != 0
+  assert b"too small" in _lib.lib.mono_last_error()
   assert _lib.lib.mono_shared_prefix_attention(C.byref(pre), None) != 0
   assert b"too small" in _lib.lib.mono_last_error()
 
 
 def test_c_cross_entropy_refuses():
   for kw in (dict(dtype=2), dict(dim=0), dict(dim=257), dict(n=-1), dict(vocab=0), dict(vocab=2 ** 31),
-             dict(n=2 ** 31)):
+             dict(n=2 ** 26), dict(scale=0.0), dict(scale=1e30), dict(workspace=4)):
     a = _lib.SoftmaxCeArgs()
     a.dim, a.n, a.vocab, a.scale = 16, 4, 100, 1.0
     for n, v in kw.items():
@@ -148,6 +157,10 @@ def test_c_cross_entropy_refuses():
       assert getattr(_lib.lib, name + "_workspace")(C.byref(a)) == -1
   a = _lib.SoftmaxCeArgs()
   a.dim, a.n, a.vocab, a.scale = 16, 40, 100000, 1.0
+  for name in ("mono_softmax_cross_entropy", "mono_softmax_cross_entropy_gradient"):
+    assert getattr(_lib.lib, name)(C.byref(a), None) != 0
+    assert b"NULL" in _lib.lib.mono_last_error()
+  a.query = a.rows = a.labels = a.loss = a.lse = 64
   assert _lib.lib.mono_softmax_cross_entropy(C.byref(a), None) != 0
   assert b"too small" in _lib.lib.mono_last_error()
 
