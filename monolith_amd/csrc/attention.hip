@@ -88,9 +88,10 @@ int64_t tiles_for(int mode, int64_t B, int64_t n, int64_t G, int BM) {
 }
 
 // rows of a streamed tile: 64 where one takes the registers of 64 bytes a thread or less on its way to LDS
-template <typename T, int DP, int NW>
+// (the forward, which keeps one product less, also for bf16 rows of 128)
+template <typename T, int DP, int NW, bool FWD = false>
 struct Tile {
-  static constexpr int BN = NW > 1 && DP * sizeof(T) <= 128 ? 64 : 32, NR = BN / 32;
+  static constexpr int BN = NW > 1 && DP * sizeof(T) <= (FWD && sizeof(T) == 2 ? 256 : 128) ? 64 : 32, NR = BN / 32;
 };
 
 // v where a column's key (rows y of a tile, from its row 0 on) is not below lim or not alive
@@ -108,7 +109,7 @@ __device__ inline void hide(f16v& s, int lim, const uint8_t* alive, float v, int
 // ---- forward -------------------------------------------------------------------------------
 template <typename T, int DP, int NC, int NW>
 __global__ __launch_bounds__(NW * 64, DP * sizeof(T) <= 256 ? 2 : 1) void k_attn_fwd(Args a) {
-  constexpr int BM = NC * NW * 32, BN = Tile<T, DP, NW>::BN, NR = Tile<T, DP, NW>::NR, NT = NW * 64;
+  constexpr int BM = NC * NW * 32, BN = Tile<T, DP, NW, true>::BN, NR = Tile<T, DP, NW, true>::NR, NT = NW * 64;
   typedef Stage<T, DP, BN, NT> St;
   typedef Mma<T, DP, St::PLANE> M;
   __shared__ __align__(16) bf16 lk[St::LDS];
