@@ -653,7 +653,8 @@ __global__ __launch_bounds__(256) void k_sum_parts(const float* part, Parts part
 // would hold one column. One wave walks the keys of a sequence (or of its split): LPR lanes hold a key's
 // row, 16 bytes each, so a wave takes R = 64 / LPR keys at once and U times that per turn; every group
 // of LPR lanes keeps softmax statistics of its own, joined behind the loop. GT query heads of the key
-// head share what is read.
+// head share what is read. 16384 rows of 825261 keys x 32 floats: 36 us, 2.9 TB/s (a large read reaches 4.0);
+// the next keys' loads ahead of the present ones' sums took as long (37 us, 104 registers for 54).
 template <typename T>
 struct Chunk {
   static constexpr int E = 16 / sizeof(T);
