@@ -261,7 +261,13 @@ __global__ __launch_bounds__(NW * 64, DP * sizeof(T) <= 256 ? 2 : 1) void k_attn
   }
 }
 
-// Where the parts of a row lie: part s at first + s * step.
+// Pooled rows in parts of `chunk` keys: only a sequence of more than one part has partial results. It has
+// ceil(length / chunk) <= floor(2 length / chunk) of them, so they lie from floor(2 start / chunk) on without
+// meeting the next one's.
+__device__ __host__ inline int64_t pool_part(int64_t start, int chunk) { return 2 * start / chunk; }
+
+// Where the parts of a row lie: part s at first + s * step; of() returns how many there are, 0 where the row
+// is whole and written already.
 struct Parts {
   int n;                // parts of a row (chunk = 0)
   int64_t rows;         // rows of a part
@@ -274,14 +280,11 @@ struct Parts {
       return n;
     }
     const int b = (int)(row / H), lo = split_at(ksp, b, nk), hi = split_at(ksp, b + 1, nk);
-    *first = (int64_t)(lo / chunk + b + 1) * H + row % H;
+    *first = pool_part(lo, chunk) * H + row % H;
     *step = H;
-    return hi > lo ? (hi - lo + chunk - 1) / chunk : 1;
+    return hi - lo > chunk ? (int)(((int64_t)hi - lo + chunk - 1) / chunk) : 0;
   }
 };
-// out = sum of the parts' results, each weighted by its share of the softmax's sum (a part without a key
-// holds zeros and a statistic of -inf: its weight is 0). A thread takes four elements of a row through
-// all parts.
 template <typename T>
 __global__ __launch_bounds__(256) void k_attn_join(const float* part, const float* part_lse, Parts parts,
                                                    int64_t rows, int D, T* out, T* rest, float* lse, int vec) {
@@ -291,6 +294,7 @@ __global__ __launch_bounds__(256) void k_attn_join(const float* part, const floa
     const int d0 = (int)(i % d4) * 4;
     int64_t first, step;
     const int n = parts.of(row, &first, &step);
+    if (n == 0) continue;
     float m = neg_inf();
     for (int s = 0; s < n; ++s) m = fmaxf(m, part_lse[first + s * step]);
     const float base = m == neg_inf() ? 0.f : m;
@@ -327,6 +331,7 @@ __global__ __launch_bounds__(1024) void k_attn_join_many(const float* part, cons
   const int64_t row = blockIdx.x;
   int64_t first, step;
   const int n = parts.of(row, &first, &step);
+  if (n == 0) return;
   float m = neg_inf();
   for (int s = tid; s < n; s += 1024) m = fmaxf(m, part_lse[first + s * step]);
   m = over_lanes<1, 64, Max>(m);
@@ -640,6 +645,7 @@ __global__ __launch_bounds__(256) void k_sum_parts(const float* part, Parts part
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     int64_t first, step;
     const int n = parts.of(i / D, &first, &step);
+    if (n == 0) continue;
     const float* p = part + first * D + i % D;
     float t = 0.f;
 #pragma unroll 8
@@ -705,34 +711,55 @@ __device__ inline void split_range(int n, int nsplit, int split, int step, int* 
 }
 
 // A wave's work: a key head of a sequence, or a part of its keys. With chunk = 0 every sequence has
-// nsplit equal parts, and part p of row b lies at p * n_query + b. Otherwise a part is `chunk` keys, so that
-// long sequences have more of them, and the parts are numbered like tiles of `chunk` rows.
+// nsplit equal parts, and part p of row b lies at p * n_query + b. Otherwise a part is `chunk` keys. Every
+// sequence's first part is the wave of its number; the others are found by search, and few: part k > 0 of a
+// sequence that starts at s is the extra e = floor(s / chunk) + k, whose first possible key e * chunk lies
+// in that sequence and in no other.
 struct PoolItem {
   Seg sk;
   int kvh, beg, end;
   int64_t part;  // times heads: the row of the partial results
+  bool whole;    // all of the sequence's keys: no partial results
 };
-__device__ __host__ inline int64_t pool_tiles(int64_t B, int64_t nk, int chunk) { return nk / chunk + B + 2; }
-__device__ inline int64_t pool_items(const Args& a) {
-  return (a.chunk ? pool_tiles(a.B, a.nk, a.chunk) : (int64_t)a.B * a.nsplit) * a.Hkv;
+__device__ __host__ inline int64_t pool_items(int64_t B, int64_t Hkv, int64_t nk, int nsplit, int chunk) {
+  return (chunk ? nk / chunk + 1 + B : B * nsplit) * Hkv;
 }
 __device__ inline PoolItem pool_item(const Args& a, int64_t item, int step) {
   PoolItem w;
   w.kvh = (int)(item % a.Hkv);
   item /= a.Hkv;
   if (a.chunk) {
-    int local;
-    w.sk = find_tile(a.ksp, kSplits, a.B, a.nk, 1, a.chunk, (int)item, &local);
-    const int64_t beg = (int64_t)local * a.chunk;
-    if (local > 0 && beg >= w.sk.n) w.sk.b = -1;  // (a tile that the rule leaves free)
+    const int extras = a.nk / a.chunk + 1;
+    int b = (int)(item - extras), k = 0;
+    if (b < 0) {  // (the long sequences' later parts first)
+      const int64_t at = item * a.chunk;
+      int lo = 0, len = a.B;
+      const int lane = threadIdx.x & 63;
+      while (len > 1) {
+        const int step64 = (len + 63) / 64, i = lo + lane * step64;
+        const uint64_t found = __ballot(i < lo + len && split_at(a.ksp, i, a.nk) <= at);
+        const int last = found ? 63 - __builtin_clzll(found) : 0;
+        len = min(step64, len - last * step64);
+        lo += last * step64;
+      }
+      b = __builtin_amdgcn_readfirstlane(lo);
+      k = (int)item - split_at(a.ksp, b, a.nk) / a.chunk;
+      if (k < 1 || a.B == 0) b = -1;
+    }
+    w.sk = {0, 0, -1};
+    if (b >= 0) w.sk = segment(a.ksp, kSplits, b, a.nk);
+    const int64_t beg = (int64_t)k * a.chunk;
+    if (k > 0 && beg >= w.sk.n) w.sk.b = -1;
     w.beg = (int)min(beg, (int64_t)w.sk.n);
     w.end = (int)min(beg + a.chunk, (int64_t)w.sk.n);
-    w.part = item;
+    w.part = pool_part(w.sk.lo, a.chunk) + k;
+    w.whole = w.sk.n <= a.chunk;
   } else {
     const int split = (int)(item % a.nsplit), b = (int)(item / a.nsplit);
     w.sk = segment(a.ksp, kSplits, b, a.nk);
     split_range(w.sk.n, a.nsplit, split, step, &w.beg, &w.end);
     w.part = (int64_t)split * a.nq + b;
+    w.whole = !a.part;
   }
   return w;
 }
@@ -742,7 +769,7 @@ __global__ __launch_bounds__(256) void k_pool_fwd(Args a) {
   constexpr int E = 16 / sizeof(T), LPR = DP / E, R = 64 / LPR, U = sizeof(T) == 4 ? 4 : 2;
   const int lane = threadIdx.x & 63;
   const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (item >= pool_items(a)) return;
+  if (item >= pool_items(a.B, a.Hkv, a.nk, a.nsplit, a.chunk)) return;
   const PoolItem w = pool_item(a, item, R);
   if (w.sk.b < 0) return;
   const int kvh = w.kvh, b = w.sk.b, beg = w.beg, end = w.end;
@@ -816,7 +843,7 @@ __global__ __launch_bounds__(256) void k_pool_fwd(Args a) {
     const float inv = lt == 0.f ? 0.f : 1.f / lt;
     const float lse = lt == 0.f ? neg_inf() : fmaf(mx, a.scale2, __log2f(lt));
     const int64_t row = (int64_t)b * a.H + kvh * a.G + g;
-    if (a.part) {
+    if (!w.whole) {
       const int64_t at = (a.chunk ? 0 : (int64_t)a.slot0 * a.nq * a.H) + w.part * a.H + kvh * a.G + g;
       if (lane == 0) a.part_lse[at] = lse;
       acc[g].store(a.part + at * a.D, e0, a.D, a.vec_o, inv);
@@ -842,7 +869,7 @@ __global__ __launch_bounds__(256) void k_pool_bwd(Args a) {
   constexpr int E = 16 / sizeof(T), LPR = DP / E, R = 64 / LPR, U = 2;
   const int lane = threadIdx.x & 63;
   const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t items = pool_items(a);
+  const int64_t items = pool_items(a.B, a.Hkv, a.nk, a.nsplit, a.chunk);
   const int sub = lane / LPR, e0 = lane % LPR * E;
   Chunk<T> zero;
   zero.clear();
@@ -931,7 +958,7 @@ __global__ __launch_bounds__(256) void k_pool_bwd(Args a) {
     for (int i = 0; i < E; ++i) dq[g].x[i] = over_lanes<LPR, 64, Sum>(dq[g].x[i]);
     if (sub) continue;
     const int64_t row = (int64_t)b * a.H + kvh * a.G + g;
-    if (a.part) {
+    if (!w.whole) {
       dq[g].store(a.part + (w.part * a.H + kvh * a.G + g) * a.D, e0, a.D, a.vec_o, 1.f);
     } else {
       dq[g].store((T*)a.dq + row * a.D, e0, a.D, a.vec_o, 1.f);
@@ -1016,14 +1043,13 @@ struct Plan {
   int64_t tiles;
   int nsplit;
   int chunk;  // pool: keys of a wave where long sequences are cut
-  int64_t part_rows(int64_t rows, int64_t heads) const { return chunk ? tiles * heads : nsplit > 1 ? nsplit * rows : 0; }
+  int64_t slots;  // chunk > 0: partial results per head
+  int64_t part_rows(int64_t rows, int64_t heads) const { return chunk ? slots * heads : nsplit > 1 ? nsplit * rows : 0; }
   bool parted() const { return chunk || nsplit > 1; }
 };
 Plan plan_tiles(int dtype, int D, int mode, int64_t B, int64_t n, int64_t G, int64_t heads,
                 double stream_rows) {
-  Plan pl;
-  pl.pool = false;
-  pl.chunk = 0;
+  Plan pl{};
   const double per = mode == kWhole ? (double)n * G : (double)n * G / std::max<int64_t>(1, B);
   pl.sh = shape_for(dtype, D, per);
   pl.tiles = tiles_for(mode, B, n, G, pl.sh.bm);
@@ -1033,9 +1059,12 @@ Plan plan_tiles(int dtype, int D, int mode, int64_t B, int64_t n, int64_t G, int
 double average(int64_t n, int64_t B) { return (double)n / std::max<int64_t>(1, B); }
 
 // One query per sequence: a wave per sequence and key head while a few heads share the keys; a group of
-// more than 4 heads fills enough of a matrix tile. Too few waves for the card's 4096 at a time: long
-// sequences are cut, into `chunk` keys (the 7 histories of pool_lifelong are of 9411 to 120000 keys: equal
-// numbers of parts left the longest alone at the end) or, behind a prefix, into equal parts.
+// more than 4 heads fills enough of a matrix tile. How the lengths differ the host does not know, so
+// sequences are cut into `chunk` keys, and whole ones cost no more than a look by the join: 1024, or what
+// fills the card's 4096 waves where few sequences are long on average (equal numbers of parts left the
+// longest of pool_lifelong's 7 histories of 9411 to 120000 keys alone at the end, 36 us for 28). One history
+// of 100000 keys among 16384 of 40: 84 us and 97 for the gradient, 2993 and 5467 if one wave walks it; where
+// there is none the look costs 4 us each way. No more keys than one chunk in all: nothing to cut. Behind a prefix, whose parts are joined in any case: equal parts.
 bool is_pool(const mono_attention_args* p) { return !p->query_splits && p->heads / p->kv_heads <= 4; }
 Plan plan_pool(const mono_attention_args* p, bool equal) {
   Plan pl{};
@@ -1043,13 +1072,15 @@ Plan plan_pool(const mono_attention_args* p, bool equal) {
   pl.nsplit = 1;
   const int64_t waves = std::max<int64_t>(1, p->batch * p->kv_heads), want = 256 * 16;
   const int64_t by_len = (int64_t)(average(p->n_key, p->batch) / 128);
-  if (waves >= want || by_len < 2) return pl;
   if (equal) {
-    pl.nsplit = (int)std::min<int64_t>(std::min<int64_t>(want / waves, by_len), 256);
+    if (waves < want && by_len >= 2) pl.nsplit = (int)std::min<int64_t>(std::min<int64_t>(want / waves, by_len), 256);
     return pl;
   }
-  pl.chunk = (int)((std::max<int64_t>(128, p->n_key * p->kv_heads / want) + 63) / 64 * 64);
-  pl.tiles = pool_tiles(p->batch, p->n_key, pl.chunk);
+  const int64_t chunk = waves >= want || by_len < 2
+                            ? 1024 : (std::max<int64_t>(128, p->n_key * p->kv_heads / want) + 63) / 64 * 64;
+  if (p->n_key <= chunk) return pl;
+  pl.chunk = (int)chunk;
+  pl.slots = pool_part(p->n_key, pl.chunk) + 1;
   return pl;
 }
 Plan plan_fwd(const mono_attention_args* p, bool behind_prefix = false) {
@@ -1075,7 +1106,7 @@ int launch1(const Args& a, const Plan& pl, hipStream_t st) {
 // the pooled kernels; backward: 64 more workgroups for the rows of no sequence
 template <int W, typename T, int DP, int GT>
 int launch_pool2(const Args& a, hipStream_t st) {
-  const int64_t wgs = ((a.chunk ? pool_tiles(a.B, a.nk, a.chunk) : (int64_t)a.B * a.nsplit) * a.Hkv + 3) / 4;
+  const int64_t wgs = (pool_items(a.B, a.Hkv, a.nk, a.nsplit, a.chunk) + 3) / 4;
   MONO_REQUIRE(wgs < (1LL << 24) - 64, "attention: too many sequences");
   if (W == kFwd) k_pool_fwd<T, DP, GT><<<(unsigned)wgs, 256, 0, st>>>(a);
   else k_pool_bwd<T, DP, GT><<<(unsigned)wgs + 64, 256, 0, st>>>(a);
@@ -1138,7 +1169,7 @@ int join(const mono_attention_args* p, const float* part, const float* part_lse,
   const int64_t rows = p->n_query * p->heads;
   if (rows == 0) return 0;
   const int vec = p->dim % 4 == 0 && (((uintptr_t)p->out | (uintptr_t)p->out_rest) & 15) == 0;
-  const bool many = chunk || n_part >= 16;
+  const bool many = (chunk && rows <= 4096) || n_part >= 16;
   const unsigned grid = many ? (unsigned)rows : (unsigned)grid_for(rows * ((p->dim + 3) / 4), 256, 1 << 20);
   const Parts parts = parts_of(p, n_part, rows, chunk);
   const auto go = [&](auto* out) {

@@ -102,6 +102,11 @@ def test_one_long_history_among_short_ones(dtype):
   run_both(rng, dtype, 2, 1, 16, None, lens, mask=0.2, pad=(3, 70))
   run_both(rng, dtype, 3, 1, 8, None, lens, shared=True)
   run_both(rng, dtype, 5, 1, 8, None, [1, 0, 9000, 3])
+  # the card full of short sequences, and some that are cut; batches around one part
+  many = list(rng.integers(0, 4, 4500)) + [2048, 2049, 0, 4096, 4097, 9001] + list(rng.integers(0, 3, 300))
+  run_both(rng, dtype, 1, 1, 4, None, many, mask=0.1)
+  for lens in ([1024], [1025], [1023, 0, 1], [600, 600], [1024, 1, 1024], [0, 2049, 2560, 3], [127, 385]):
+    run_both(rng, dtype, 2, 2, 8, None, lens, shared=True)
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
@@ -230,7 +235,7 @@ def test_two_dimensional_rows_are_one_head():
   assert k.grad.shape == k.shape
 
 
-@pytest.mark.parametrize("nq,B,nk", [(0, 0, 0), (0, 3, 0), (3, 3, 0), (0, 1, 7)])
+@pytest.mark.parametrize("nq,B,nk", [(0, 0, 0), (0, 3, 0), (3, 3, 0), (0, 1, 7), (0, 0, 2000)])
 def test_nothing_to_do(nq, B, nk):
   from monolith_amd import attention_ops
   q = torch.randn(nq, 2, 16, device=dev(), requires_grad=True)
