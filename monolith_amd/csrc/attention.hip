@@ -184,16 +184,16 @@ __global__ __launch_bounds__(NW * 64, DP * sizeof(T) <= 256 ? 2 : 1) void k_attn
   St stk, stv;
   uint8_t mk = 0;
   auto fetch = [&](int y0) {
-    const auto alive = [&](int row) { return mb[row] != 0; };
-    stk.load(kr, y0, kend, tid, mb, alive);
-    stv.load(vr, y0, kend, tid, mb, alive);
+    const auto word = [&](int row) { return (uint32_t)mb[row]; };
+    stk.load(kr, y0, kend, tid, mb, word);
+    stv.load(vr, y0, kend, tid, mb, word);
     if (mb && tid < BN) mk = y0 + tid < kend ? mb[y0 + tid] : 0;
   };
   if (kbeg < kend) fetch(kbeg);
   for (int y0 = kbeg; y0 < kend; y0 += BN) {
     __syncthreads();
-    stk.store(lk, tid, mb);
-    stv.store(lv, tid, mb);
+    stk.store(lk, tid, mb, 0);
+    stv.store(lv, tid, mb, 0);
     if (mb && tid < BN) lm[tid] = mk;
     __syncthreads();
     if (y0 + BN < kend) fetch(y0 + BN);
@@ -462,16 +462,16 @@ __global__ __launch_bounds__(NW * 64, DP <= 64 || (sizeof(T) == 2 && NW > 1) ? 2
   St stk, stv;
   uint8_t mk = 0;
   auto fetch = [&](int y0) {
-    const auto alive = [&](int row) { return mb[row] != 0; };
-    stk.load(kr, y0, kend, tid, mb, alive);
-    stv.load(vr, y0, kend, tid, mb, alive);
+    const auto word = [&](int row) { return (uint32_t)mb[row]; };
+    stk.load(kr, y0, kend, tid, mb, word);
+    stv.load(vr, y0, kend, tid, mb, word);
     if (mb && tid < BN) mk = y0 + tid < kend ? mb[y0 + tid] : 0;
   };
   if (kbeg < kend) fetch(kbeg);
   for (int y0 = kbeg; y0 < kend; y0 += BN) {
     __syncthreads();
-    stk.store(lk, tid, mb);
-    stv.store(lv, tid, mb);
+    stk.store(lk, tid, mb, 0);
+    stv.store(lv, tid, mb, 0);
     if (mb && tid < BN) lm[tid] = mk;
     __syncthreads();
     if (y0 + BN < kend) fetch(y0 + BN);
@@ -561,33 +561,31 @@ __global__ __launch_bounds__(NW * 64, DP * sizeof(T) <= 128 ? 2 : 1) void k_attn
   float el = 0.f, ed = 0.f;
   const float inv_scale2 = 1.f / a.scale2;
   auto fetch = [&](int64_t it) {
-    const auto all = [](int) { return true; };
+    const auto all = [](int) { return 1u; };
     const int head = kvh * a.G + (int)(it / nt), y0 = (int)(tfirst + it % nt) * BN;
     const Rows<T> qr = {(const T*)a.q + (int64_t)sq.lo * a.qs + (int64_t)head * a.qh, a.qs, a.D, a.vec_q != 0};
     const Rows<T> gr = {(const T*)a.go + (int64_t)sq.lo * a.gs + (int64_t)head * a.gh, a.gs, a.D, a.vec_g != 0};
     stq.load(qr, y0, sq.n, tid, false, all);
     stg.load(gr, y0, sq.n, tid, false, all);
     if (tid < BN) {
-      el = __builtin_inff();
+      el = neg_inf();
       ed = 0.f;
       if (y0 + tid < sq.n) {
         const int64_t row = (int64_t)(sq.lo + y0 + tid) * a.H + head;
-        const float e = a.lse[row];
-        if (e != neg_inf()) {
-          el = e;
-          ed = a.delta[row];
-        }
+        el = a.lse[row];
+        ed = a.delta[row];
       }
     }
   };
   if (ibeg < iend) fetch(ibeg);
   for (int64_t it = ibeg; it < iend; ++it) {
     __syncthreads();
-    stq.store(lq, tid, false);
-    stg.store(lg, tid, false);
-    if (tid < BN) {
-      ll[tid] = -el * inv_scale2;
-      ld[tid] = -ed;
+    stq.store(lq, tid, false, 0);
+    stg.store(lg, tid, false, 0);
+    if (tid < BN) {  // a query without keys, and none: every weight is 0
+      const bool empty = el == neg_inf();
+      ll[tid] = empty ? neg_inf() : -el * inv_scale2;
+      ld[tid] = empty ? 0.f : -ed;
     }
     __syncthreads();
     const int y0 = (int)(tfirst + it % nt) * BN;

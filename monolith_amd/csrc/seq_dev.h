@@ -122,9 +122,9 @@ __device__ inline void split3(const float* x, int n, bf16* hi, bf16* mid, bf16* 
 }
 
 // A tile of BN rows on its way from global memory to LDS: load() takes the thread's chunks into
-// registers, store() writes them, one plane of bf16 behind the other. Rows outside [0, n) and rows that
-// are not alive(row) become zeros, so that nothing that lies in such a row reaches a product; what
-// alive() reads is read beside the row and needed only by store().
+// registers, store() writes them, one plane of bf16 behind the other. Rows outside [0, n) and rows whose
+// word(row) is `dead` become zeros, so that nothing that lies in such a row reaches a product. word() is a
+// plain load that nothing but store() looks at: a comparison in load() would wait for the rows there.
 template <typename T, int DP, int BN, int NT>
 struct Stage {
   static constexpr int E = 16 / sizeof(T);   // elements of a chunk
@@ -136,17 +136,17 @@ struct Stage {
   static constexpr int PLANE = BN * LDW + (DP < 32 ? 16 : 0), LDS = kPlanes<T> * PLANE;
   static_assert(NT % CH == 0 && (PER == 1 || BN * CH % NT == 0), "every thread holds one column of chunks");
   u4 r[PER];
-  bool live[PER];
+  uint32_t words[PER];
 
-  template <typename Alive>
-  __device__ inline void load(const Rows<T>& x, int row0, int n, int tid, bool filter, Alive alive) {
+  template <typename Word>
+  __device__ inline void load(const Rows<T>& x, int row0, int n, int tid, bool filter, Word word) {
     const int row = row0 + tid / CH, e0 = tid % CH * E;
     const bool mine = (PER > 1 || tid < BN * CH) && e0 < x.D;
     const T* p = x.base + (int64_t)row * x.stride + e0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       r[i] = u4{0u, 0u, 0u, 0u};
-      live[i] = true;
+      words[i] = 0;  // (such a row is zeros already)
     }
     if (x.vec && row0 + BN <= n) {
       if (mine)
@@ -164,14 +164,14 @@ struct Stage {
     if (filter)
 #pragma unroll
       for (int i = 0; i < PER; ++i)
-        if (mine && row + i * STEP < n) live[i] = alive(row + i * STEP);
+        if (mine && row + i * STEP < n) words[i] = word(row + i * STEP);
   }
-  __device__ inline void store(bf16* lds, int tid, bool filter) const {
+  __device__ inline void store(bf16* lds, int tid, bool filter, uint32_t dead) const {
     if (PER > 1 || tid < BN * CH) {
       bf16* p = lds + tid / CH * LDW + tid % CH * E;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const u4 w = !filter || live[i] ? r[i] : u4{0u, 0u, 0u, 0u};
+        const u4 w = filter && words[i] == dead ? u4{0u, 0u, 0u, 0u} : r[i];
         bf16* to = p + i * STEP * LDW;
         if constexpr (sizeof(T) == 2) {
           *(u4*)to = w;

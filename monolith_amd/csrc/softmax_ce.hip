@@ -32,10 +32,7 @@ struct Tile {
   static constexpr int BN = DP * sizeof(T) <= 256 ? 64 : 32, NR = BN / 32;
 };
 
-// what the products of a candidate start from: its bias in units of scale
-__device__ inline float start_of(const float* bias, int v, float inv_scale) {
-  return bias ? bias[v] * inv_scale : 0.f;
-}
+constexpr uint32_t kMinusInf = 0xff800000u, kPlusInf = 0x7f800000u;
 __device__ inline void range_of(int n, int nsplit, int split, int BN, int* beg, int* end) {
   const int chunk = ((n + nsplit - 1) / nsplit + BN - 1) / BN * BN;
   *beg = (int)min((int64_t)n, (int64_t)split * chunk);
@@ -74,14 +71,17 @@ __global__ __launch_bounds__(256, DP <= 128 || sizeof(T) == 2 ? 2 : 1) void k_ce
   const float inv_scale = 1.f / a.scale;
   const Rows<T> wr = {(const T*)a.w, a.ws, a.D, a.vec_w != 0};
   auto fetch = [&](int y0) {
-    st.load(wr, y0, vend, tid, a.bias, [&](int row) { return a.bias[row] != neg_inf(); });
-    if (tid < BN) eb = y0 + tid < vend ? start_of(a.bias, y0 + tid, inv_scale) : neg_inf();
+    st.load(wr, y0, vend, tid, a.bias, [&](int row) { return __float_as_uint(a.bias[row]); });
+    if (tid < BN) {
+      eb = y0 + tid < vend ? 0.f : neg_inf();
+      if (a.bias && y0 + tid < vend) eb = a.bias[y0 + tid];
+    }
   };
   if (vbeg < vend) fetch(vbeg);
   for (int y0 = vbeg; y0 < vend; y0 += BN) {
     __syncthreads();
-    st.store(lw, tid, a.bias);
-    if (tid < BN) lb[tid] = eb;
+    st.store(lw, tid, a.bias, kMinusInf);
+    if (tid < BN) lb[tid] = eb * inv_scale;  // what a candidate's products start from, in units of scale
     __syncthreads();
     if (y0 + BN < vend) fetch(y0 + BN);
     f16v s[NR][NC];
@@ -196,14 +196,17 @@ __device__ inline void query_half(const Args& a, int tile, int piece, bf16* lw, 
   const float inv_scale = 1.f / a.scale;
   const Rows<T> wr = {(const T*)a.w, a.ws, a.D, a.vec_w != 0};
   auto fetch = [&](int y0) {
-    st.load(wr, y0, vend, tid, a.bias, [&](int row) { return a.bias[row] != neg_inf(); });
-    if (tid < BN) eb = y0 + tid < vend ? start_of(a.bias, y0 + tid, inv_scale) : neg_inf();
+    st.load(wr, y0, vend, tid, a.bias, [&](int row) { return __float_as_uint(a.bias[row]); });
+    if (tid < BN) {
+      eb = y0 + tid < vend ? 0.f : neg_inf();
+      if (a.bias && y0 + tid < vend) eb = a.bias[y0 + tid];
+    }
   };
   if (vbeg < vend) fetch(vbeg);
   for (int y0 = vbeg; y0 < vend; y0 += BN) {
     __syncthreads();
-    st.store(lw, tid, a.bias);
-    if (tid < BN) lb[tid] = eb;
+    st.store(lw, tid, a.bias, kMinusInf);
+    if (tid < BN) lb[tid] = eb * inv_scale;  // what a candidate's products start from, in units of scale
     __syncthreads();
     if (y0 + BN < vend) fetch(y0 + BN);
 #pragma unroll
@@ -269,28 +272,25 @@ __device__ inline void rows_half(const Args& a, int tile, int piece, bf16* lq, f
   float el = 0.f, eg = 0.f;
   int lb = -1;
   auto fetch = [&](int y0) {
-    st.load(qr, y0, nend, tid, true, [&](int row) { return a.lse[row] != __builtin_inff(); });
+    st.load(qr, y0, nend, tid, true, [&](int row) { return __float_as_uint(a.lse[row]); });
     if (tid < BN) {
       el = __builtin_inff();
-      eg = 0.f;
-      lb = -1;
       if (y0 + tid < nend) {
         el = a.lse[y0 + tid];
-        if (el != __builtin_inff()) {
-          eg = a.grad[y0 + tid];
-          lb = (int)a.labels[y0 + tid];
-        }
+        eg = a.grad[y0 + tid];
+        lb = (int)a.labels[y0 + tid];
       }
     }
   };
   if (nbeg < nend) fetch(nbeg);
   for (int y0 = nbeg; y0 < nend; y0 += BN) {
     __syncthreads();
-    st.store(lq, tid, true);
+    st.store(lq, tid, true, kPlusInf);
     if (tid < BN) {
+      const bool live = el != __builtin_inff();
       ll[tid] = -el * inv_scale2;
-      lg[tid] = eg;
-      lab[tid] = lb;
+      lg[tid] = live ? eg : 0.f;
+      lab[tid] = live ? lb : -1;
     }
     __syncthreads();
     if (y0 + BN < nend) fetch(y0 + BN);
