@@ -113,9 +113,9 @@ __device__ inline void hide(f16v& s, int lim, const uint8_t* alive, float v, int
 // the vector unit's exponential, multiply-add, maximum and sum per logit beside 4 dim / 1024 matrix
 // instructions, and by the clock that the card keeps under such a load. Dense bf16 rows, 2048 keys, 64
 // elements: 610 TFLOP/s, 128 elements 800 (a library matrix product of 8192: 1133); fp32 183 (151). Ragged
-// causal rows (seq_train, 58602 rows of 8 x 64, 112 to 2048 a sequence): 193 us, 330 TFLOP/s: some five
+// causal rows (seq_train, 58602 rows of 8 x 64, 112 to 2048 a sequence): 189 us, 337 TFLOP/s: some five
 // tiles a workgroup, two of them on the diagonal, and four memory latencies before the first. (Sorting the
-// tiles by their work changed nothing: 193 us.)
+// tiles by their work changed nothing.)
 template <typename T, int DP, int NC, int NW>
 __global__ __launch_bounds__(NW * 64, DP * sizeof(T) <= 256 ? 2 : 1) void k_attn_fwd(Args a) {
   constexpr int BM = NC * NW * 32, BN = Tile<T, DP, NW, true>::BN, NR = Tile<T, DP, NW, true>::NR, NT = NW * 64;
@@ -381,7 +381,7 @@ __global__ __launch_bounds__(1024) void k_attn_join_many(const float* part, cons
 // ---- backward ------------------------------------------------------------------------------
 // dQ, then dK and dV: two passes that each make the logits again, 7 products instead of the 5 of one pass
 // that adds dQ up with atomics, but every sum has one order and the result is the same from call to call.
-// seq_train: 240 + 290 us, 420 TFLOP/s of executed products; 2048 keys without a mask: 660.
+// seq_train: 231 + 268 us, 450 TFLOP/s of executed products; 2048 keys without a mask: 660.
 //
 // dQ: the forward's tiles again. With p = exp2(s - lse) from the forward's statistics and
 // delta = g.o, ds = p (g.v - delta), dq = scale sum ds k. Also writes delta for the pass over keys. A bf16
