@@ -522,7 +522,9 @@ typedef struct {
   const float* bias;             /* [vocab], may be NULL */
   float scale;                   /* 1e-20 .. 1e20 */
   float* loss;                   /* [n] */
-  float* lse;                    /* [n], in units of log 2; +inf: the row has no gradient */
+  /* [2 n], of the forward, for the gradient: the log-sums in units of log 2 (+inf: the row has no gradient),
+   * behind them 1 - p of the labels */
+  float* lse;
   const float* grad_loss;        /* backward: [n] */
   void *grad_query, *grad_rows;  /* contiguous, may each be NULL */
   float* grad_bias;              /* [vocab], may be NULL */

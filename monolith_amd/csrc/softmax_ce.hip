@@ -40,20 +40,25 @@ __device__ inline void range_of(int n, int nsplit, int split, int BN, int* beg, 
 }
 
 // ---- forward: running maximum and sum of a tile of queries over one piece of the vocabulary ----
-// loss_i = log sum_v exp(l_iv) - l_i,label. A tile of 128 or (bf16 rows of 64 elements or less: two column
+// loss_i = log(1 + x_i), x_i = sum over v other than the label of exp(l_iv - l_i,label), and 1 - p_label =
+// x / (1 + x): the label is left out of the sum where its tile comes by, so that loss and gradient of a likely label
+// are made from the others' small sum and not as the difference of two numbers near each other. (1000 candidates of
+// 64 elements, p_label 0.984: dquery rows 1.6e-3 off in the median for bf16 and 4.5e-7 for fp32, the loss 4e-7; with
+// p - 1 from the stored log-sum and the label's row taken off a sum of rounded weights 5e-2, 4e-5 and 6e-5.)
+// A tile of 128 or (bf16 rows of 64 elements or less: two column
 // tiles a wave, half the LDS reads of a product) 256 queries stays in registers, the candidates stream.
 // Bound by the vector unit: an exponential, a multiply-add, a sum and half a maximum for each logit.
 // 4096 queries against 1000003 rows of 64 bf16: 740 us, 5.5e12 logits a second; 8192 against 16385 rows of
 // 64 floats: 109 us.
 template <typename T, int DP, int NC>
-__global__ __launch_bounds__(256, DP <= 128 || sizeof(T) == 2 ? 2 : 1) void k_ce_fwd(Args a) {
+__global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 || sizeof(T) == 2 ? 2 : 1) void k_ce_fwd(Args a) {
   constexpr int BM = NC * 128, BN = Tile<T, DP>::BN, NR = Tile<T, DP>::NR;
   typedef Stage<T, DP, BN, 256> St;
   typedef Mma<T, DP, St::PLANE> M;
   __shared__ __align__(16) bf16 lw[St::LDS];
   __shared__ __align__(16) float lb[BN];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int col[NC];
+  int col[NC], label[NC];
   typename M::Frag qf[NC][M::KF];
   float m[NC], l[NC];
 #pragma unroll
@@ -63,6 +68,8 @@ __global__ __launch_bounds__(256, DP <= 128 || sizeof(T) == 2 ? 2 : 1) void k_ce
     M::load_cols(qf[c], (const T*)a.q + (int64_t)(ok ? col[c] : 0) * a.qs, ok, a.D, a.vec_q, lane);
     m[c] = neg_inf();
     l[c] = 0.f;
+    const int64_t known = ok ? a.labels[col[c]] : -1;
+    label[c] = known >= 0 && known < a.v ? (int)known : -1;
   }
   int vbeg, vend;
   range_of(a.v, a.nsplit, blockIdx.y, BN, &vbeg, &vend);
@@ -84,11 +91,24 @@ __global__ __launch_bounds__(256, DP <= 128 || sizeof(T) == 2 ? 2 : 1) void k_ce
     if (tid < BN) lb[tid] = eb * inv_scale;  // what a candidate's products start from, in units of scale
     __syncthreads();
     if (y0 + BN < vend) fetch(y0 + BN);
+    bool mine = false;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) mine |= label[c] >= y0 && label[c] < y0 + BN;
+    const bool hits = __any(mine);
     f16v s[NR][NC];
 #pragma unroll
     for (int rt = 0; rt < NR; ++rt) {
       if (a.bias || y0 + BN > vend) M::template scores<NC>(lw, rt, qf, s[rt], by_rows(lb + 32 * rt, lane), lane);
       else M::template scores<NC>(lw, rt, qf, s[rt], all_of(0.f), lane);
+      if (hits) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const int at = label[c] - y0 - 32 * rt - 4 * (lane >> 5);
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (at == 8 * (r >> 2) + (r & 3)) s[rt][c][r] = neg_inf();
+        }
+      }
     }
     // every lane keeps the maximum and sum of the candidates that it holds itself; the two lanes
     // of a query are joined once, behind the loop. m is in units of scale (scale > 0).
@@ -120,7 +140,8 @@ __global__ __launch_bounds__(256, DP <= 128 || sizeof(T) == 2 ? 2 : 1) void k_ce
   }
 }
 
-// One wave per query: joins the pieces of the vocabulary and takes the label's own logit off.
+// One wave per query: joins the pieces of the vocabulary and the label, whose logit it makes. In units of log 2
+// the others' sum is base + log2 z and the label's logit base + d.
 template <typename T>
 __global__ __launch_bounds__(256) void k_ce_loss(Args a) {
   const int lane = threadIdx.x & 63;
@@ -130,10 +151,12 @@ __global__ __launch_bounds__(256) void k_ce_loss(Args a) {
   for (int s = lane; s < a.nsplit; s += 64) m = fmaxf(m, a.part[(int64_t)s * a.n + i]);
 #pragma unroll
   for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
-  const float base = m == neg_inf() ? 0.f : m;
+  float base = m == neg_inf() ? 0.f : m;
   float z = 0.f;
   for (int s = lane; s < a.nsplit; s += 64)
     z += a.part2[(int64_t)s * a.n + i] * exp2_hw(a.part[(int64_t)s * a.n + i] - base);
+#pragma unroll
+  for (int x = 32; x; x >>= 1) z += __shfl_xor(z, x);
   const int64_t label = a.labels[i];
   const bool known = label >= 0 && label < a.v;
   float hit = 0.f;
@@ -141,32 +164,41 @@ __global__ __launch_bounds__(256) void k_ce_loss(Args a) {
     for (int d = lane; d < a.D; d += 64)
       hit = fmaf((float)((const T*)a.q)[i * a.qs + d], (float)((const T*)a.w)[label * a.ws + d], hit);
 #pragma unroll
-  for (int x = 32; x; x >>= 1) {
-    z += __shfl_xor(z, x);
-    hit += __shfl_xor(hit, x);
-  }
+  for (int x = 32; x; x >>= 1) hit += __shfl_xor(hit, x);
   if (lane) return;
   const float b = known && a.bias ? a.bias[label] : 0.f;
-  const bool out = b == neg_inf();
-  const float lse = m + __log2f(z);
-  float loss = fmaf(lse, kLn2, -fmaf(hit, a.scale, b));
-  if (out) loss = __builtin_inff();
-  if (!known) loss = label == -1 ? 0.f : __builtin_nanf("");
+  float loss = label == -1 ? 0.f : __builtin_nanf(""), lse = __builtin_inff(), miss = 0.f;
+  if (b == neg_inf()) {
+    loss = __builtin_inff();
+  } else if (known) {
+    hit = fmaf(hit, a.scale2, b * kLog2e);
+    if (m == neg_inf()) base = hit;  // (there are no others)
+    const float d = hit - base, x = z * exp2_hw(-d);
+    if (d > -64.f) {
+      loss = log1pf(x);
+      miss = x / (1.f + x);
+    } else {  // (the 1 is less than a rounding of x, which may be beyond the largest number)
+      loss = (__log2f(z) - d) * kLn2;
+      miss = 1.f;
+    }
+    lse = d > 0.f ? hit + __log2f(1.f + x) : base + __log2f(z + exp2_hw(d));
+  }
   a.loss[i] = loss;
-  a.lse[i] = known && !out ? lse : __builtin_inff();
+  a.lse[i] = lse;
+  a.lse[a.n + i] = miss;
 }
 
 // ---- backward ------------------------------------------------------------------------------
-// dquery_i = scale g_i (sum_v p_iv w_v - w_label): g and the label's row are taken in behind the
-// loop, in 32 bits, so that the products see nothing but the probabilities.
+// dquery_i = scale g_i (sum over v other than the label of p_iv w_v - (1 - p_label) w_label): g and the label's row
+// are taken in behind the loop, in 32 bits, so that the products see nothing but the others' probabilities.
 template <typename T>
 __device__ inline f4 minus_label(const Args& a, int i, int d0, f4 t) {
   const float lse = a.lse[i];
   if (lse == __builtin_inff()) return f4{0.f, 0.f, 0.f, 0.f};
-  const float g = a.grad[i] * a.scale;
+  const float g = a.grad[i] * a.scale, miss = a.lse[a.n + (int64_t)i];
   const T* w = (const T*)a.w + a.labels[i] * a.ws;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) t[r] = d0 + r < a.D ? g * (t[r] - (float)w[d0 + r]) : 0.f;
+  for (int r = 0; r < 4; ++r) t[r] = d0 + r < a.D ? g * (t[r] - miss * (float)w[d0 + r]) : 0.f;
   return t;
 }
 
@@ -179,6 +211,7 @@ __device__ inline void query_half(const Args& a, int tile, int piece, bf16* lw, 
   int col[NC];
   typename M::Frag qf[NC][M::KF];
   float lse[NC];
+  int label[NC];
   f16v acc[M::NDT][NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
@@ -186,6 +219,7 @@ __device__ inline void query_half(const Args& a, int tile, int piece, bf16* lw, 
     const bool ok = col[c] < a.n;
     M::load_cols(qf[c], (const T*)a.q + (int64_t)(ok ? col[c] : 0) * a.qs, ok, a.D, a.vec_q, lane);
     lse[c] = ok ? a.lse[col[c]] : __builtin_inff();
+    label[c] = lse[c] == __builtin_inff() ? -1 : (int)a.labels[col[c]];
 #pragma unroll
     for (int d = 0; d < M::NDT; ++d) acc[d][c] = all_of(0.f);
   }
@@ -209,6 +243,10 @@ __device__ inline void query_half(const Args& a, int tile, int piece, bf16* lw, 
     if (tid < BN) lb[tid] = eb * inv_scale;  // what a candidate's products start from, in units of scale
     __syncthreads();
     if (y0 + BN < vend) fetch(y0 + BN);
+    bool mine = false;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) mine |= label[c] >= y0 && label[c] < y0 + BN;
+    const bool hits = __any(mine);
 #pragma unroll
     for (int rt = 0; rt < NR; ++rt) {
       f16v s[NC];
@@ -218,6 +256,15 @@ __device__ inline void query_half(const Args& a, int tile, int piece, bf16* lw, 
       for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[c][r] = exp2_hw(fmaf(s[c][r], a.scale2, -lse[c]));
+      if (hits) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const int at = label[c] - y0 - 32 * rt - 4 * (lane >> 5);
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (at == 8 * (r >> 2) + (r & 3)) s[c][r] = 0.f;
+        }
+      }
       M::template accumulate<NC>(lw, rt, s, acc, lane);
     }
   }
@@ -241,10 +288,10 @@ __device__ inline void query_half(const Args& a, int tile, int piece, bf16* lw, 
 }
 
 // drows_v = scale sum_i g_i (p_iv - [v = label_i]) query_i, dbias_v the same without scale and query:
-// a tile of candidates keeps its sums while all queries stream by. The label's share is rare: one
-// ballot per tile of queries says whether any label falls into the candidates of the workgroup.
+// a tile of candidates keeps its sums while all queries stream by. The label's weight is the forward's
+// 1 - p, and rare: one ballot per tile of queries says whether any label falls into the candidates of the workgroup.
 template <typename T, int DP, int NC>
-__device__ inline void rows_half(const Args& a, int tile, int piece, bf16* lq, float* ll, float* lg, int* lab) {
+__device__ inline void rows_half(const Args& a, int tile, int piece, bf16* lq, float* ll, float* lg, float* lm, int* lab) {
   constexpr int BM = NC * 128, BN = Tile<T, DP>::BN, NR = Tile<T, DP>::NR;
   typedef Stage<T, DP, BN, 256> St;
   typedef Mma<T, DP, St::PLANE> M;
@@ -269,7 +316,7 @@ __device__ inline void rows_half(const Args& a, int tile, int piece, bf16* lq, f
   St st;
   const Rows<T> qr = {(const T*)a.q, a.qs, a.D, a.vec_q != 0};
   const float inv_scale2 = 1.f / a.scale2;
-  float el = 0.f, eg = 0.f;
+  float el = 0.f, eg = 0.f, em = 0.f;
   int lb = -1;
   auto fetch = [&](int y0) {
     st.load(qr, y0, nend, tid, true, [&](int row) { return __float_as_uint(a.lse[row]); });
@@ -277,6 +324,7 @@ __device__ inline void rows_half(const Args& a, int tile, int piece, bf16* lq, f
       el = __builtin_inff();
       if (y0 + tid < nend) {
         el = a.lse[y0 + tid];
+        em = a.lse[a.n + (int64_t)(y0 + tid)];
         eg = a.grad[y0 + tid];
         lb = (int)a.labels[y0 + tid];
       }
@@ -290,6 +338,7 @@ __device__ inline void rows_half(const Args& a, int tile, int piece, bf16* lq, f
       const bool live = el != __builtin_inff();
       ll[tid] = -el * inv_scale2;
       lg[tid] = live ? eg : 0.f;
+      lm[tid] = -em;
       lab[tid] = live ? lb : -1;
     }
     __syncthreads();
@@ -307,10 +356,11 @@ __device__ inline void rows_half(const Args& a, int tile, int piece, bf16* lq, f
       if (hits) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int label = lab[32 * rt + tile_row(r, lane)];
+          const int row = 32 * rt + tile_row(r, lane), label = lab[row];
+          const float weight = lm[row];
 #pragma unroll
           for (int c = 0; c < NC; ++c)
-            if (label == col[c]) s[c][r] -= 1.f;
+            if (label == col[c]) s[c][r] = weight;
         }
       }
       const f16v g = by_rows(lg + 32 * rt, lane);
@@ -342,14 +392,14 @@ __device__ inline void rows_half(const Args& a, int tile, int piece, bf16* lq, f
 // of 8192 reaches 1.13: with operands that are not random but zeros the same loop takes half the time, so
 // it is the card's power that bounds it. 415 us for 8192 against 16385 rows of 64 floats.
 template <typename T, int DP, int NC>
-__global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void k_ce_bwd(Args a) {
+__global__ __launch_bounds__(256, DP <= 32 ? 3 : DP * sizeof(T) <= 256 ? 2 : 1) void k_ce_bwd(Args a) {
   constexpr int BN = Tile<T, DP>::BN;
   __shared__ __align__(16) bf16 rows[Stage<T, DP, BN, 256>::LDS];
-  __shared__ __align__(16) float first[BN], second[BN];
+  __shared__ __align__(16) float first[BN], second[BN], third[BN];
   __shared__ __align__(16) int labels[BN];
   const int of_queries = a.q_tiles * a.q_split, i = blockIdx.x - of_queries;
   if (i < 0) query_half<T, DP, NC>(a, blockIdx.x % a.q_tiles, blockIdx.x / a.q_tiles, rows, first);
-  else rows_half<T, DP, NC>(a, i % a.w_tiles, i / a.w_tiles, rows, first, second, labels);
+  else rows_half<T, DP, NC>(a, i % a.w_tiles, i / a.w_tiles, rows, first, second, third, labels);
 }
 
 // four elements from `at` on of the pieces' partial sums, first to last; several pieces' loads in flight

@@ -27,7 +27,7 @@ def _fields(query, rows, labels, bias, scale, loss, lse, grad_loss=0, dq=0, dw=0
 
 def _forward(query, rows, labels, bias, scale):
   loss = torch.empty(query.shape[0], dtype=torch.float32, device=query.device)
-  lse = torch.empty_like(loss)
+  lse = torch.empty(2 * query.shape[0], dtype=torch.float32, device=query.device)  # log-sums, 1 - p of the labels
   _lib.launch("mono_softmax_cross_entropy", _lib.pack_softmax_ce,
               _fields(query, rows, labels, bias, scale, loss.data_ptr(), lse), query.device)
   return loss, lse
