@@ -510,7 +510,7 @@ int mono_shared_prefix_attention(const mono_attention_args* args, void* stream);
 /* loss[i] = log sum_v exp(l[i, v]) - l[i, label_i], l = scale query rows^T + bias. A label of -1
  * marks a row without one (loss 0, no gradient), any other label outside [0, vocab) gives a loss of
  * NaN and no gradient. A bias of -inf takes a candidate out, whatever its row holds; a row whose own
- * label is taken out has a loss of +inf and no gradient. */
+ * label is taken out has a loss of +inf and no gradient. A finite bias below -1e7 counts as -1e7 in the sum. */
 typedef struct {
   int32_t dtype, dim;            /* 1 <= dim <= 256 */
   int64_t n, vocab;              /* n < 2^26 */

@@ -32,6 +32,12 @@ struct Tile {
   static constexpr int BN = DP * sizeof(T) <= 256 ? 64 : 32, NR = BN / 32;
 };
 
+// A finite bias below kFloor counts as kFloor beside other candidates: its weight is 0 either way, but on a tile of
+// nothing else the exponent's base, the rounded product of maximum and scale, would be off by more than an
+// exponential holds, and infinite for the type's lowest value.
+constexpr float kFloor = -1e7f;
+__device__ inline float floored(float bias) { return bias < kFloor && bias != neg_inf() ? kFloor : bias; }
+
 constexpr uint32_t kMinusInf = 0xff800000u, kPlusInf = 0x7f800000u;
 __device__ inline void range_of(int n, int nsplit, int split, int BN, int* beg, int* end) {
   const int chunk = ((n + nsplit - 1) / nsplit + BN - 1) / BN * BN;
@@ -88,7 +94,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 || sizeof(T) == 2 ? 2
   for (int y0 = vbeg; y0 < vend; y0 += BN) {
     __syncthreads();
     st.store(lw, tid, a.bias, kMinusInf);
-    if (tid < BN) lb[tid] = eb * inv_scale;  // what a candidate's products start from, in units of scale
+    if (tid < BN) lb[tid] = floored(eb) * inv_scale;  // what a candidate's products start from, in units of scale
     __syncthreads();
     if (y0 + BN < vend) fetch(y0 + BN);
     bool mine = false;
@@ -171,14 +177,14 @@ __global__ __launch_bounds__(256) void k_ce_loss(Args a) {
   if (b == neg_inf()) {
     loss = __builtin_inff();
   } else if (known) {
-    hit = fmaf(hit, a.scale2, b * kLog2e);
+    hit = fmaf(hit, a.scale2, floored(b) * kLog2e);
     if (m == neg_inf()) base = hit;  // (there are no others)
     const float d = hit - base, x = z * exp2_hw(-d);
     if (d > -64.f) {
       loss = log1pf(x);
       miss = x / (1.f + x);
     } else {  // (the 1 is less than a rounding of x, which may be beyond the largest number)
-      loss = (__log2f(z) - d) * kLn2;
+      loss = (__log2f(z) - d) * kLn2 + (floored(b) - b);
       miss = 1.f;
     }
     lse = d > 0.f ? hit + __log2f(1.f + x) : base + __log2f(z + exp2_hw(d));
@@ -240,7 +246,7 @@ __device__ inline void query_half(const Args& a, int tile, int piece, bf16* lw, 
   for (int y0 = vbeg; y0 < vend; y0 += BN) {
     __syncthreads();
     st.store(lw, tid, a.bias, kMinusInf);
-    if (tid < BN) lb[tid] = eb * inv_scale;  // what a candidate's products start from, in units of scale
+    if (tid < BN) lb[tid] = floored(eb) * inv_scale;  // what a candidate's products start from, in units of scale
     __syncthreads();
     if (y0 + BN < vend) fetch(y0 + BN);
     bool mine = false;
@@ -305,7 +311,7 @@ __device__ inline void rows_half(const Args& a, int tile, int piece, bf16* lq, f
   for (int c = 0; c < NC; ++c) {
     col[c] = v0 + (wave * NC + c) * 32 + (lane & 31);
     const bool ok = col[c] < a.v;
-    b2[c] = !ok ? neg_inf() : a.bias ? a.bias[col[c]] * kLog2e : 0.f;
+    b2[c] = !ok ? neg_inf() : a.bias ? floored(a.bias[col[c]]) * kLog2e : 0.f;
     M::load_cols(wf[c], (const T*)a.w + (int64_t)(ok ? col[c] : 0) * a.ws, b2[c] != neg_inf(), a.D, a.vec_w, lane);
     sb[c] = 0.f;
 #pragma unroll

@@ -73,7 +73,8 @@ def softmax_cross_entropy(query: torch.Tensor, rows: torch.Tensor, labels: torch
   query [n, dim], rows [vocab, dim]: float32 or bfloat16, dim <= 256; labels int64 [n]: a label of -1
   marks a query without one (loss 0, no gradient), any other label outside [0, vocab) gives a loss of
   NaN and no gradient. bias: float32 [vocab]; -inf takes a candidate out, whatever its row holds, and
-  a query whose own label is taken out has a loss of +inf and no gradient. scale: 1 / temperature."""
+  a query whose own label is taken out has a loss of +inf and no gradient; a finite bias below -1e7
+  counts as -1e7 beside the other candidates. scale: 1 / temperature."""
   who = "softmax_cross_entropy"
   for name, x in (("query", query), ("rows", rows)):
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
