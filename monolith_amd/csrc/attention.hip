@@ -557,6 +557,10 @@ __global__ __launch_bounds__(NW * 64, DP * sizeof(T) <= 128 ? 2 : 1) void k_attn
     ibeg = min(iend, split * chunk);
     iend = min(iend, ibeg + chunk);
   }
+  // A query without keys has weights of 0, but a product with them would still carry on what its row and its
+  // gradient hold, NaN say: rows of zeros then. There is none where the queries are no more than the keys and no
+  // key is masked.
+  const bool some_empty = a.mask || (a.causal && sq.n > sk.n);
   St stq, stg;
   float el = 0.f, ed = 0.f;
   const float inv_scale2 = 1.f / a.scale2;
@@ -589,6 +593,14 @@ __global__ __launch_bounds__(NW * 64, DP * sizeof(T) <= 128 ? 2 : 1) void k_attn
     }
     __syncthreads();
     const int y0 = (int)(tfirst + it % nt) * BN;
+    if (some_empty) {
+      const auto empty = [&](int row) { return ll[row] == neg_inf(); };
+      if (__any(y0 + (lane & (BN - 1)) < sq.n && empty(lane & (BN - 1)))) {  // (every wave finds the same)
+        St::clear(lq, tid, empty);
+        St::clear(lg, tid, empty);
+        __syncthreads();
+      }
+    }
     if (it + 1 < iend) fetch(it + 1);
     const bool need = y0 < qmax;
 #pragma unroll

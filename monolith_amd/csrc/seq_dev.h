@@ -187,6 +187,20 @@ struct Stage {
       }
     }
   }
+  // zeros in the place of a thread's chunks of the rows that are dead(row of the tile)
+  template <typename Dead>
+  static __device__ inline void clear(bf16* lds, int tid, Dead dead) {
+    if (PER > 1 || tid < BN * CH)
+      for (int i = 0; i < PER; ++i) {
+        const int row = tid / CH + i * STEP;
+        if (dead(row))
+          for (int j = 0; j < kPlanes<T>; ++j) {
+            bf16* to = lds + row * LDW + tid % CH * E + j * PLANE;
+            if constexpr (sizeof(T) == 2) *(u4*)to = u4{0u, 0u, 0u, 0u};
+            else *(uint64_t*)to = 0;
+          }
+      }
+  }
 };
 
 // The 32x32 matrix instructions: a C tile gives lane l column l & 31 and, in register r, row

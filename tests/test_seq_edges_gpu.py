@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from tests import seq_ref
-from tests.test_attention_gpu import dev, on, rows
+from tests.test_attention_gpu import dev, on, rows, splits
 
 pytestmark = [pytest.mark.gpu, pytest.mark.timeout(300)]
 LOW = [-2e7, -1e10, -1e30, float(np.finfo(np.float32).min)]
@@ -47,3 +47,42 @@ def test_biases_of_the_lowest_value(dtype, low, scale):
   want = -g[3].double() * q[3].double() * scale
   half = seq_ref.HALF[dtype]
   assert ((dw[5].double() - want).abs() <= (2 * half + half * half + 4 * seq_ref.U32) * want.abs()).all()
+
+
+# ---- queries without a key -----------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("form", ["causal", "mask", "one", "one_many_heads"])
+def test_queries_without_a_key_hold_anything(dtype, bad, form):
+  """Neither their rows nor what arrives as their gradient reaches a key's gradient."""
+  from monolith_amd import attention_ops
+  rng = np.random.default_rng(21)
+  one = form.startswith("one")
+  heads = 10 if form == "one_many_heads" else 4
+  lk = [30, 40, 90, 5]
+  lq = [1] * 4 if one else [100, 40, 130, 5]
+  q, _ = rows(rng, (sum(lq), heads, 16), dtype)
+  k, _ = rows(rng, (sum(lk), 2, 16), dtype)
+  v, _ = rows(rng, (sum(lk), 2, 16), dtype)
+  g, _ = rows(rng, (sum(lq), heads, 16), dtype)
+  mask = torch.ones(sum(lk), dtype=torch.bool, device=dev())
+  empty = np.zeros(sum(lq), bool)
+  ks, qs = splits(lk), splits(lq)
+  if form == "causal":
+    for b in range(4):
+      empty[qs[b]:qs[b] + max(0, lq[b] - lk[b])] = True
+  else:
+    mask[ks[1]:ks[2]] = False
+    empty[qs[1]:qs[2]] = True
+  assert empty.any()
+  res = []
+  for value in (0.0, bad):
+    q2, g2 = q.clone(), g.clone()
+    q2[on(empty)], g2[on(empty)] = value, value
+    leaves = [t.clone().requires_grad_() for t in (q2, k, v)]
+    out = attention_ops.ragged_attention(*leaves, on(ks), None if one else on(qs), None if form == "causal" else mask,
+                                         form == "causal")
+    res.append(grads(out, leaves, g2))
+  for a, b in zip(*res):
+    assert torch.isfinite(b.float()).all() and torch.equal(a, b)
+  assert (res[1][0][on(empty)] == 0).all() and (res[1][1][on(empty)] == 0).all()
