@@ -502,7 +502,7 @@ int mono_ragged_attention(const mono_attention_args* args, void* stream);
 /* its gradient: reads out and lse of the forward, recomputes the probabilities */
 int64_t mono_ragged_attention_gradient_workspace(const mono_attention_args* args);
 int mono_ragged_attention_gradient(const mono_attention_args* args, void* stream);
-/* Every query sees the n_prefix prefix rows, which lie in memory once for the whole batch, and the
+/* Every query of a sequence sees the n_prefix prefix rows, which lie in memory once for the whole batch, and the
  * keys of its own sequence (key_splits NULL: none). */
 int64_t mono_shared_prefix_attention_workspace(const mono_attention_args* args);
 int mono_shared_prefix_attention(const mono_attention_args* args, void* stream);

@@ -214,7 +214,8 @@ def shared_prefix_attention(query: torch.Tensor, prefix_key: torch.Tensor,
   keys of its own sequence, in one softmax. Forward only.
 
   prefix_key, prefix_value [n_prefix, kv_heads, dim]; the other arguments as in ragged_attention;
-  key=None: no keys of their own. causal concerns a sequence's own keys, which stand behind the
+  key=None: no keys of their own (with query_splits, queries outside of them see no prefix either and get
+  zeros). causal concerns a sequence's own keys, which stand behind the
   prefix; prefix_mask: bool [n_prefix]. value=None / prefix_value=None: the keys are the values."""
   who = "shared_prefix_attention"
   q = _query(query, who)

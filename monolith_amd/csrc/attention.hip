@@ -27,6 +27,7 @@ struct Args {
   const int64_t *qsp, *ksp;
   const uint8_t* mask;
   int B, nq, nk, H, Hkv, G, D, qmode, kmode, causal, shared;
+  int qbatch;                      // kWhole with query splits: their sequences; other queries see nothing
   int nsplit, slot0;
   int chunk;                       // pooled rows: keys of a wave, 0 = a split of a sequence's keys
   float scale, scale2;
@@ -138,18 +139,23 @@ __global__ __launch_bounds__(NW * 64, DP * sizeof(T) <= 256 ? 2 : 1) void k_attn
   int tok[NC], head[NC], klim[NC];
   bool ok[NC];
   typename M::Frag qf[NC][M::KF];
-  int kmin = sk.n, kmax = 0;
+  int kmin = sk.n, kmax = 0, tfirst = 0, tlast = a.nq;
+  if (a.qmode == kWhole && a.qsp) {  // (behind the shared prefix: rows of no sequence)
+    tfirst = split_at(a.qsp, 0, a.nq);
+    tlast = split_at(a.qsp, a.qbatch, a.nq);
+  }
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int64_t r = r0 + (wave * NC + c) * 32 + (lane & 31);
     ok[c] = r < nrow;
     tok[c] = ok[c] ? (int)(r / a.G) : 0;
     head[c] = kvh * a.G + (ok[c] ? (int)(r % a.G) : 0);
-    int lim = sk.n;
+    const bool sees = sq.lo + tok[c] >= tfirst && sq.lo + tok[c] < tlast;
+    int lim = sees ? sk.n : 0;
     if (a.causal) lim = min(lim, max(0, sk.n - sq.n + tok[c] + 1));
     klim[c] = ok[c] ? lim : 0;
     if (ok[c]) kmin = min(kmin, lim), kmax = max(kmax, lim);
-    M::load_cols(qf[c], (const T*)a.q + (int64_t)(sq.lo + tok[c]) * a.qs + (int64_t)head[c] * a.qh, ok[c],
+    M::load_cols(qf[c], (const T*)a.q + (int64_t)(sq.lo + tok[c]) * a.qs + (int64_t)head[c] * a.qh, ok[c] && sees,
                  a.D, a.vec_q, lane);
   }
 #pragma unroll
@@ -1333,6 +1339,7 @@ int mono_shared_prefix_attention(const mono_attention_args* p, void* stream) {
   a.mask = p->prefix_mask;
   a.nk = (int)p->n_prefix;
   a.qmode = a.kmode = kWhole;
+  a.qbatch = a.B;
   a.B = 1;
   a.causal = 0;
   a.nsplit = pl.pre.nsplit;

@@ -86,3 +86,43 @@ def test_queries_without_a_key_hold_anything(dtype, bad, form):
   for a, b in zip(*res):
     assert torch.isfinite(b.float()).all() and torch.equal(a, b)
   assert (res[1][0][on(empty)] == 0).all() and (res[1][1][on(empty)] == 0).all()
+
+
+# ---- a padded request behind a prefix ------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("prefix", [1, 70, 5000])
+@pytest.mark.parametrize("own", [None, [5, 0, 40, 3], [3000, 1, 2, 900]])
+@pytest.mark.parametrize("heads", [2, 12])
+def test_prefix_rows_of_no_sequence(dtype, prefix, own, heads):
+  """Queries in front of the first split and behind the last hold anything and get zeros; the others get what
+  they get without them."""
+  from monolith_amd import attention_ops
+  rng = np.random.default_rng(22)
+  lq = [3, 70, 1, 20]
+  qs = splits(lq, 37)
+  nq = int(qs[-1]) + 150
+  q, q64 = rows(rng, (nq, heads, 24), dtype)
+  pk, pk64 = rows(rng, (prefix, 2, 24), dtype)
+  pv, pv64 = rows(rng, (prefix, 2, 24), dtype)
+  lk = own if own is not None else [0] * 4
+  k, k64 = rows(rng, (sum(lk), 2, 24), dtype)
+  v, v64 = rows(rng, (sum(lk), 2, 24), dtype)
+  q[:37], q[int(qs[-1]):] = float("nan"), float("inf")
+  kw = {} if own is None else dict(key=k, value=v, key_splits=on(splits(lk)), causal=True)
+  out = attention_ops.shared_prefix_attention(q, pk, pv, query_splits=on(qs), **kw)
+  assert (out[:37] == 0).all() and (out[int(qs[-1]):] == 0).all()
+  ks = splits(lk)
+  segs = [(np.arange(qs[b], qs[b + 1]), np.concatenate([np.arange(prefix), prefix + np.arange(ks[b], ks[b + 1])]))
+          for b in range(4)]
+
+  def keep(c, n, m):
+    ok = np.ones((n, m), bool)
+    ok[:, prefix:] = np.arange(m - prefix)[None] <= np.arange(n)[:, None] + m - prefix - n
+    return ok
+
+  want = seq_ref.attention(q64, np.concatenate([pk64, k64]), np.concatenate([pv64, v64]), segs, keep,
+                           24 ** -0.5, dtype)["out"]
+  live = slice(37, int(qs[-1]))
+  # the parts are joined in 32 bits: one more exponential, product and sum for every part
+  seq_ref.check(out[live], (want[0][live], (want[1] * (1 + 2.0 ** -10) + 64 * seq_ref.U32 * np.abs(want[0]))[live]),
+                "out")
