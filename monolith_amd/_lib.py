@@ -7,6 +7,7 @@ import struct
 # torch must load its HIP runtime before libmonolith_hip.so pulls in libamdhip64: with the order
 # reversed both end up sharing the system copy and torch then reports "No HIP GPUs are available".
 import torch  # noqa: F401  pylint: disable=unused-import
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmonolith_hip.so")
@@ -108,6 +109,16 @@ def stream_ptr(device=None):
 pack_attention = struct.Struct("@6i3q" + 3 * "P2q" + "3Pfq" + 2 * "P2q" + "P3P" + "P2q" + "3PPq").pack
 pack_softmax_ce = struct.Struct("@2i2q" + 2 * "Pq" + "2Pf" + 2 * "P" + "PPPPPq").pack
 _raw_stream = torch._C._cuda_getCurrentRawStream  # (current_stream() builds an object on every call)
+
+
+def no_tangents(who, *tensors):
+  """The sequence operators have gradients, but no forward-mode derivative: a tangent (torch.autograd.forward_ad)
+  would be dropped, as the kernels see the primal's memory only."""
+  if getattr(forward_ad, "_current_level", 0) < 0:  # (no level is open: spares 3 us a call)
+    return
+  for x in tensors:
+    if x is not None and forward_ad.unpack_dual(x).tangent is not None:
+      raise ValueError("%s has no forward-mode derivative" % who)
 
 
 def launch(name, pack, fields, device):

@@ -11,7 +11,8 @@ no sequence: their outputs and gradients are zero. Splits that break this give w
 an access outside the tensors. Softmax statistics and sums are held in 32 bits; results have the
 rows' type and are the same bit for bit from call to call. Elements that a query sees have to be finite
 (float32 rows are multiplied as three bfloat16 numbers each; an infinite element gives NaN). Nothing synchronises the host, and
-scratch memory comes from torch's allocator, so every op can be captured into a HIP graph."""
+scratch memory comes from torch's allocator, so every op can be captured into a HIP graph. There is no
+forward-mode derivative: a tangent (torch.autograd.forward_ad) is refused."""
 import math
 from typing import Optional
 
@@ -150,6 +151,7 @@ class _RaggedAttention(torch.autograd.Function):
   def backward(ctx, grad):
     query, key, value, key_splits, query_splits, key_mask, out, lse, rest = ctx.saved_tensors
     shared = value is None
+    _lib.no_tangents("the gradient of ragged_attention", grad)
     grad = grad if grad.stride(2) == 1 and grad.dtype == query.dtype else \
         grad.to(query.dtype).contiguous()
     dq = torch.empty(query.shape, dtype=query.dtype, device=query.device)
@@ -191,6 +193,7 @@ def ragged_attention(query: torch.Tensor, key: torch.Tensor, value: Optional[tor
                                                  "query_splits", who)
   mask = _mask(key_mask, k.shape[0], q.device, "key_mask", who)
   scale = _scale(scale, q.shape[2], who)
+  _lib.no_tangents(who, q, k, v)
   _on_gpu(q, who)
   if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
     out = _RaggedAttention.apply(q, k, None if value is None else v, ks, qs, mask, bool(causal),
@@ -234,6 +237,7 @@ def shared_prefix_attention(query: torch.Tensor, prefix_key: torch.Tensor,
       query_splits, None if ks is None else ks.numel() - 1, q.device, "query_splits", who)
   if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, pk, pv, k, v)):
     raise ValueError("%s has no gradient: detach the tensors or use ragged_attention" % who)
+  _lib.no_tangents(who, q, pk, pv, k, v)
   scale = _scale(scale, q.shape[2], who)
   mask = None if k is None else _mask(key_mask, k.shape[0], q.device, "key_mask", who)
   pmask = _mask(prefix_mask, pk.shape[0], q.device, "prefix_mask", who)

@@ -6,7 +6,8 @@ the reference's op set.
 
 The logits [n, vocab] never exist in memory. Sums and statistics are held in 32 bits; results are the
 same bit for bit from call to call. Nothing synchronises the host and scratch memory comes from
-torch's allocator, so loss and gradient can be captured into a HIP graph."""
+torch's allocator, so loss and gradient can be captured into a HIP graph. There is no forward-mode
+derivative: a tangent (torch.autograd.forward_ad) is refused."""
 from typing import Optional
 
 import torch
@@ -46,6 +47,7 @@ class _SoftmaxCrossEntropy(torch.autograd.Function):
   @torch.autograd.function.once_differentiable
   def backward(ctx, grad):
     query, rows, labels, bias, lse = ctx.saved_tensors
+    _lib.no_tangents("the gradient of softmax_cross_entropy", grad)
     if grad.dtype != torch.float32 or not grad.is_contiguous():
       grad = grad.to(torch.float32).contiguous()
     dq = dw = db = None
@@ -102,6 +104,7 @@ def softmax_cross_entropy(query: torch.Tensor, rows: torch.Tensor, labels: torch
   scale = float(scale)
   if not 1e-20 <= scale <= 1e20:
     raise ValueError("%s: scale must be in [1e-20, 1e20], got %r" % (who, scale))
+  _lib.no_tangents(who, query, rows, bias)
   if not query.is_cuda:
     raise _lib.MonolithHipError("%s: tensors must live on the GPU (no CPU fallback)" % who)
   query = query if query.stride(1) == 1 else query.contiguous()

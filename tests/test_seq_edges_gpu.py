@@ -126,3 +126,21 @@ def test_prefix_rows_of_no_sequence(dtype, prefix, own, heads):
   # the parts are joined in 32 bits: one more exponential, product and sum for every part
   seq_ref.check(out[live], (want[0][live], (want[1] * (1 + 2.0 ** -10) + 64 * seq_ref.U32 * np.abs(want[0]))[live]),
                 "out")
+
+
+# ---- forward mode --------------------------------------------------------------------------------
+def test_gradients_refuse_tangents():
+  """A tangent that arrives with the output's gradient is refused as one in the inputs is."""
+  from torch.autograd import forward_ad
+  from monolith_amd import attention_ops, loss_ops
+  q = torch.randn(4, 1, 16, device=dev(), requires_grad=True)
+  k = torch.randn(9, 1, 16, device=dev())
+  calls = (lambda: attention_ops.ragged_attention(q, k, None, on(np.array([0, 2, 4, 6, 9]))),
+           lambda: loss_ops.softmax_cross_entropy(q[:, 0], k[:, 0], on(np.array([0, 3, 8, 1]))))
+  for call in calls:
+    with forward_ad.dual_level():
+      out = call()
+      weight = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+      with pytest.raises(ValueError, match="forward-mode"):
+        torch.autograd.grad((out * weight).sum(), q)
+      torch.autograd.grad(call().sum(), q)
