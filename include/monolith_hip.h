@@ -513,7 +513,7 @@ int mono_shared_prefix_attention(const mono_attention_args* args, void* stream);
  * label is taken out has a loss of +inf and no gradient. A finite bias below -1e7 counts as -1e7 in the sum. */
 typedef struct {
   int32_t dtype, dim;            /* 1 <= dim <= 256 */
-  int64_t n, vocab;              /* n < 2^26 */
+  int64_t n, vocab;              /* n < 2^26; vocab < 2^31 - 2^16, 2^31 - 2^27 for its gradients */
   const void* query;             /* [n, dim], rows query_stride elements apart */
   int64_t query_stride;
   const void* rows;              /* [vocab, dim] */

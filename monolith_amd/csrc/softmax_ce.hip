@@ -151,47 +151,48 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 || sizeof(T) == 2 ? 2
 template <typename T>
 __global__ __launch_bounds__(256) void k_ce_loss(Args a) {
   const int lane = threadIdx.x & 63;
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= a.n) return;
-  float m = neg_inf();
-  for (int s = lane; s < a.nsplit; s += 64) m = fmaxf(m, a.part[(int64_t)s * a.n + i]);
+  for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < a.n; i += (int64_t)gridDim.x * 4) {
+    float m = neg_inf();
+    for (int s = lane; s < a.nsplit; s += 64) m = fmaxf(m, a.part[(int64_t)s * a.n + i]);
 #pragma unroll
-  for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
-  float base = m == neg_inf() ? 0.f : m;
-  float z = 0.f;
-  for (int s = lane; s < a.nsplit; s += 64)
-    z += a.part2[(int64_t)s * a.n + i] * exp2_hw(a.part[(int64_t)s * a.n + i] - base);
+    for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+    float base = m == neg_inf() ? 0.f : m;
+    float z = 0.f;
+    for (int s = lane; s < a.nsplit; s += 64)
+      z += a.part2[(int64_t)s * a.n + i] * exp2_hw(a.part[(int64_t)s * a.n + i] - base);
 #pragma unroll
-  for (int x = 32; x; x >>= 1) z += __shfl_xor(z, x);
-  const int64_t label = a.labels[i];
-  const bool known = label >= 0 && label < a.v;
-  float hit = 0.f;
-  if (known)
-    for (int d = lane; d < a.D; d += 64)
-      hit = fmaf((float)((const T*)a.q)[i * a.qs + d], (float)((const T*)a.w)[label * a.ws + d], hit);
+    for (int x = 32; x; x >>= 1) z += __shfl_xor(z, x);
+    const int64_t label = a.labels[i];
+    const bool known = label >= 0 && label < a.v;
+    float hit = 0.f;
+    if (known)
+      for (int d = lane; d < a.D; d += 64)
+        hit = fmaf((float)((const T*)a.q)[i * a.qs + d], (float)((const T*)a.w)[label * a.ws + d], hit);
 #pragma unroll
-  for (int x = 32; x; x >>= 1) hit += __shfl_xor(hit, x);
-  if (lane) return;
-  const float b = known && a.bias ? a.bias[label] : 0.f;
-  float loss = label == -1 ? 0.f : __builtin_nanf(""), lse = __builtin_inff(), miss = 0.f;
-  if (b == neg_inf()) {
-    loss = __builtin_inff();
-  } else if (known) {
-    hit = fmaf(hit, a.scale2, floored(b) * kLog2e);
-    if (m == neg_inf()) base = hit;  // (there are no others)
-    const float d = hit - base, x = z * exp2_hw(-d);
-    if (d > -64.f) {
-      loss = log1pf(x);
-      miss = x / (1.f + x);
-    } else {  // (the 1 is less than a rounding of x, which may be beyond the largest number)
-      loss = (__log2f(z) - d) * kLn2 + (floored(b) - b);
-      miss = 1.f;
+    for (int x = 32; x; x >>= 1) hit += __shfl_xor(hit, x);
+    if (lane == 0) {
+      const float b = known && a.bias ? a.bias[label] : 0.f;
+      float loss = label == -1 ? 0.f : __builtin_nanf(""), lse = __builtin_inff(), miss = 0.f;
+      if (b == neg_inf()) {
+        loss = __builtin_inff();
+      } else if (known) {
+        hit = fmaf(hit, a.scale2, floored(b) * kLog2e);
+        if (m == neg_inf()) base = hit;  // (there are no others)
+        const float d = hit - base, x = z * exp2_hw(-d);
+        if (d > -64.f) {
+          loss = log1pf(x);
+          miss = x / (1.f + x);
+        } else {  // (the 1 is less than a rounding of x, which may be beyond the largest number)
+          loss = (__log2f(z) - d) * kLn2 + (floored(b) - b);
+          miss = x == x ? 1.f : x;
+        }
+        lse = d > 0.f ? hit + __log2f(1.f + x) : base + __log2f(z + exp2_hw(d));
+      }
+      a.loss[i] = loss;
+      a.lse[i] = lse;
+      a.lse[a.n + i] = miss;
     }
-    lse = d > 0.f ? hit + __log2f(1.f + x) : base + __log2f(z + exp2_hw(d));
   }
-  a.loss[i] = loss;
-  a.lse[i] = lse;
-  a.lse[a.n + i] = miss;
 }
 
 // ---- backward ------------------------------------------------------------------------------
@@ -493,6 +494,15 @@ Args base_args(const mono_softmax_ce_args* p) {
   return a;
 }
 
+// a gradient's launch has a workgroup for every 128 candidates or fewer beside the queries' ones, of 256 threads each:
+// fewer than 2^32 threads
+int check_grad(const mono_softmax_ce_args* p, const char* who) {
+  MONO_TRY(check(p, who));
+  MONO_REQUIRE((!p->grad_rows && !p->grad_bias) || p->vocab < (1LL << 31) - (1LL << 27),
+               "%s: the gradient of %lld rows is out of range", who, (long long)p->vocab);
+  return 0;
+}
+
 enum Which { kFwd, kBwd };
 template <int W, typename T, int DP, int NC>
 int launch1(const Args& a, hipStream_t st) {
@@ -546,7 +556,7 @@ int mono_softmax_cross_entropy(const mono_softmax_ce_args* p, void* stream) {
   a.part = (float*)p->workspace;
   a.part2 = (float*)((char*)p->workspace + round16((int64_t)a.nsplit * p->n * 4));
   MONO_TRY(launch<kFwd>(p->dtype, a, st));
-  const unsigned grid = (unsigned)((p->n + 3) / 4);
+  const int grid = grid_for(p->n, 4, 1 << 20);
   if (p->dtype == MONO_ROW_BF16) k_ce_loss<bf16><<<grid, 256, 0, st>>>(a);
   else k_ce_loss<float><<<grid, 256, 0, st>>>(a);
   MONO_HIP(hipGetLastError());
@@ -575,13 +585,13 @@ int64_t place_parts(const mono_softmax_ce_args* p, Args* a) {
 }  // namespace
 
 int64_t mono_softmax_cross_entropy_gradient_workspace(const mono_softmax_ce_args* p) {
-  if (check(p, "mono_softmax_cross_entropy_gradient_workspace")) return -1;
+  if (check_grad(p, "mono_softmax_cross_entropy_gradient_workspace")) return -1;
   Args a;
   return place_parts(p, &a);
 }
 
 int mono_softmax_cross_entropy_gradient(const mono_softmax_ce_args* p, void* stream) {
-  MONO_TRY(check(p, "mono_softmax_cross_entropy_gradient"));
+  MONO_TRY(check_grad(p, "mono_softmax_cross_entropy_gradient"));
   Args a = base_args(p);
   MONO_REQUIRE(p->rows && (p->n == 0 || (p->query && p->labels && p->lse && p->grad_loss)),
                "mono_softmax_cross_entropy_gradient: an array is NULL");

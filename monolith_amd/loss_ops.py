@@ -101,6 +101,8 @@ def softmax_cross_entropy(query: torch.Tensor, rows: torch.Tensor, labels: torch
                            bias.device != query.device):
     raise ValueError("%s: bias must be a float32 vector [%d] on %s" % (who, rows.shape[0],
                                                                       query.device))
+  if rows.shape[0] >= 2 ** 31 - 2 ** 27 and (rows.requires_grad or (bias is not None and bias.requires_grad)):
+    raise ValueError("%s: %d rows are too many for their gradient" % (who, rows.shape[0]))
   scale = float(scale)
   if not 1e-20 <= scale <= 1e20:
     raise ValueError("%s: scale must be in [1e-20, 1e20], got %r" % (who, scale))
