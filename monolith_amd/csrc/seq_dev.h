@@ -106,15 +106,17 @@ struct Rows {
 // one the rounded rest of those before: 24 bits, as many as x has. Of the nine products of two such
 // sums the six that reach 2^-24 of the whole are taken (hi hi, hi mid, mid hi, mid mid, hi lo, lo hi),
 // so a product is off by about 2^-25 of its size, less than the 32-bit sum it goes into, at 6/16 of the
-// fp32 matrix instructions' time. (An infinite element gives NaN; the hi of a number within 2^-9 of the
-// largest is infinite.)
+// fp32 matrix instructions' time. (An infinite element gives NaN. Rows are split with LARGE: a number within 2^-9
+// of the largest would round to an infinite hi.)
 template <typename T>
 constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
 
+template <bool LARGE = false>
 __device__ inline void split3(const float* x, int n, bf16* hi, bf16* mid, bf16* lo) {
+  constexpr float kMost = 0x1.fep127f;  // the largest bf16
 #pragma unroll
   for (int i = 0; i < n; ++i) {
-    hi[i] = (bf16)x[i];
+    hi[i] = (bf16)(LARGE ? __builtin_amdgcn_fmed3f(x[i], -kMost, kMost) : x[i]);
     const float r = x[i] - (float)hi[i];
     mid[i] = (bf16)r;
     lo[i] = (bf16)(r - (float)mid[i]);
@@ -179,7 +181,7 @@ struct Stage {
           const f4 x = __builtin_bit_cast(f4, w);
           const float v[4] = {x[0], x[1], x[2], x[3]};
           bf16 h[4], m[4], l[4];
-          split3(v, 4, h, m, l);
+          split3<true>(v, 4, h, m, l);
           *(bf4*)to = bf4{h[0], h[1], h[2], h[3]};
           *(bf4*)(to + PLANE) = bf4{m[0], m[1], m[2], m[3]};
           *(bf4*)(to + 2 * PLANE) = bf4{l[0], l[1], l[2], l[3]};
@@ -270,10 +272,11 @@ struct Mma {
         if (ok) c[1] = load_chunk(row, e0 + 4, D, vec);
         const f4 x = __builtin_bit_cast(f4, c[0]), y = __builtin_bit_cast(f4, c[1]);
         const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-        f[k] = frag(v);
+        f[k] = frag<true>(v);
       }
     }
   }
+  template <bool LARGE = false>
   static __device__ inline Frag frag(const float* v) {
     Frag f;
     if constexpr (PL == 1) {
@@ -281,7 +284,7 @@ struct Mma {
       for (int j = 0; j < 8; ++j) f.p[0][j] = (bf16)v[j];
     } else {
       bf16 h[8], m[8], l[8];
-      split3(v, 8, h, m, l);
+      split3<LARGE>(v, 8, h, m, l);
 #pragma unroll
       for (int j = 0; j < 8; ++j) f.p[0][j] = h[j], f.p[1][j] = m[j], f.p[2][j] = l[j];
     }

@@ -144,3 +144,27 @@ def test_gradients_refuse_tangents():
       with pytest.raises(ValueError, match="forward-mode"):
         torch.autograd.grad((out * weight).sum(), q)
       torch.autograd.grad(call().sum(), q)
+
+
+# ---- numbers near the largest --------------------------------------------------------------------
+def test_the_largest_finite_numbers():
+  """fp32 rows near the largest number against keys near the smallest: products of ordinary size."""
+  from monolith_amd import attention_ops, loss_ops
+  rng = np.random.default_rng(23)
+  big = float(np.finfo(np.float32).max)
+  n, D = 40, 16
+  x = np.sign(rng.standard_normal((n, D))) * big * (1 - rng.uniform(0, 2.0 ** -9, (n, D)))
+  y = np.exp2(-125 - rng.integers(0, 2, (n, D))) * np.sign(rng.standard_normal((n, D)))  # (no bits behind the first)
+  v, v64 = rows(rng, (n, 1, D), "fp32")
+  x, y = (t.astype(np.float32) for t in (x, y))
+  s = on(np.array([0, n]))
+  out = attention_ops.ragged_attention(on(x).unsqueeze(1), on(y).unsqueeze(1), v, s, s, scale=0.25)
+  x6, y6 = x.astype(np.float64), y.astype(np.float64)
+  segs = seq_ref.segments(np.array([0, n]), np.array([0, n]))
+  want = seq_ref.attention(x6[:, None], y6[:, None], v64, segs, seq_ref.keep_rule(segs, None, False), 0.25, "fp32")
+  seq_ref.check(out, want["out"], "out")
+  labels = rng.integers(0, n, n)
+  for a, b in ((x, y), (y, x)):
+    loss = loss_ops.softmax_cross_entropy(on(a), on(b), on(labels), None, 0.25)
+    want = seq_ref.cross_entropy(a.astype(np.float64), b.astype(np.float64), labels, None, 0.25, "fp32")
+    seq_ref.check(loss, want["loss"], "loss")
