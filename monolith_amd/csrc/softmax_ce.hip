@@ -57,7 +57,7 @@ __device__ inline void range_of(int n, int nsplit, int split, int BN, int* beg, 
 // 4096 queries against 1000003 rows of 64 bf16: 740 us, 5.5e12 logits a second; 8192 against 16385 rows of
 // 64 floats: 109 us.
 template <typename T, int DP, int NC>
-__global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 || sizeof(T) == 2 ? 2 : 1) void k_ce_fwd(Args a) {
+__global__ __launch_bounds__(256, DP <= 128 || sizeof(T) == 2 ? 2 : 1) void k_ce_fwd(Args a) {
   constexpr int BM = NC * 128, BN = Tile<T, DP>::BN, NR = Tile<T, DP>::NR;
   typedef Stage<T, DP, BN, 256> St;
   typedef Mma<T, DP, St::PLANE> M;
@@ -97,10 +97,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 || sizeof(T) == 2 ? 2
     if (tid < BN) lb[tid] = floored(eb) * inv_scale;  // what a candidate's products start from, in units of scale
     __syncthreads();
     if (y0 + BN < vend) fetch(y0 + BN);
-    bool mine = false;
+    uint32_t near = ~0u;  // (a label in front of the tile, or none, is far behind it as an unsigned number)
 #pragma unroll
-    for (int c = 0; c < NC; ++c) mine |= label[c] >= y0 && label[c] < y0 + BN;
-    const bool hits = __any(mine);
+    for (int c = 0; c < NC; ++c) near = min(near, (uint32_t)(label[c] - y0));
+    const bool hits = __any(near < BN);
     f16v s[NR][NC];
 #pragma unroll
     for (int rt = 0; rt < NR; ++rt) {
@@ -250,10 +250,10 @@ __device__ inline void query_half(const Args& a, int tile, int piece, bf16* lw, 
     if (tid < BN) lb[tid] = floored(eb) * inv_scale;  // what a candidate's products start from, in units of scale
     __syncthreads();
     if (y0 + BN < vend) fetch(y0 + BN);
-    bool mine = false;
+    uint32_t near = ~0u;  // (a label in front of the tile, or none, is far behind it as an unsigned number)
 #pragma unroll
-    for (int c = 0; c < NC; ++c) mine |= label[c] >= y0 && label[c] < y0 + BN;
-    const bool hits = __any(mine);
+    for (int c = 0; c < NC; ++c) near = min(near, (uint32_t)(label[c] - y0));
+    const bool hits = __any(near < BN);
 #pragma unroll
     for (int rt = 0; rt < NR; ++rt) {
       f16v s[NC];
