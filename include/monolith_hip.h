@@ -463,7 +463,10 @@ int mono_embedding_to_layout_grad(const mono_layout_slice* h_slices, int n_slice
  * non-decreasing, inside [0, rows]; rows in front of the first split and behind the last belong to
  * no sequence (their outputs and gradients are zero). Splits that break this give wrong values, but
  * no access outside the arrays. fp32 rows are multiplied as three bf16 numbers each (24 bits): elements
- * have to be finite where a query sees them, an infinite one gives NaN. Rows are [rows, heads, dim] with the last dimension contiguous. */
+ * have to be finite where a query sees them, an infinite one gives NaN. Weights of bf16 rows are rounded to
+ * bf16 for the products that they go into. The log-sums that the gradients read are 32-bit numbers: weights are
+ * off by 2^-23 of a logit's magnitude (scale times product, plus bias) of themselves, and where logits pass
+ * 2^31 results are NaN. Rows are [rows, heads, dim] with the last dimension contiguous. */
 enum { MONO_ROW_FP32 = 0, MONO_ROW_BF16 = 1 };
 typedef struct {
   const void* ptr;

@@ -9,10 +9,14 @@ head); the sequences of a batch lie one behind the other and are given by int64 
 Rows in front of the first split and behind the last (the padding of a fixed-size buffer) belong to
 no sequence: their outputs and gradients are zero. Splits that break this give wrong values, never
 an access outside the tensors. Softmax statistics and sums are held in 32 bits; results have the
-rows' type and are the same bit for bit from call to call. Elements that a query sees have to be finite
-(float32 rows are multiplied as three bfloat16 numbers each; an infinite element gives NaN). Nothing synchronises the host, and
-scratch memory comes from torch's allocator, so every op can be captured into a HIP graph. There is no
-forward-mode derivative: a tangent (torch.autograd.forward_ad) is refused."""
+rows' type and are the same bit for bit from call to call. Weights of bfloat16 rows are rounded to
+bfloat16 for the product with the values, as are the gradient's for its products. Elements that a query
+sees have to be finite (float32 rows are multiplied as three bfloat16 numbers each; an infinite element
+gives NaN). The log-sum that the gradient reads is a 32-bit number: its weights are off by
+2^-23 |scale * query . key| of themselves, and where that product passes 2^31 the softmax itself gives
+NaN. Nothing synchronises the host, and scratch memory comes from torch's allocator, so every op can be
+captured into a HIP graph. There is no forward-mode derivative: a tangent (torch.autograd.forward_ad) is
+refused."""
 import math
 from typing import Optional
 

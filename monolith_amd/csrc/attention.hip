@@ -114,9 +114,9 @@ __device__ inline void hide(f16v& s, int lim, const uint8_t* alive, float v, int
 // the vector unit's exponential, multiply-add, maximum and sum per logit beside 4 dim / 1024 matrix
 // instructions, and by the clock that the card keeps under such a load. Dense bf16 rows, 2048 keys, 64
 // elements: 610 TFLOP/s, 128 elements 800 (a library matrix product of 8192: 1133); fp32 183 (151). Ragged
-// causal rows (seq_train, 58602 rows of 8 x 64, 112 to 2048 a sequence): 189 us, 337 TFLOP/s: some five
-// tiles a workgroup, two of them on the diagonal, and four memory latencies before the first. (Sorting the
-// tiles by their work changed nothing.)
+// causal rows (58602 rows of 8 x 64, 112 to 2048 a sequence): 183 us, 347 TFLOP/s, and there neither unit is the
+// bound: vector unit 49% of the time, matrix unit 16%. Some five tiles a workgroup, two of them on the diagonal, and
+// four memory latencies before the first. (Sorting the tiles by their work changed nothing.)
 template <typename T, int DP, int NC, int NW>
 __global__ __launch_bounds__(NW * 64, DP * sizeof(T) <= 256 ? 2 : 1) void k_attn_fwd(Args a) {
   constexpr int BM = NC * NW * 32, BN = Tile<T, DP, NW, true>::BN, NR = Tile<T, DP, NW, true>::NR, NT = NW * 64;
@@ -387,7 +387,7 @@ __global__ __launch_bounds__(1024) void k_attn_join_many(const float* part, cons
 // ---- backward ------------------------------------------------------------------------------
 // dQ, then dK and dV: two passes that each make the logits again, 7 products instead of the 5 of one pass
 // that adds dQ up with atomics, but every sum has one order and the result is the same from call to call.
-// seq_train: 231 + 268 us, 450 TFLOP/s of executed products; 2048 keys without a mask: 660.
+// The same rows: 224 + 256 us, 463 and 593 TFLOP/s of executed products; 2048 keys without a mask: 660.
 //
 // dQ: the forward's tiles again. With p = exp2(s - lse) from the forward's statistics and
 // delta = g.o, ds = p (g.v - delta), dq = scale sum ds k. Also writes delta for the pass over keys. A bf16
@@ -987,8 +987,12 @@ struct Shape {
   int nc, nw, bm;
 };
 // Short sequences (64 rows of a key head or fewer on average) leave most of a 128-row tile empty: one
-// wave with 32 columns per workgroup then. (fp32 rows of more than 32 elements: a tile's way to LDS
-// alone would take a wave's registers.)
+// wave with 32 columns per workgroup then. 49152 causal rows of 8 heads in sequences of random length, forward and
+// with its gradient, one wave against four: bf16 of 64 elements, 32 rows on average 55 us against 106 and 316 against
+// 481, 64 rows 55 against 80 and 331 against 393, 128 rows 63 against 75 and 371 against 387, 192 rows 73 against 79 and
+// 413 against 402; fp32 of 32 elements 77 against 140 and 294 against 616, 81 against 103 and 307 against 459, 107
+// against 106 and 387 against 464, 137 against 120 and 486 against 525. (fp32 rows of more than 32 elements: a tile's
+// way to LDS alone would take a wave's registers.)
 Shape shape_for(int dtype, int D, double rows_per_seq) {
   if (rows_per_seq <= 64 && (dtype == MONO_ROW_BF16 || D <= 32)) return {1, 1, 32};
   return {1, 4, 128};
@@ -1080,7 +1084,9 @@ double average(int64_t n, int64_t B) { return (double)n / std::max<int64_t>(1, B
 // fills the card's 4096 waves where few sequences are long on average (equal numbers of parts left the
 // longest of pool_lifelong's 7 histories of 9411 to 120000 keys alone at the end, 36 us for 28). One history
 // of 100000 keys among 16384 of 40: 84 us and 97 for the gradient, 2993 and 5467 if one wave walks it; where
-// there is none the look costs 4 us each way. No more keys than one chunk in all: nothing to cut. Behind a prefix, whose parts are joined in any case: equal parts.
+// there is none the look costs 4 us each way. No more keys than one chunk in all: nothing to cut. Behind a prefix,
+// whose parts are joined in any case: equal parts by the average length, so that one candidate with a very long history
+// of its own among many short ones is one wave's walk there, as it is one tile's in the tile kernels.
 bool is_pool(const mono_attention_args* p) { return !p->query_splits && p->heads / p->kv_heads <= 4; }
 Plan plan_pool(const mono_attention_args* p, bool equal) {
   Plan pl{};

@@ -104,9 +104,9 @@ struct Rows {
 
 // fp32 rows go through the bf16 matrix instructions as three bf16 numbers each, x = hi + mid + lo, every
 // one the rounded rest of those before: 24 bits, as many as x has. Of the nine products of two such
-// sums the six that reach 2^-24 of the whole are taken (hi hi, hi mid, mid hi, mid mid, hi lo, lo hi),
-// so a product is off by about 2^-25 of its size, less than the 32-bit sum it goes into, at 6/16 of the
-// fp32 matrix instructions' time. (An infinite element gives NaN. Rows are split with LARGE: a number within 2^-9
+// sums six are taken (hi hi, hi mid, mid hi, mid mid, hi lo, lo hi), at 6/16 of the fp32 matrix instructions'
+// time. The three left out are 2^-27.4 of a product in the mean square of normal numbers, a tenth of one fp32
+// rounding, and 2^-23 at worst: mid is up to 2^-8 of x and lo 2^-16, both at once in 1 + 2^-8 + 2^-16. (An infinite element gives NaN. Rows are split with LARGE: a number within 2^-9
 // of the largest would round to an infinite hi.)
 template <typename T>
 constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
@@ -311,8 +311,10 @@ struct Mma {
     return __builtin_bit_cast(bf4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p));
   }
   // acc[dt][c] += sum over the 32 rows from 32 rt on of Z[y][32 dt + ..] P[y][x]. For bf16 rows P is
-  // rounded to bf16 here: half a step of 2^-8 of every weight, independent from weight to weight, beside
-  // the one rounding of the result to the same type.
+  // rounded to bf16 here, the one type that the matrix instructions multiply with the rows as they are: up to 2^-8 of
+  // every weight, independent from weight to weight, beside the one rounding of the result to the same type (results
+  // 2.4e-3 off 64 bits in the root mean square, of which their own rounding is 1.7e-3). A caller who wants more bits
+  // takes fp32 rows.
   template <int NC>
   static __device__ inline void accumulate(const bf16* lds, int rt, const f16v (&p)[NC], f16v (&acc)[NDT][NC],
                                            int lane) {

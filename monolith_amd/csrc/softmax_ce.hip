@@ -54,8 +54,8 @@ __device__ inline void range_of(int n, int nsplit, int split, int BN, int* beg, 
 // A tile of 128 or (bf16 rows of 64 elements or less: two column
 // tiles a wave, half the LDS reads of a product) 256 queries stays in registers, the candidates stream.
 // Bound by the vector unit: an exponential, a multiply-add, a sum and half a maximum for each logit.
-// 4096 queries against 1000003 rows of 64 bf16: 740 us, 5.5e12 logits a second; 8192 against 16385 rows of
-// 64 floats: 109 us.
+// 4096 queries against 1000003 rows of 64 bf16: 770 us, 5.3e12 logits a second, the vector unit at work 85% of the
+// time; 8192 against 16385 rows of 64 floats: 111 us.
 template <typename T, int DP, int NC>
 __global__ __launch_bounds__(256, DP <= 128 || sizeof(T) == 2 ? 2 : 1) void k_ce_fwd(Args a) {
   constexpr int BM = NC * 128, BN = Tile<T, DP>::BN, NR = Tile<T, DP>::NR;
@@ -394,10 +394,11 @@ __device__ inline void rows_half(const Args& a, int tile, int piece, bf16* lq, f
   }
 }
 
-// Both halves of the gradient in one launch: they share nothing, the queries' half first. 2.27 ms for 4096
-// queries against 1000003 rows of 64 bf16, 0.92 PFLOP/s of executed products where a library matrix product
-// of 8192 reaches 1.13: with operands that are not random but zeros the same loop takes half the time, so
-// it is the card's power that bounds it. 415 us for 8192 against 16385 rows of 64 floats.
+// Both halves of the gradient in one launch: they share nothing, the queries' half first. 2.15 ms for 4096
+// queries against 1000003 rows of 64 bf16, 0.98 PFLOP/s of executed products where a library matrix product
+// of 8192 reaches 1.13: with operands that are not random but zeros the same loop takes half the time, and the clock
+// falls to 1.75 GHz, so it is the card's power that bounds it. 410 us for 8192 against 16385 rows of 64 floats.
+// (Rows of 32 elements or less: three waves a SIMD, for which pieces_of cuts; 169 registers without the bound.)
 template <typename T, int DP, int NC>
 __global__ __launch_bounds__(256, DP <= 32 ? 3 : DP * sizeof(T) <= 256 ? 2 : 1) void k_ce_bwd(Args a) {
   constexpr int BN = Tile<T, DP>::BN;

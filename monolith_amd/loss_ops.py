@@ -4,8 +4,10 @@ of the rows goes to HashTable.apply_gradients, and the bias takes the correction
 candidate is drawn (what a table under entry.BatchSoftmaxOptimizer estimates). No counterpart in
 the reference's op set.
 
-The logits [n, vocab] never exist in memory. Sums and statistics are held in 32 bits; results are the
-same bit for bit from call to call. Nothing synchronises the host and scratch memory comes from
+The logits [n, vocab] never exist in memory. Sums and statistics are held in 32 bits; in the gradient of bfloat16 rows
+the probabilities, the label's p - 1 in the rows' gradient among them, are rounded to bfloat16 for the products. Rows
+are to be finite. The log-sum that the gradient reads is a 32-bit number: its probabilities are off by 2^-23 |logit| of
+themselves, and where logits pass 2^31 the loss is NaN. Results are the same bit for bit from call to call. Nothing synchronises the host and scratch memory comes from
 torch's allocator, so loss and gradient can be captured into a HIP graph. There is no forward-mode
 derivative: a tangent (torch.autograd.forward_ad) is refused."""
 from typing import Optional

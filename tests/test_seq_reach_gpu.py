@@ -133,3 +133,19 @@ def test_broken_splits_stay_inside(dtype, heads, form, nk):
                       backward=(True, ao._rows(g), dq.data_ptr(), dk.data_ptr(), 0)))
     torch.cuda.synchronize()
     room.check()
+
+
+@pytest.mark.parametrize("D", [16, 128])
+def test_worst_products_of_fp32_rows(D):
+  """x = 1 + 2^-8 + 2^-16 has three bf16 parts of one bit each, and what the six products of x * x leave out is
+  2 * 2^-24 of it, in every element the same way: a logit of D of them is 2^-23 too small and rounds at most D + 8
+  times on the way to the loss, log(1 + exp(l)) = l for an l of more than 17 below a candidate of zeros."""
+  from monolith_amd import loss_ops
+  x = 1 + 2.0 ** -8 + 2.0 ** -16
+  q = torch.full((40, D), x, device=dev())
+  w = torch.zeros(2, D, device=dev())
+  w[0] = x
+  want = D * x * x * 2  # (scale 2; exp(-32) is under 2^-46)
+  loss = loss_ops.softmax_cross_entropy(q, w, torch.ones(40, dtype=torch.int64, device=dev()), scale=2.0).double()
+  off = (loss / want - 1).abs().max().item()
+  assert off <= 2.0 ** -23 + (D + 8) * seq_ref.U32, off
