@@ -106,8 +106,9 @@ struct Rows {
 // one the rounded rest of those before: 24 bits, as many as x has. Of the nine products of two such
 // sums six are taken (hi hi, hi mid, mid hi, mid mid, hi lo, lo hi), at 6/16 of the fp32 matrix instructions'
 // time. The three left out are 2^-27.4 of a product in the mean square of normal numbers, a tenth of one fp32
-// rounding, and 2^-23 at worst: mid is up to 2^-8 of x and lo 2^-16, both at once in 1 + 2^-8 + 2^-16. (An infinite element gives NaN. Rows are split with LARGE: a number within 2^-9
-// of the largest would round to an infinite hi.)
+// rounding, and 2^-23 at worst: mid is up to 2^-8 of x and lo 2^-16, both at once in 1 + 2^-8 + 2^-16. (An
+// infinite element gives NaN. Rows are split with LARGE: a number within 2^-9 of the largest would round to an
+// infinite hi.)
 template <typename T>
 constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
 

@@ -149,3 +149,33 @@ def test_worst_products_of_fp32_rows(D):
   loss = loss_ops.softmax_cross_entropy(q, w, torch.ones(40, dtype=torch.int64, device=dev()), scale=2.0).double()
   off = (loss / want - 1).abs().max().item()
   assert off <= 2.0 ** -23 + (D + 8) * seq_ref.U32, off
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("scale", [1e-20, 1e20])
+def test_scales_at_their_ends(dtype, scale):
+  """Rows that much larger or smaller, so that the logits are ordinary: the bounds do not depend on the scale."""
+  from monolith_amd import attention_ops, loss_ops
+  rng = np.random.default_rng(3)
+  size = scale ** -0.5
+  lens = [50, 90]
+  s = on(splits(lens))
+  segs = seq_ref.segments(splits(lens), splits(lens))
+  q, q64 = rows(rng, (140, 2, 16), dtype, size)
+  k, k64 = rows(rng, (140, 1, 16), dtype, size)
+  v, v64 = rows(rng, (140, 1, 16), dtype)
+  g, g64 = rows(rng, (140, 2, 16), dtype)
+  leaves = [t.requires_grad_() for t in (q, k, v)]
+  out = attention_ops.ragged_attention(*leaves, s, s, scale=scale)
+  want = seq_ref.attention(q64, k64, v64, segs, seq_ref.keep_rule(segs, None, False), scale, dtype, g64)
+  for got, name in zip([out] + list(torch.autograd.grad(out, leaves, g)), ("out", "dq", "dk", "dv")):
+    seq_ref.check(got, want[name], name)
+  w, w64 = rows(rng, (300, 16), dtype, size)
+  labels, bias = rng.integers(0, 300, 140), rng.standard_normal(300).astype(np.float32)
+  b = on(bias).requires_grad_()
+  leaves = [q[:, 0].detach().requires_grad_(), w.requires_grad_(), b]
+  loss = loss_ops.softmax_cross_entropy(leaves[0], w, on(labels), b, scale)
+  gl = rng.standard_normal(140).astype(np.float32)
+  want = seq_ref.cross_entropy(q64[:, 0], w64, labels, bias.astype(np.float64), scale, dtype, gl.astype(np.float64))
+  for got, name in zip([loss] + list(torch.autograd.grad(loss, leaves, on(gl))), ("loss", "dq", "dw", "db")):
+    seq_ref.check(got, want[name], name)
